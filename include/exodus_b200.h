@@ -394,6 +394,83 @@ int exb_leaky_forward_scan_static(float *out, const float *input, const float *v
                                   float *v_last,
                                   int64_t B, int64_t T, int64_t M, int device, void *stream);
 
+/* ------------------------------------------------------------------ sequence operators
+ *
+ * Selective scan (a leaky integrator whose decay, input weight and readout depend on the input), the short causal
+ * convolution in front of it and the group norm with an activation on channels-last tensors.  No counterpart in the
+ * reference, whose recurrences have decays that are fixed in time.
+ *
+ * These take float32, bfloat16 and float16 tensors (`dtype`) and views: element (b, t, c) of a tensor lies at
+ * data + b*stride_b + t*stride_t + c, so a slice of a wider projection is used where it lies.  Outputs are contiguous.
+ * Parameters, states and all sums are float32 unless stated otherwise.  A NULL view, or one whose data is NULL, is an
+ * absent tensor.  `lengths` (NULL: T for all) holds B numbers of valid steps, clamped to 0 ... T; rows behind them do
+ * not enter anything, whatever they hold: their outputs and gradients are 0 and the state passes them unchanged.
+ * Workspaces are scratch: they need not be cleared and hold nothing between calls; calls that may run at the same time
+ * need one each. */
+enum { EXB_F32 = 0, EXB_BF16 = 1, EXB_F16 = 2 };
+enum { EXB_ACT_NONE = 0, EXB_ACT_SILU = 1, EXB_ACT_RELU = 2 };
+
+typedef struct { void *data; int64_t stride_b, stride_t; } exb_rows;
+
+/* Selective scan over M channels with N states each; B and C are shared by the M/G channels of a group:
+ *     s_t = softplus(dt_t + dt_bias)   (without softplus: dt_t + dt_bias)
+ *     h_t[m,n] = exp(s_t[m] A[m,n]) h_{t-1}[m,n] + s_t[m] x_t[m] B_t[g,n]
+ *     y_t[m]   = (sum_n C_t[g,n] h_t[m,n] + D[m] x_t[m]) * silu(z_t[m])
+ * x, dt, z: (B, T, M); B, C: (B, T, G, N) with contiguous (G, N); A: (M, N); D, dt_bias: (M); h0, h_last: (B, M, N).
+ * D, z, dt_bias and h0 may be absent.  `ckpt` (optional in the forward pass, required by the backward pass, 16-byte
+ * aligned): exb_selective_checkpoint_floats(...) floats that keep the state every EXB_SELECTIVE_CHECKPOINT steps. */
+#define EXB_SELECTIVE_MAX_STATES 128
+#define EXB_SELECTIVE_CHECKPOINT 8
+int64_t exb_selective_checkpoint_floats(int64_t B, int64_t T, int64_t M, int64_t N);
+int64_t exb_selective_workspace_bytes(int64_t B, int64_t T, int64_t M, int64_t N, int64_t G, int backward);
+int exb_selective_forward(void *y, float *h_last, float *ckpt, const exb_rows *x, const exb_rows *dt, const float *A,
+                          const exb_rows *Bm, const exb_rows *Cm, const float *D, const exb_rows *z, const float *dt_bias,
+                          const float *h0, const int32_t *lengths, int softplus, void *workspace, int64_t workspace_bytes,
+                          int dtype, int64_t B, int64_t T, int64_t M, int64_t N, int64_t G, int device, void *stream);
+/* All gradients in one reverse sweep.  dh_last: gradient of h_last (NULL: none).  dz is required with z; dD, ddt_bias
+ * and dh0 may be NULL.  dB, dC: (B, T, G, N) contiguous.  Sums over batch, time and channels run in a fixed order. */
+int exb_selective_backward(void *dx, void *ddt, float *dA, void *dB, void *dC, float *dD, void *dz, float *ddt_bias, float *dh0,
+                           const exb_rows *dy, const float *dh_last, const float *ckpt, const exb_rows *x, const exb_rows *dt,
+                           const float *A, const exb_rows *Bm, const exb_rows *Cm, const float *D, const exb_rows *z,
+                           const float *dt_bias, const int32_t *lengths, int softplus, void *workspace,
+                           int64_t workspace_bytes, int dtype, int64_t B, int64_t T, int64_t M, int64_t N, int64_t G,
+                           int device, void *stream);
+/* One step; h (B, M, N), batch items h_stride floats apart, is updated in place.  stride_t of the views is not used. */
+int exb_selective_step(void *y, float *h, int64_t h_stride, const exb_rows *x, const exb_rows *dt, const float *A,
+                       const exb_rows *Bm, const exb_rows *Cm, const float *D, const exb_rows *z, const float *dt_bias,
+                       int softplus, int dtype, int64_t B, int64_t M, int64_t N, int64_t G, int device, void *stream);
+
+/* Causal convolution along time with one filter of W <= 8 steps per channel:
+ *     y_t[m] = act(bias[m] + sum_k weight[m,k] x_{t-W+1+k}[m])
+ * The rows in front of x are `state` (B, W-1, M) or zeros; `last` receives the W-1 rows that the next call starts from.
+ * weight (M, W) and bias (M) are float32 with params_f32 != 0, else of type `dtype`; so are their gradients. */
+int64_t exb_causal_conv_workspace_bytes(int64_t B, int64_t T, int64_t M, int64_t W);
+int exb_causal_conv_forward(void *y, void *last, const exb_rows *x, const void *weight, const void *bias, const void *state,
+                            const int32_t *lengths, int activation, int params_f32, int dtype, int64_t B, int64_t T,
+                            int64_t M, int64_t W, int device, void *stream);
+int exb_causal_conv_backward(void *dx, void *dweight, void *dbias, void *dstate, const exb_rows *dy, const void *dlast,
+                             const exb_rows *x, const void *weight, const void *bias, const void *state,
+                             const int32_t *lengths, int activation, int params_f32, void *workspace,
+                             int64_t workspace_bytes, int dtype, int64_t B, int64_t T, int64_t M, int64_t W, int device,
+                             void *stream);
+/* One step; state (batch items state_stride elements apart) is shifted by one row in place. */
+int exb_causal_conv_step(void *y, void *state, int64_t state_stride, const exb_rows *x, const void *weight, const void *bias,
+                         int activation, int params_f32, int dtype, int64_t B, int64_t M, int64_t W, int device,
+                         void *stream);
+
+/* Group norm on (R samples, S positions, C channels), channels last:
+ *     y = act((x - mean) * rstd * weight + bias),  rstd = 1 / sqrt(var + eps)
+ * over the S positions and C/G <= 16384 channels of a group; weight and bias (C) may be NULL, float32 with
+ * params_f32 != 0, else of type `dtype`.  mean, rstd: (R, G), written by the forward pass and read by the backward. */
+int64_t exb_group_norm_workspace_bytes(int64_t R, int64_t S, int64_t C, int64_t G, int dtype, int backward);
+int exb_group_norm_forward(void *y, float *mean, float *rstd, const exb_rows *x, const void *weight, const void *bias,
+                           float eps, int activation, int params_f32, void *workspace, int64_t workspace_bytes, int dtype,
+                           int64_t R, int64_t S, int64_t C, int64_t G, int device, void *stream);
+int exb_group_norm_backward(void *dx, void *dweight, void *dbias, const exb_rows *dy, const exb_rows *x, const float *mean,
+                            const float *rstd, const void *weight, const void *bias, int activation, int params_f32,
+                            void *workspace, int64_t workspace_bytes, int dtype, int64_t R, int64_t S, int64_t C, int64_t G,
+                            int device, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,7 +8,13 @@ Public surface (same names as the reference's ``sinabs.exodus`` package):
 * ``conversion``  -- ``sinabs_to_exodus``, ``exodus_to_sinabs``, ``module_map``
 
 Beyond the reference: ``GraphedStep`` (``graphs``) captures a whole forward(+backward) step of a
-network of these layers in a CUDA graph.
+network of these layers in a CUDA graph.  Sequence operators, with ``layers.SelectiveLeak`` and
+``layers.GroupNorm`` built on them:
+
+* ``selective_scan`` / ``selective_step`` -- leaky integrator whose decay, input weight and readout depend on the
+  input, for prompts (differentiable) and single tokens
+* ``causal_conv`` / ``causal_conv_step``  -- short causal convolution per channel, likewise
+* ``group_norm``                          -- group norm with an activation on channels-last tensors
 
 All computation runs in ``libexodus_b200.so`` (hand-written CUDA for sm_100a,
 C ABI in ``include/exodus_b200.h``).  There is no PyTorch or CPU fallback: a
@@ -22,6 +28,7 @@ __version__ = "0.1.0"
 
 from . import _lib  # noqa: E402
 from . import leaky, spike  # noqa: E402
+from . import convolution, normalization, selective  # noqa: E402
 from . import layers  # noqa: E402
 from . import conversion  # noqa: E402
 from . import graphs  # noqa: E402
@@ -29,6 +36,9 @@ from .graphs import GraphedStep  # noqa: E402
 from ._lib import device_status, set_nvtx_ranges, set_status_checks  # noqa: E402
 from .leaky import LeakyIntegrator, LeakyIntegratorTM  # noqa: E402
 from .spike import IntegrateAndFire, IntegrateAndFireTM, LIFSynapticTM  # noqa: E402
+from .selective import SelectiveScanTM, selective_scan, selective_step  # noqa: E402
+from .convolution import CausalConvTM, causal_conv, causal_conv_step  # noqa: E402
+from .normalization import GroupNormCL, group_norm  # noqa: E402
 
 
 def install_as_sinabs_exodus() -> None:

@@ -44,7 +44,16 @@ EXPORTS = (
     "exb_lif_forward", "exb_lif_forward_record", "exb_lif_forward_u8", "exb_lif_syn_forward_u8", "exb_lif_backward", "exb_lif_forward_ckpt", "exb_lif_backward_ckpt", "exb_leaky_forward", "exb_leaky_backward",
     "exb_leaky_scan_workspace_bytes", "exb_leaky_forward_scan", "exb_leaky_backward_scan",
     "exb_leaky_forward_scan_static", "exb_static_scratch_bytes", "exb_lif_syn_forward", "exb_lif_syn_backward",
+    "exb_selective_checkpoint_floats", "exb_selective_workspace_bytes", "exb_selective_forward", "exb_selective_backward",
+    "exb_selective_step", "exb_causal_conv_workspace_bytes", "exb_causal_conv_forward", "exb_causal_conv_backward",
+    "exb_causal_conv_step", "exb_group_norm_workspace_bytes", "exb_group_norm_forward", "exb_group_norm_backward",
 )
+
+
+class Rows(ctypes.Structure):
+    """``exb_rows``: element (b, t, c) of a tensor at ``data + b*stride_b + t*stride_t + c``."""
+
+    _fields_ = [("data", _vp), ("stride_b", _i64), ("stride_t", _i64)]
 
 
 class ExodusLibraryError(RuntimeError):
@@ -124,6 +133,35 @@ def load() -> ctypes.CDLL:
     lib.exb_static_scratch_bytes.argtypes = []
     lib.exb_leaky_forward_scan_static.restype = _i
     lib.exb_leaky_forward_scan_static.argtypes = [_vp, _vp, _vp, _vp, _i, _vp, _i, _vp, _i64, _i64, _i64, _i, _vp]
+    # sequence operators
+    rows = ctypes.POINTER(Rows)
+    lib.exb_selective_checkpoint_floats.restype = _i64
+    lib.exb_selective_checkpoint_floats.argtypes = [_i64] * 4
+    lib.exb_selective_workspace_bytes.restype = _i64
+    lib.exb_selective_workspace_bytes.argtypes = [_i64] * 5 + [_i]
+    lib.exb_selective_forward.restype = _i
+    lib.exb_selective_forward.argtypes = ([_vp] * 3 + [rows, rows, _vp, rows, rows, _vp, rows, _vp, _vp, _vp, _i, _vp, _i64, _i]
+                                          + [_i64] * 5 + [_i, _vp])
+    lib.exb_selective_backward.restype = _i
+    lib.exb_selective_backward.argtypes = ([_vp] * 9 + [rows, _vp, _vp, rows, rows, _vp, rows, rows, _vp, rows, _vp, _vp, _i, _vp,
+                                                       _i64, _i] + [_i64] * 5 + [_i, _vp])
+    lib.exb_selective_step.restype = _i
+    lib.exb_selective_step.argtypes = [_vp, _vp, _i64, rows, rows, _vp, rows, rows, _vp, rows, _vp, _i, _i] + [_i64] * 4 + [_i, _vp]
+    lib.exb_causal_conv_workspace_bytes.restype = _i64
+    lib.exb_causal_conv_workspace_bytes.argtypes = [_i64] * 4
+    lib.exb_causal_conv_forward.restype = _i
+    lib.exb_causal_conv_forward.argtypes = [_vp, _vp, rows] + [_vp] * 4 + [_i] * 3 + [_i64] * 4 + [_i, _vp]
+    lib.exb_causal_conv_backward.restype = _i
+    lib.exb_causal_conv_backward.argtypes = ([_vp] * 4 + [rows, _vp, rows] + [_vp] * 4 + [_i, _i, _vp, _i64, _i] + [_i64] * 4
+                                             + [_i, _vp])
+    lib.exb_causal_conv_step.restype = _i
+    lib.exb_causal_conv_step.argtypes = [_vp, _vp, _i64, rows, _vp, _vp, _i, _i, _i] + [_i64] * 3 + [_i, _vp]
+    lib.exb_group_norm_workspace_bytes.restype = _i64
+    lib.exb_group_norm_workspace_bytes.argtypes = [_i64] * 4 + [_i, _i]
+    lib.exb_group_norm_forward.restype = _i
+    lib.exb_group_norm_forward.argtypes = [_vp] * 3 + [rows, _vp, _vp, _f, _i, _i, _vp, _i64, _i] + [_i64] * 4 + [_i, _vp]
+    lib.exb_group_norm_backward.restype = _i
+    lib.exb_group_norm_backward.argtypes = ([_vp] * 3 + [rows, rows] + [_vp] * 4 + [_i, _i, _vp, _i64, _i] + [_i64] * 4 + [_i, _vp])
     _lib = lib
     return lib
 
@@ -527,11 +565,123 @@ def lif_syn_backward(grad_input, grad_alpha_mem, grad_scale_mem, grad_alpha_syn,
     _after_launch(dev)
 
 
+# ---- sequence operators (selective.py, convolution.py, normalization.py check shapes and types) ----
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+ACTIVATIONS = {None: 0, "silu": 1, "relu": 2}
+SELECTIVE_MAX_STATES = 128
+CONV_MAX_WIDTH = 8
+NORM_MAX_GROUP = 16384
+
+
+def rows_of(t: Optional[torch.Tensor]):
+    """View of a (B, T, ...) or (B, ...) tensor whose trailing dimensions are contiguous; None passes through."""
+    if t is None:
+        return None
+    if t.ndim > 2:
+        return Rows(t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0)
+    return Rows(t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0, 0)
+
+
+def _workspace(nbytes: int, dev: torch.device) -> Tuple[Optional[torch.Tensor], int]:
+    return (torch.empty(nbytes, dtype=torch.uint8, device=dev), nbytes) if nbytes > 0 else (None, 0)
+
+
+def selective_checkpoint(B: int, T: int, M: int, N: int, dev: torch.device) -> torch.Tensor:
+    return torch.empty(int(load().exb_selective_checkpoint_floats(B, T, M, N)), dtype=torch.float32, device=dev)
+
+
+def selective_forward(y, h_last, ckpt, x, dt, A, Bm, Cm, D, z, dt_bias, h0, lengths, softplus: bool, B: int, T: int, M: int,
+                      N: int, G: int) -> None:
+    lib, dev = load(), x.device
+    ws, nbytes = _workspace(int(lib.exb_selective_workspace_bytes(B, T, M, N, G, 0)), dev)
+    st = lib.exb_selective_forward(ptr(y), ptr(h_last), ptr(ckpt), rows_of(x), rows_of(dt), ptr(A), rows_of(Bm), rows_of(Cm), ptr(D),
+                                   rows_of(z), ptr(dt_bias), ptr(h0), ptr(lengths), int(softplus), ptr(ws), nbytes, DTYPES[x.dtype],
+                                   B, T, M, N, G, dev.index, _stream(dev))
+    _check(st, "exb_selective_forward")
+    _after_launch(dev)
+
+
+def selective_backward(dx, ddt, dA, dB, dC, dD, dz, ddt_bias, dh0, dy, dh_last, ckpt, x, dt, A, Bm, Cm, D, z, dt_bias, lengths,
+                       softplus: bool, B: int, T: int, M: int, N: int, G: int) -> None:
+    lib, dev = load(), x.device
+    ws, nbytes = _workspace(int(lib.exb_selective_workspace_bytes(B, T, M, N, G, 1)), dev)
+    st = lib.exb_selective_backward(ptr(dx), ptr(ddt), ptr(dA), ptr(dB), ptr(dC), ptr(dD), ptr(dz), ptr(ddt_bias), ptr(dh0),
+                                    rows_of(dy), ptr(dh_last), ptr(ckpt), rows_of(x), rows_of(dt), ptr(A), rows_of(Bm), rows_of(Cm),
+                                    ptr(D), rows_of(z), ptr(dt_bias), ptr(lengths), int(softplus), ptr(ws), nbytes, DTYPES[x.dtype],
+                                    B, T, M, N, G, dev.index, _stream(dev))
+    _check(st, "exb_selective_backward")
+    _after_launch(dev)
+
+
+def selective_step(y, h, x, dt, A, Bm, Cm, D, z, dt_bias, softplus: bool, B: int, M: int, N: int, G: int) -> None:
+    dev = x.device
+    st = load().exb_selective_step(y.data_ptr(), h.data_ptr(), h.stride(0), rows_of(x), rows_of(dt), A.data_ptr(), rows_of(Bm),
+                                   rows_of(Cm), ptr(D), rows_of(z), ptr(dt_bias), int(softplus), DTYPES[x.dtype], B, M, N, G,
+                                   dev.index, _stream(dev))
+    _check(st, "exb_selective_step")
+    _after_launch(dev)
+
+
+def causal_conv_forward(y, last, x, weight, bias, state, lengths, activation, B: int, T: int, M: int, W: int) -> None:
+    dev = x.device
+    st = load().exb_causal_conv_forward(ptr(y), ptr(last), rows_of(x), ptr(weight), ptr(bias), ptr(state), ptr(lengths),
+                                        ACTIVATIONS[activation], int(weight.dtype == torch.float32), DTYPES[x.dtype], B, T, M, W,
+                                        dev.index, _stream(dev))
+    _check(st, "exb_causal_conv_forward")
+    _after_launch(dev)
+
+
+def causal_conv_backward(dx, dweight, dbias, dstate, dy, dlast, x, weight, bias, state, lengths, activation, B: int, T: int, M: int,
+                         W: int) -> None:
+    lib, dev = load(), x.device
+    ws, nbytes = _workspace(int(lib.exb_causal_conv_workspace_bytes(B, T, M, W)), dev)
+    st = lib.exb_causal_conv_backward(ptr(dx), ptr(dweight), ptr(dbias), ptr(dstate), rows_of(dy), ptr(dlast), rows_of(x), ptr(weight),
+                                      ptr(bias), ptr(state), ptr(lengths), ACTIVATIONS[activation],
+                                      int(weight.dtype == torch.float32), ptr(ws), nbytes, DTYPES[x.dtype], B, T, M, W, dev.index,
+                                      _stream(dev))
+    _check(st, "exb_causal_conv_backward")
+    _after_launch(dev)
+
+
+def causal_conv_step(y, state, x, weight, bias, activation, B: int, M: int, W: int) -> None:
+    dev = x.device
+    st = load().exb_causal_conv_step(y.data_ptr(), state.data_ptr(), state.stride(0), rows_of(x), weight.data_ptr(), ptr(bias),
+                                     ACTIVATIONS[activation], int(weight.dtype == torch.float32), DTYPES[x.dtype], B, M, W, dev.index,
+                                     _stream(dev))
+    _check(st, "exb_causal_conv_step")
+    _after_launch(dev)
+
+
+def group_norm_forward(y, mean, rstd, x, weight, bias, eps: float, activation, R: int, S: int, C: int, G: int) -> None:
+    lib, dev = load(), x.device
+    f32 = weight is None or weight.dtype == torch.float32
+    ws, nbytes = _workspace(int(lib.exb_group_norm_workspace_bytes(R, S, C, G, DTYPES[x.dtype], 0)), dev)
+    st = lib.exb_group_norm_forward(ptr(y), ptr(mean), ptr(rstd), rows_of(x), ptr(weight), ptr(bias), float(eps),
+                                    ACTIVATIONS[activation], int(f32), ptr(ws), nbytes, DTYPES[x.dtype], R, S, C, G, dev.index,
+                                    _stream(dev))
+    _check(st, "exb_group_norm_forward")
+    _after_launch(dev)
+
+
+def group_norm_backward(dx, dweight, dbias, dy, x, mean, rstd, weight, bias, activation, R: int, S: int, C: int, G: int) -> None:
+    lib, dev = load(), x.device
+    f32 = weight is None or weight.dtype == torch.float32
+    ws, nbytes = _workspace(int(lib.exb_group_norm_workspace_bytes(R, S, C, G, DTYPES[x.dtype], 1)), dev)
+    st = lib.exb_group_norm_backward(ptr(dx), ptr(dweight), ptr(dbias), rows_of(dy), rows_of(x), ptr(mean), ptr(rstd), ptr(weight),
+                                     ptr(bias), ACTIVATIONS[activation], int(f32), ptr(ws), nbytes, DTYPES[x.dtype], R, S, C, G,
+                                     dev.index, _stream(dev))
+    _check(st, "exb_group_norm_backward")
+    _after_launch(dev)
+
+
 # Tracing aid: NVTX ranges around the calls that launch kernels, named after the entry point, so that a timeline
 # shows which layer call a kernel belongs to.  Off unless asked for (a range costs a few microseconds per call).
 _LAUNCHERS = ("lif_forward", "lif_forward_u8", "lif_forward_ckpt", "lif_backward", "lif_backward_ckpt", "leaky_forward",
               "leaky_backward", "leaky_forward_scan", "leaky_backward_scan", "leaky_forward_scan_static",
-              "lif_syn_forward", "lif_syn_forward_u8", "lif_syn_backward", "acc_finish", "allreduce_oneshot")
+              "lif_syn_forward", "lif_syn_forward_u8", "lif_syn_backward", "acc_finish", "allreduce_oneshot",
+              "selective_forward", "selective_backward", "selective_step", "causal_conv_forward", "causal_conv_backward",
+              "causal_conv_step", "group_norm_forward", "group_norm_backward")
 _nvtx_on = False
 
 

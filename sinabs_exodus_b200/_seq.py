@@ -1,0 +1,72 @@
+"""Argument checks shared by the sequence operators (``selective``, ``convolution``, ``normalization``)."""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+
+
+def require_data(name: str, x: torch.Tensor) -> None:
+    """The main input of an operator: a tensor of a type that the kernels take."""
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"'{name}' must be a tensor, got {type(x).__name__}")
+    if x.dtype not in _lib.DTYPES:
+        raise ValueError(f"'{name}' must be float32, bfloat16 or float16, got {x.dtype}")
+
+
+def require_cuda(name: str, x: torch.Tensor) -> None:
+    """Comes last: shapes and types are checked wherever the tensors are."""
+    if not x.is_cuda:
+        raise _lib.ExodusLibraryError(
+            f"exodus_b200 kernels only run on CUDA tensors; '{name}' is on {x.device}. There is no CPU implementation in this package.")
+
+
+def require_like(name: str, t: Optional[torch.Tensor], shape: Tuple[int, ...], dtypes: Tuple[torch.dtype, ...],
+                 device: torch.device) -> None:
+    if t is None:
+        return
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"'{name}' must be a tensor, got {type(t).__name__}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"'{name}' must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.dtype not in dtypes:
+        raise ValueError(f"'{name}' must be {' or '.join(str(d).replace('torch.', '') for d in dtypes)}, got {t.dtype}")
+    if t.device != device:
+        raise _lib.ExodusLibraryError(f"tensors on different devices: {device} and {t.device} ('{name}')")
+
+
+def check_lengths(lengths: Optional[torch.Tensor], batch: int, device: torch.device) -> Optional[torch.Tensor]:
+    if lengths is None:
+        return None
+    require_like("lengths", lengths, (batch,), (torch.int32, torch.int64), device)
+    return lengths.to(torch.int32).contiguous()
+
+
+def channels_contiguous(t: Optional[torch.Tensor], trailing: int = 1) -> Optional[torch.Tensor]:
+    """``t`` with its last ``trailing`` dimensions contiguous: itself where they are, else a copy."""
+    if t is None:
+        return None
+    step = 1
+    for d in range(t.ndim - 1, t.ndim - 1 - trailing, -1):
+        if t.shape[d] > 1 and t.stride(d) != step:
+            return t.contiguous()
+        step *= t.shape[d]
+    return t
+
+
+def dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return None if t is None else t.contiguous()
+
+
+def refuse_grad(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """The in-place single-token forms are not differentiable."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} updates its state in place and is not differentiable: call it under torch.no_grad()")
+
+
+def mark_changed(t: torch.Tensor) -> None:
+    """Tells autograd that a kernel wrote to ``t``."""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)

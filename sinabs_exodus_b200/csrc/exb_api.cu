@@ -8,11 +8,16 @@
 #include <cstring>
 #include <cstdlib>
 
+#include "exb_host.cuh"
 #include "exb_kernels.cuh"
 
 namespace {
 
 thread_local char g_err[512] = "";
+
+}  // namespace
+
+namespace exb {
 
 int fail(int code, const char *fmt, ...)
 {
@@ -23,23 +28,12 @@ int fail(int code, const char *fmt, ...)
     return code;
 }
 
-// Makes `device` current for the duration of one entry point and restores the
-// previous device afterwards (the reference calls cudaSetDevice without
-// restoring, cuda/bindings.cu:45).
-struct DeviceGuard {
-    int prev = -1;
-    bool ok = true;
-    explicit DeviceGuard(int device)
-    {
-        if (cudaGetDevice(&prev) != cudaSuccess) { ok = false; return; }
-        if (device >= 0 && device != prev && cudaSetDevice(device) != cudaSuccess) ok = false;
-    }
-    ~DeviceGuard()
-    {
-        int cur = -1;
-        if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
-    }
-};
+}  // namespace exb
+
+namespace {
+
+using exb::DeviceGuard;
+using exb::fail;
 
 // Shape in the low bits; the derived-parameter bits only where they mean something: IS_TAU on a decay
 // argument, the SCALE bits on a scale argument.

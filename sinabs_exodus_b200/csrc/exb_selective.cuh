@@ -1,0 +1,68 @@
+// Arguments of the selective scan's kernels and its launchers.
+#pragma once
+
+#include "exb_seq_common.cuh"
+
+namespace exb {
+
+constexpr int SEL_CHUNK = EXB_SELECTIVE_CHECKPOINT;      // steps between two checkpoints of the state
+
+struct SelArgs {
+    View x, dt, z, Bm, Cm;               // z.p may be null
+    const float *A, *D, *dt_bias, *h0;   // [M][N], [M], [M], [B][M][N]; all but A may be null
+    const int32_t *lengths;              // [B] or null
+    int64_t B, T;
+    int M, N, G;
+    int softplus;
+    // forward
+    void *y;                             // contiguous
+    float *h_last;                       // [B][M][N]
+    float *ckpt;                         // [B][ceil(T / SEL_CHUNK)][M][NP], or null
+    // backward
+    View dy;
+    const float *dh_last;                // [B][M][N] or null
+    void *dx, *ddt, *dz;                 // contiguous
+    float *dh0;                          // [B][M][N] or null
+    float *part_bc;                      // [tiles][B][T][G][2][NP]
+    float *part_a;                       // [B * segments][M][NP]
+    float *part_d;                       // [B * segments][2][M]   (D, dt_bias)
+    // time split: `segments` pieces of `seg` steps; state (or gradient) entering each piece
+    int segments;
+    int64_t seg;
+    float *seg_h;                        // [B][segments][M][NP]
+    float *seg_dt;                       // [B][segments][M]
+};
+
+// Lanes per channel: four states in each.
+inline int sel_lanes(int N)
+{
+    int l = 1;
+    while (4 * l < N) l *= 2;
+    return l;
+}
+inline int sel_channels(int L) { return L == 1 ? 128 : 256 / L; }      // channels of a block
+
+struct SelPlan {
+    int L, NP, CC, tiles, segments;
+    int64_t seg, chunks;
+    int64_t off_h, off_dt, off_bc, off_a, off_d, bytes;      // offsets into the workspace
+};
+SelPlan sel_plan(int64_t B, int64_t T, int M, int N, int G, bool backward);
+
+cudaError_t launch_selective_forward(SelArgs a, int dtype, void *ws, cudaStream_t stream);
+cudaError_t launch_selective_backward(SelArgs a, int dtype, void *dB, void *dC, float *dA, float *dD, float *dbias, void *ws,
+                                      cudaStream_t stream);
+
+struct SelStepArgs {
+    View x, dt, z, Bm, Cm;               // st unused
+    const float *A, *D, *dt_bias;
+    float *h;                            // [B][M][N], updated
+    int64_t sh;                          // elements between two batch items of h
+    void *y;                             // [B][M]
+    int64_t B;
+    int M, N, G;
+    int softplus;
+};
+cudaError_t launch_selective_step(const SelStepArgs &a, int dtype, cudaStream_t stream);
+
+}  // namespace exb

@@ -1,0 +1,89 @@
+"""Group norm with an activation on channels-last tensors::
+
+    y = act((x - mean) * rstd * weight + bias)
+
+with mean and variance over all positions of a sample and the channels of a group.  ``(samples, *positions, channels)``:
+a ``channels_last`` feature map, or tokens ``(samples, channels)`` with one position each.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib, _seq
+
+__all__ = ["GroupNormCL", "group_norm"]
+
+
+class GroupNormCL(torch.autograd.Function):
+    """``apply(x, num_groups, weight, bias, eps, activation) -> y`` on (samples, positions, channels); see
+    :func:`group_norm`, which checks the arguments."""
+
+    @staticmethod
+    def forward(ctx, x, num_groups, weight, bias, eps, activation):
+        R, S, C = x.shape
+        x = _seq.channels_contiguous(x)
+        weight, bias = _seq.dense(weight), _seq.dense(bias)
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        mean = torch.empty(R, num_groups, dtype=torch.float32, device=x.device)
+        rstd = torch.empty_like(mean)
+        if R * S * C:
+            _lib.group_norm_forward(y, mean, rstd, x, weight, bias, eps, activation, R, S, C, num_groups)
+        ctx.num_groups, ctx.activation = num_groups, activation
+        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, mean, rstd = ctx.saved_tensors
+        R, S, C = x.shape
+        empty = R * S * C == 0
+        new = torch.zeros_like if empty else torch.empty_like
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dweight = new(weight) if weight is not None else None
+        dbias = new(bias) if bias is not None else None
+        if not empty:
+            _lib.group_norm_backward(dx, dweight, dbias, _seq.channels_contiguous(dy), x, mean, rstd, weight, bias, ctx.activation, R, S,
+                                     C, ctx.num_groups)
+        return dx, None, dweight, dbias, None, None
+
+
+def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5, activation: Optional[str] = None) -> torch.Tensor:
+    """Group norm of a channels-last tensor; differentiable.
+
+    Parameters
+    ----------
+    x: (samples, *positions, channels), float32, bfloat16 or float16; at most 16384 channels per group.
+    num_groups: divides the channels.
+    weight, bias: (channels,) float32 or the type of ``x``, both of one type; each may be absent.
+    eps: added to the variance.
+    activation: None, "silu" or "relu".
+
+    Returns the normalised tensor, contiguous, of the shape and type of ``x``.
+    """
+    _seq.require_data("x", x)
+    if x.ndim < 2:
+        raise ValueError("'x' must have at least 2 dimensions, (samples, ..., channels)")
+    C = x.shape[-1]
+    if not isinstance(num_groups, int) or num_groups < 1 or C % num_groups:
+        raise ValueError(f"'num_groups' must divide the {C} channels, got {num_groups!r}")
+    if C // num_groups > _lib.NORM_MAX_GROUP:
+        raise ValueError(f"at most {_lib.NORM_MAX_GROUP} channels in a group are supported, got {C // num_groups}")
+    if activation not in _lib.ACTIVATIONS:
+        raise ValueError(f"'activation' must be None, 'silu' or 'relu', got {activation!r}")
+    if not eps >= 0.0:
+        raise ValueError(f"'eps' must not be negative, got {eps}")
+    _seq.require_like("weight", weight, (C,), (torch.float32, x.dtype), x.device)
+    _seq.require_like("bias", bias, (C,), (torch.float32, x.dtype), x.device)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError(f"'weight' and 'bias' must have one type, got {weight.dtype} and {bias.dtype}")
+    _seq.require_cuda("x", x)
+    positions = 1
+    for n in x.shape[1:-1]:
+        positions *= n
+    y = GroupNormCL.apply(x.reshape(x.shape[0], positions, C), num_groups, weight, bias, float(eps), activation)
+    return y.reshape(x.shape)
