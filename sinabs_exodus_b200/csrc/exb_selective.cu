@@ -16,14 +16,9 @@ template <int L> struct Geo {
     static constexpr int CC = L == 1 ? 128 : 256 / L;
     static constexpr int NT = CC * L;
     static constexpr int NP = 4 * L;
-    static constexpr int COLS = CC / 4;      // four-channel packs of a row
+    static constexpr int WARPS = NT / 32;
+    static constexpr int KF = L == 1 ? 8 : 16;      // steps of a chunk in the forward direction
 };
-
-__device__ __forceinline__ float step_size(float dt, float bias, int softplus)
-{
-    const float v = dt + bias;
-    return (softplus && v <= 20.0f) ? log1pf(expf(v)) : v;      // beyond 20 the difference is below 2^-31 of the value
-}
 
 // Which tile, piece of time and batch item a block works on.
 struct Where {
@@ -77,146 +72,438 @@ __device__ __forceinline__ void store_states(float *p, const float (&v)[4], int 
     }
 }
 
-// Stages rows t0 .. t0 + K of B (and C) of one group as float, zero beyond `steps` rows and N columns.
-template <typename T, int NT, int NP, int K>
-__device__ __forceinline__ void stage_group(float *dst, const View &v, int64_t b, int64_t t0, int steps, int g, int N)
+// Rates, kept finite: an infinite one times the step size 0 of a row behind the sequence would not be the 0 it stands for.
+__device__ __forceinline__ void load_rates(float (&v)[4], const float *p, int n0, int N)
 {
-    const T *base = static_cast<const T *>(v.p) + b * v.sb + (int64_t)g * N;
-    for (int i = threadIdx.x; i < K * NP; i += NT) {
-        const int t = i / NP, n = i % NP;
-        dst[i] = (t < steps && n < N) ? to_f32(base[(t0 + t) * v.st + n]) : 0.0f;
+    load_states(v, p, n0, N);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = min_nan(max_nan(v[j], -2.0e38f), 2.0e38f);
+}
+
+// Two kinds of warps.  The first NT threads of a block run the recurrence; NH more prepare its inputs and take its
+// results away.  They meet at one barrier per chunk of K steps: while the recurrence runs through chunk k, the others
+// store chunk k - 1's results, prepare chunk k + 1 and have chunk k + 2 on its way from memory.  A training problem has
+// few channels for the size of the GPU (8192 channels are two recurrence warps on each scheduler), so the elementwise
+// work, which has long chains of dependent instructions, must not stand between two of their steps.
+template <int THREADS>
+__device__ __forceinline__ void meet()
+{
+    asm volatile("bar.sync 0, %0;" ::"n"(THREADS) : "memory");
+}
+
+// The elementwise work of a chunk of K steps on CC channels by NH threads: packs of V channels, ITEMS per thread, all of
+// a thread in the same columns (its channels' D and dt_bias stay in registers).
+template <int K, int CC, int NH> struct Items {
+    static constexpr int V = K * CC / NH >= 4 ? 4 : 2;
+    static constexpr int COLS = CC / V;
+    static constexpr int ROWS = NH / COLS;      // rows between two items of a thread
+    static constexpr int ITEMS = (K + ROWS - 1) / ROWS;
+    static_assert(NH % COLS == 0, "");
+};
+
+// A block's piece of the problem.
+template <int K, int CC>
+struct Block {
+    Where w;
+    int per;                        // channels of a group
+    int64_t t_lo, t_hi, t_end;      // its steps; those that belong to the sequence end at t_end
+    int64_t count;                  // chunks
+
+    __device__ __forceinline__ explicit Block(const SelArgs &a)
+    {
+        w = locate<CC>(a);
+        per = a.M / a.G;
+        const int64_t len = sequence_length(a, w.b);
+        t_lo = w.seg * a.seg;
+        t_hi = t_lo + a.seg < a.T ? t_lo + a.seg : a.T;
+        t_end = t_hi < len ? t_hi : len;
+        count = t_end > t_lo ? (t_end - t_lo + K - 1) / K : 0;
+    }
+    __device__ __forceinline__ int64_t time(int64_t k) const { return t_lo + k * K; }
+    __device__ __forceinline__ int steps(int64_t k) const { return t_end - time(k) < K ? (int)(t_end - time(k)) : K; }
+};
+
+// A preparing thread's part of a chunk.
+template <int K, int CC, int NH>
+struct Part {
+    using I = Items<K, CC, NH>;
+    static constexpr int V = I::V;
+    int row, col, ch, left;      // first row, column, channel and number of channels of its packs
+
+    __device__ __forceinline__ Part(const Block<K, CC> &b, int thread)
+    {
+        row = thread / I::COLS;
+        col = thread % I::COLS * V;
+        ch = b.w.g * b.per + b.w.ch0 + col;
+        left = b.per - (b.w.ch0 + col);
+    }
+    // Number of the pack's channels that exist in row `r` of a chunk of `steps` rows (0 or less: none).
+    __device__ __forceinline__ int there(int steps, int r) const { return r < steps ? left : 0; }
+
+    template <typename T, bool VEC>
+    __device__ __forceinline__ void fetch(RawPack<T, V, VEC> (&p)[I::ITEMS], const View &v, const Block<K, CC> &b, int64_t k) const
+    {
+        const T *at = static_cast<const T *>(v.p) + b.w.b * v.sb + (b.time(k) + row) * v.st + ch;
+        const int steps = b.steps(k);
+#pragma unroll
+        for (int i = 0; i < I::ITEMS; ++i, at += I::ROWS * v.st) p[i].load(at, there(steps, row + i * I::ROWS));
+    }
+    __device__ __forceinline__ void channel_values(float (&v)[V], const float *p) const
+    {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = (p && j < left) ? p[ch + j] : 0.0f;
+    }
+};
+
+// Step sizes of a pack; channels and rows that do not exist get 0, which changes no state.
+template <typename R, int V>
+__device__ __forceinline__ void step_sizes(float (&d)[V], float (&pre)[V], const R &raw, const float (&bias)[V], int softplus, int have)
+{
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+        pre[j] = raw.get(j) + bias[j];
+        pre[j + 1] = raw.get(j + 1) + bias[j + 1];
+        float2 s = make_float2(pre[j], pre[j + 1]);
+        if (softplus) s = softplus2(s);
+        d[j] = j < have ? s.x : 0.0f;
+        d[j + 1] = j + 1 < have ? s.y : 0.0f;
     }
 }
 
-// ---------------------------------------------------------------------------------------------- forward
+// Rows of B or C of one group: fetched as they are, and left in shared memory as float, 0 beyond the sequence and N.
+// COPIES of each row, the i-th with column n at n ^ i (see the backward kernel).
+template <typename T, int K, int CC, int NP, int NH, int COPIES = 1>
+struct GroupRows {
+    static constexpr int ITEMS = (K * NP + NH - 1) / NH;
+    RawPack<T, 1, false> r[ITEMS];
 
-constexpr int KF = 16;      // steps staged at a time
-
-// STATE_ONLY: the state a piece of time ends with when it starts from zero, and its sum of step sizes.
-template <typename T, int L, bool VEC, bool STATE_ONLY>
-__global__ void __launch_bounds__(Geo<L>::NT) sel_forward_kernel(const SelArgs a)
-{
-    using Q = Geo<L>;
-    constexpr int CC = Q::CC, NT = Q::NT, NP = Q::NP, COLS = Q::COLS;
-    constexpr int GS = L < SEL_CHUNK ? L : SEL_CHUNK;      // steps whose readouts are summed over the lanes together
-    __shared__ float2 s_in[KF * CC];         // dt, dt * x
-    __shared__ float s_b[KF * NP], s_c[STATE_ONLY ? 4 : KF * NP];
-    __shared__ float s_y[STATE_ONLY ? 4 : KF * CC];
-    const Where w = locate<CC>(a);
-    const int per = a.M / a.G;
-    const int tid = threadIdx.x, c = tid / L, l = tid % L, n0 = 4 * l;
-    const bool alive = w.ch0 + c < per;
-    const int m = w.g * per + w.ch0 + c;
-    const int64_t len = sequence_length(a, w.b);
-    const int64_t t_lo = w.seg * a.seg, t_hi = t_lo + a.seg < a.T ? t_lo + a.seg : a.T;
-    const int64_t t_end = t_hi < len ? t_hi : len;
-    const int64_t nchunks = (a.T + SEL_CHUNK - 1) / SEL_CHUNK;
-
-    float A2[4] = {0.f, 0.f, 0.f, 0.f}, h[4] = {0.f, 0.f, 0.f, 0.f};
-    if (alive) {
-        load_states(A2, a.A + (int64_t)m * a.N, n0, a.N);
+    __device__ __forceinline__ void fetch(const Block<K, CC> &b, const View &v, int N, int64_t k, int thread)
+    {
+        const T *base = static_cast<const T *>(v.p) + b.w.b * v.sb + b.time(k) * v.st + (int64_t)b.w.g * N;
+        const int steps = b.steps(k);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) A2[j] *= LOG2E;
-        if (!STATE_ONLY) {
-            if (a.segments > 1) load_states(h, a.seg_h + ((w.b * a.segments + w.seg) * a.M + m) * NP, n0, NP);
-            else if (a.h0) load_states(h, a.h0 + (w.b * a.M + m) * a.N, n0, a.N);
+        for (int i = 0; i < ITEMS; ++i) {
+            const int e = thread + i * NH, t = e / NP, n = e % NP;
+            r[i].load(base + t * v.st + n, (t < steps && n < N) ? 1 : 0);
         }
     }
-    float dt_sum = 0.0f;
-
-    for (int64_t tc = t_lo; tc < t_end; tc += KF) {
-        const int steps = t_end - tc < KF ? (int)(t_end - tc) : KF;
-        __syncthreads();      // the previous chunk's readouts have been taken
-        for (int i = tid; i < KF * COLS; i += NT) {
-            const int row = i / COLS, col = (i % COLS) * 4;
-            const int left = row < steps ? per - (w.ch0 + col) : 0;
-            const int ch = w.g * per + w.ch0 + col;
-            Pack<T, 4> px, pd;
-            load_pack<VEC>(px, static_cast<const T *>(a.x.p) + w.b * a.x.sb + (tc + row) * a.x.st + ch, left);
-            load_pack<VEC>(pd, static_cast<const T *>(a.dt.p) + w.b * a.dt.sb + (tc + row) * a.dt.st + ch, left);
+    __device__ __forceinline__ void stage(float *dst, int thread) const
+    {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float d = 0.0f, u = 0.0f;
-                if (j < left) {
-                    d = step_size(to_f32(pd.v[j]), a.dt_bias ? a.dt_bias[ch + j] : 0.0f, a.softplus);
-                    u = d * to_f32(px.v[j]);
-                }
-                s_in[row * CC + col + j] = make_float2(d, u);
+        for (int i = 0; i < ITEMS; ++i) {
+            const int e = thread + i * NH, t = e / NP, n = e % NP;
+            if (t < K) {
+#pragma unroll
+                for (int q = 0; q < COPIES; ++q) dst[(t * COPIES + q) * NP + (n ^ q)] = r[i].get(0);
             }
         }
-        stage_group<T, NT, NP, KF>(s_b, a.Bm, w.b, tc, steps, w.g, a.N);
-        if (!STATE_ONLY) stage_group<T, NT, NP, KF>(s_c, a.Cm, w.b, tc, steps, w.g, a.N);
-        __syncthreads();
+    }
+};
+
+// Where a channel's 16 bytes lie in a row: a preparing thread writes four neighbouring channels one after the other, so
+// neighbouring packs use the places in different orders, which halves the bank conflicts of those stores.
+__device__ __forceinline__ int place_of(int c) { return c ^ ((c >> 2) & 3); }
+
+__device__ __forceinline__ float2 low(const float4 &v) { return make_float2(v.x, v.y); }
+__device__ __forceinline__ float2 high(const float4 &v) { return make_float2(v.z, v.w); }
+
+// Four states of a lane as two pairs.
+struct Quad {
+    float2 q[2];
+    __device__ __forceinline__ void set(const float (&v)[4]) { q[0] = make_float2(v[0], v[1]); q[1] = make_float2(v[2], v[3]); }
+    __device__ __forceinline__ void get(float (&v)[4]) const { v[0] = q[0].x; v[1] = q[0].y; v[2] = q[1].x; v[3] = q[1].y; }
+};
+
+// ---------------------------------------------------------------------------------------------- forward
+
+constexpr int NH_FORWARD = 256;
+
+template <int L>
+constexpr int forward_smem_bytes()
+{
+    using Q = Geo<L>;
+    return (int)sizeof(float) * 2 * (Q::KF * Q::CC * 7 + 2 * Q::KF * Q::NP);
+}
+
+template <typename T, int L, bool VEC>
+__global__ void __launch_bounds__(Geo<L>::NT + NH_FORWARD) sel_forward_kernel(const SelArgs a)
+{
+    using Q = Geo<L>;
+    constexpr int K = Q::KF, CC = Q::CC, NT = Q::NT, NP = Q::NP, NH = NH_FORWARD;
+    extern __shared__ float smem[];
+    float4 *s_in = reinterpret_cast<float4 *>(smem);       // [2][K][CC]: dt twice, dt x twice (pairs as the arithmetic takes them)
+    float *s_skip = smem + 8 * K * CC, *s_gate = s_skip + 2 * K * CC;      // [2][K][CC]: D x, silu(z)
+    float *s_y = s_gate + 2 * K * CC;                      // [2][K][CC]
+    float *s_b = s_y + 2 * K * CC, *s_c = s_b + 2 * K * NP;      // [2][K][NP]
+    const Block<K, CC> blk(a);
+
+    if (threadIdx.x >= NT) {
+        using P = Part<K, CC, NH>;
+        constexpr int V = P::V, ITEMS = P::I::ITEMS, ROWS = P::I::ROWS;
+        const int tid = threadIdx.x - NT;
+        const P part(blk, tid);
+        float skip[V], bias[V];
+        part.channel_values(skip, a.D);
+        part.channel_values(bias, a.dt_bias);
+        struct Raw {
+            RawPack<T, V, VEC> x[ITEMS], dt[ITEMS], z[ITEMS];
+            GroupRows<T, K, CC, NP, NH> b, c;
+        } raw[2];
+        auto fetch = [&](Raw &f, int64_t k) {
+            if (k >= blk.count) return;
+            part.fetch(f.x, a.x, blk, k);
+            part.fetch(f.dt, a.dt, blk, k);
+            if (a.z.p) part.fetch(f.z, a.z, blk, k);
+            f.b.fetch(blk, a.Bm, a.N, k, tid);
+            f.c.fetch(blk, a.Cm, a.N, k, tid);
+        };
+        auto stage = [&](const Raw &f, int64_t k) {
+            if (k >= blk.count) return;
+            const int buf = (int)(k & 1) * K * CC, steps = blk.steps(k);
 #pragma unroll
-        for (int t0 = 0; t0 < KF; t0 += GS) {
-            if (!STATE_ONLY && a.ckpt && t0 % SEL_CHUNK == 0 && t0 < steps && alive)
-                store_states(a.ckpt + ((w.b * nchunks + (tc + t0) / SEL_CHUNK) * a.M + m) * NP, h, n0, NP);
+            for (int i = 0; i < ITEMS; ++i) {
+                const int r = part.row + i * ROWS, at = buf + r * CC + part.col;
+                if (r >= K) continue;
+                float d[V], pre[V];
+                step_sizes(d, pre, f.dt[i], bias, a.softplus, part.there(steps, r));
+                Pack<float, V> sk, ga;
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float x = f.x[i].get(j), u = d[j] * x;
+                    s_in[buf + r * CC + place_of(part.col + j)] = make_float4(d[j], d[j], u, u);
+                    sk.v[j] = skip[j] * x;
+                    ga.v[j] = a.z.p ? silu_f(f.z[i].get(j)) : 1.0f;
+                }
+                *reinterpret_cast<Pack<float, V> *>(s_skip + at) = sk;
+                *reinterpret_cast<Pack<float, V> *>(s_gate + at) = ga;
+            }
+            f.b.stage(s_b + (k & 1) * K * NP, tid);
+            f.c.stage(s_c + (k & 1) * K * NP, tid);
+        };
+        auto emit = [&](int64_t k) {
+            if (k < 0) return;
+            const int buf = (int)(k & 1) * K * CC, steps = blk.steps(k);
+            T *to = static_cast<T *>(a.y) + (blk.w.b * a.T + blk.time(k) + part.row) * a.M + part.ch;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i, to += ROWS * (int64_t)a.M) {
+                const int r = part.row + i * ROWS, have = part.there(steps, r), at = buf + r * CC + part.col;
+                if (have <= 0) continue;
+                const Pack<float, V> y = *reinterpret_cast<const Pack<float, V> *>(s_y + at), sk = *reinterpret_cast<const Pack<float, V> *>(s_skip + at),
+                                     ga = *reinterpret_cast<const Pack<float, V> *>(s_gate + at);
+                Pack<T, V> out;
+#pragma unroll
+                for (int j = 0; j < V; ++j) out.v[j] = from_f32<T>((y.v[j] + sk.v[j]) * ga.v[j]);
+                store_pack<VEC>(to, out, have);
+            }
+        };
+        fetch(raw[0], 0);
+        fetch(raw[1], 1);
+        stage(raw[0], 0);
+        fetch(raw[0], 2);
+        for (int64_t k = 0; k < blk.count; k += 2) {
+            meet<NT + NH>();
+            emit(k - 1);
+            stage(raw[1], k + 1);
+            fetch(raw[1], k + 3);
+            if (k + 1 >= blk.count) break;
+            meet<NT + NH>();
+            emit(k);
+            stage(raw[0], k + 2);
+            fetch(raw[0], k + 4);
+        }
+        meet<NT + NH>();
+        emit(blk.count - 1);
+        // rows behind the sequence
+        const int64_t z_lo = blk.t_end > blk.t_lo ? blk.t_end : blk.t_lo;
+        for (int64_t i = tid; i < (blk.t_hi - z_lo) * CC; i += NH) {
+            const int ch = blk.w.ch0 + (int)(i % CC);
+            if (ch < blk.per) static_cast<T *>(a.y)[(blk.w.b * a.T + z_lo + i / CC) * a.M + blk.w.g * blk.per + ch] = from_f32<T>(0.0f);
+        }
+        return;
+    }
+
+    constexpr int GS = L < SEL_CHUNK ? L : SEL_CHUNK;      // steps whose readouts are summed over the lanes together
+    const int tid = threadIdx.x, c = tid / L, l = tid % L, n0 = 4 * l;
+    const bool alive = blk.w.ch0 + c < blk.per;
+    const int m = blk.w.g * blk.per + blk.w.ch0 + c;
+    const int64_t nchunks = (a.T + SEL_CHUNK - 1) / SEL_CHUNK;
+    Quad A2, h;
+    {
+        float r[4] = {0.f, 0.f, 0.f, 0.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
+        if (alive) {
+            load_rates(r, a.A + (int64_t)m * a.N, n0, a.N);
+            if (a.segments > 1) load_states(s, a.seg_h + ((blk.w.b * a.segments + blk.w.seg) * a.M + m) * NP, n0, NP);
+            else if (a.h0) load_states(s, a.h0 + (blk.w.b * a.M + m) * a.N, n0, a.N);
+        }
+        A2.set(r);
+        h.set(s);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) A2.q[q] = mul2(A2.q[q], both(LOG2E));
+    }
+    float *ckpt = a.ckpt ? a.ckpt + ((blk.w.b * nchunks + blk.t_lo / SEL_CHUNK) * a.M + m) * NP : nullptr;
+    for (int64_t k = 0; k < blk.count; ++k) {
+        meet<NT + NH>();
+        const float4 *in = s_in + (k & 1) * K * CC + place_of(c);
+        const float *b = s_b + (k & 1) * K * NP + n0, *cc = s_c + (k & 1) * K * NP + n0;
+        float *y = s_y + (k & 1) * K * CC + c;
+        const int steps = blk.steps(k);
+#pragma unroll
+        for (int t0 = 0; t0 < K; t0 += GS) {
+            if (t0 % SEL_CHUNK == 0 && ckpt) {
+                if (alive && t0 < steps) *reinterpret_cast<float4 *>(ckpt + n0) = make_float4(h.q[0].x, h.q[0].y, h.q[1].x, h.q[1].y);
+                ckpt += (int64_t)a.M * NP;
+            }
             float v[GS];
 #pragma unroll
             for (int i = 0; i < GS; ++i) {
                 const int t = t0 + i;
-                v[i] = 0.0f;
-                if (t < steps) {
-                    const float2 in = s_in[t * CC + c];
-                    const float4 b4 = *reinterpret_cast<const float4 *>(s_b + t * NP + n0);
-                    const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
-                    float cc[4] = {0.f, 0.f, 0.f, 0.f};
-                    if (!STATE_ONLY) {
-                        const float4 c4 = *reinterpret_cast<const float4 *>(s_c + t * NP + n0);
-                        cc[0] = c4.x; cc[1] = c4.y; cc[2] = c4.z; cc[3] = c4.w;
-                    } else {
-                        dt_sum += in.x;
-                    }
+                const float4 d4 = in[t * CC];
+                const float4 b4 = *reinterpret_cast<const float4 *>(b + t * NP), c4 = *reinterpret_cast<const float4 *>(cc + t * NP);
+                const float2 bb[2] = {low(b4), high(b4)}, ccv[2] = {low(c4), high(c4)};
+                float2 sum;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        h[j] = fmaf(exp2_fast(in.x * A2[j]), h[j], in.y * bb[j]);
-                        if (!STATE_ONLY) v[i] = fmaf(cc[j], h[j], v[i]);
-                    }
+                for (int q = 0; q < 2; ++q) {
+                    const float2 e = mul2(low(d4), A2.q[q]);
+                    h.q[q] = fma2(make_float2(exp2_fast(e.x), exp2_fast(e.y)), h.q[q], mul2(high(d4), bb[q]));
+                    sum = q ? fma2(ccv[q], h.q[q], sum) : mul2(ccv[q], h.q[q]);
                 }
+                v[i] = sum.x + sum.y;
             }
-            if (!STATE_ONLY) {
-                reduce_scatter<GS, L, 1>(v, tid);
-                if (writes_total<GS, L>(l)) s_y[(t0 + first_of<GS, L>(l)) * CC + c] = v[0];
-            }
-        }
-        if (STATE_ONLY) continue;
-        __syncthreads();
-        for (int i = tid; i < KF * COLS; i += NT) {
-            const int row = i / COLS, col = (i % COLS) * 4;
-            const int left = row < steps ? per - (w.ch0 + col) : 0;
-            const int ch = w.g * per + w.ch0 + col;
-            if (left <= 0) continue;
-            Pack<T, 4> px, pz, out;
-            load_pack<VEC>(px, static_cast<const T *>(a.x.p) + w.b * a.x.sb + (tc + row) * a.x.st + ch, left);
-            if (a.z.p) load_pack<VEC>(pz, static_cast<const T *>(a.z.p) + w.b * a.z.sb + (tc + row) * a.z.st + ch, left);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float y = s_y[row * CC + col + j];
-                if (j < left && a.D) y = fmaf(a.D[ch + j], to_f32(px.v[j]), y);
-                if (a.z.p) y *= silu_f(to_f32(pz.v[j]));
-                out.v[j] = from_f32<T>(y);
-            }
-            store_pack<VEC>(static_cast<T *>(a.y) + (w.b * a.T + tc + row) * a.M + ch, out, left);
+            reduce_scatter<GS, L, 1>(v, tid);
+            if (writes_total<GS, L>(l)) y[(t0 + first_of<GS, L>(l)) * CC] = v[0];
         }
     }
-    if (STATE_ONLY) {
-        if (alive) {
-            store_states(a.seg_h + ((w.b * a.segments + w.seg) * a.M + m) * NP, h, n0, NP);
-            if (l == 0) a.seg_dt[(w.b * a.segments + w.seg) * a.M + m] = dt_sum;
-        }
-        return;
-    }
-    if (alive && w.seg == a.segments - 1) store_states(a.h_last + (w.b * a.M + m) * a.N, h, n0, a.N);
-    // rows behind the sequence
-    const int64_t z_lo = t_end > t_lo ? t_end : t_lo;
-    for (int64_t i = tid; i < (t_hi - z_lo) * CC; i += NT) {
-        const int ch = w.ch0 + (int)(i % CC);
-        if (ch < per) static_cast<T *>(a.y)[(w.b * a.T + z_lo + i / CC) * a.M + w.g * per + ch] = from_f32<T>(0.0f);
+    meet<NT + NH>();
+    if (alive && blk.w.seg == a.segments - 1) {
+        float s[4];
+        h.get(s);
+        store_states(a.h_last + (blk.w.b * a.M + m) * a.N, s, n0, a.N);
     }
 }
 
-// Turns every piece's own end state (started from zero) into the state that enters it, in place.  REVERSE: the same for
-// the gradient, from the last piece to the first.  One thread per state.
+// ---------------------------------------------------------------------------------------------- time split
+
+constexpr int NH_STATE = 256;
+
+template <int L>
+constexpr int state_smem_bytes()
+{
+    using Q = Geo<L>;
+    return (int)sizeof(float) * 2 * (Q::KF * Q::CC * 4 + Q::KF * Q::NP);
+}
+
+// What a piece of time hands on when nothing enters it, and its sum of step sizes: the state behind its last step, or
+// (REVERSE) the gradient that goes to the step in front of its first one.
+template <typename T, int L, bool VEC, bool REVERSE>
+__global__ void __launch_bounds__(Geo<L>::NT + NH_STATE) sel_state_kernel(const SelArgs a)
+{
+    using Q = Geo<L>;
+    constexpr int K = Q::KF, CC = Q::CC, NT = Q::NT, NP = Q::NP, NH = NH_STATE;
+    extern __shared__ float smem[];
+    float4 *s_in = reinterpret_cast<float4 *>(smem);      // [2][K][CC]: dt twice, and dt x or p twice
+    float *s_w = smem + 8 * K * CC;                       // [2][K][NP]: B or C
+    const Block<K, CC> blk(a);
+    if (blk.w.seg == (REVERSE ? 0 : a.segments - 1)) return;      // nobody comes after it
+
+    if (threadIdx.x >= NT) {
+        using P = Part<K, CC, NH>;
+        constexpr int V = P::V, ITEMS = P::I::ITEMS, ROWS = P::I::ROWS;
+        const int tid = threadIdx.x - NT;
+        const P part(blk, tid);
+        float bias[V];
+        part.channel_values(bias, a.dt_bias);
+        struct Raw {
+            RawPack<T, V, VEC> dt[ITEMS], w[ITEMS], z[ITEMS];
+            GroupRows<T, K, CC, NP, NH> g;
+        } raw[2];
+        const bool gated = REVERSE && a.z.p;
+        // k counts in the order of the walk
+        auto chunk = [&](int64_t k) { return REVERSE ? blk.count - 1 - k : k; };
+        auto fetch = [&](Raw &f, int64_t k) {
+            if (k >= blk.count) return;
+            part.fetch(f.dt, a.dt, blk, chunk(k));
+            part.fetch(f.w, REVERSE ? a.dy : a.x, blk, chunk(k));
+            if (gated) part.fetch(f.z, a.z, blk, chunk(k));
+            f.g.fetch(blk, REVERSE ? a.Cm : a.Bm, a.N, chunk(k), tid);
+        };
+        auto stage = [&](const Raw &f, int64_t k) {
+            if (k >= blk.count) return;
+            const int buf = (int)(k & 1) * K * CC, steps = blk.steps(chunk(k));
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const int r = part.row + i * ROWS;
+                if (r >= K) continue;
+                float d[V], pre[V];
+                step_sizes(d, pre, f.dt[i], bias, a.softplus, part.there(steps, r));
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    float v = f.w[i].get(j);
+                    if (!REVERSE) v *= d[j];
+                    else if (gated) v *= silu_f(f.z[i].get(j));
+                    s_in[buf + r * CC + place_of(part.col + j)] = make_float4(d[j], d[j], v, v);
+                }
+            }
+            f.g.stage(s_w + (k & 1) * K * NP, tid);
+        };
+        fetch(raw[0], 0);
+        fetch(raw[1], 1);
+        stage(raw[0], 0);
+        fetch(raw[0], 2);
+        for (int64_t k = 0; k < blk.count; k += 2) {
+            meet<NT + NH>();
+            stage(raw[1], k + 1);
+            fetch(raw[1], k + 3);
+            if (k + 1 >= blk.count) break;
+            meet<NT + NH>();
+            stage(raw[0], k + 2);
+            fetch(raw[0], k + 4);
+        }
+        return;
+    }
+
+    const int tid = threadIdx.x, c = tid / L, l = tid % L, n0 = 4 * l;
+    const bool alive = blk.w.ch0 + c < blk.per;
+    const int m = blk.w.g * blk.per + blk.w.ch0 + c;
+    Quad A2, h;
+    {
+        float r[4] = {0.f, 0.f, 0.f, 0.f};
+        if (alive) load_rates(r, a.A + (int64_t)m * a.N, n0, a.N);
+        A2.set(r);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            A2.q[q] = mul2(A2.q[q], both(LOG2E));
+            h.q[q] = both(0.0f);
+        }
+    }
+    float dt_sum = 0.0f;
+    for (int64_t k = 0; k < blk.count; ++k) {
+        meet<NT + NH>();
+        const float4 *in = s_in + (k & 1) * K * CC + place_of(c);
+        const float *w = s_w + (k & 1) * K * NP + n0;
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            const int t = REVERSE ? K - 1 - i : i;
+            const float4 d4 = in[t * CC];
+            const float4 w4 = *reinterpret_cast<const float4 *>(w + t * NP);
+            const float2 ww[2] = {low(w4), high(w4)};
+            dt_sum += d4.x;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const float2 e = mul2(low(d4), A2.q[q]), f = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                h.q[q] = REVERSE ? mul2(f, fma2(ww[q], high(d4), h.q[q])) : fma2(f, h.q[q], mul2(high(d4), ww[q]));
+            }
+        }
+    }
+    if (alive) {
+        float s[4];
+        h.get(s);
+        store_states(a.seg_h + ((blk.w.b * a.segments + blk.w.seg) * a.M + m) * NP, s, n0, NP);
+        if (l == 0) a.seg_dt[(blk.w.b * a.segments + blk.w.seg) * a.M + m] = dt_sum;
+    }
+}
+
+// Turns what every piece hands on by itself into what enters it, in place: from the first piece to the last, or
+// (REVERSE, gradients) the other way.  One thread per state.
 template <bool REVERSE>
 __global__ void sel_carry_kernel(const SelArgs a, int NP)
 {
@@ -226,334 +513,367 @@ __global__ void sel_carry_kernel(const SelArgs a, int NP)
     const int64_t bm = i / NP, b = bm / a.M, m = bm % a.M;
     const float *start = REVERSE ? a.dh_last : a.h0;
     float carry = (start && n < a.N) ? start[bm * a.N + n] : 0.0f;
-    const float A2 = n < a.N ? a.A[m * a.N + n] * LOG2E : 0.0f;
+    const float A2 = n < a.N ? min_nan(max_nan(a.A[m * a.N + n], -2.0e38f), 2.0e38f) * LOG2E : 0.0f;
+#pragma unroll 4
     for (int k = 0; k < a.segments; ++k) {
         const int s = REVERSE ? a.segments - 1 - k : k;
         const int64_t at = (b * a.segments + s) * a.M + m;
-        const float own = a.seg_h[at * NP + n], sum = a.seg_dt[at];
+        const bool more = k < a.segments - 1;
+        const float own = more ? a.seg_h[at * NP + n] : 0.0f, sum = more ? a.seg_dt[at] : 0.0f;
         a.seg_h[at * NP + n] = carry;
-        carry = fmaf(sum == 0.0f ? 1.0f : exp2_fast(sum * A2), carry, own);
+        carry = fmaf(exp2_fast(sum * A2), carry, own);
     }
 }
 
 // ---------------------------------------------------------------------------------------------- backward
 
-constexpr int KB = SEL_CHUNK;
-
-// What the elementwise part of the backward derives from one element of dt, x, z and dy.
-struct Elem {
-    float dt, x, p;
+// How the sums over the channels of a warp (gradients of B and C) are formed.  The CW channels of a warp lie in the
+// lane bits above the state lanes.  The first exchanges halve the four states of a lane: lanes of different channels keep
+// their states in different orders (state j at place j ^ order), so that what a lane keeps and what it sends always lie
+// at the same places and no selection is needed.  The other exchanges halve SC consecutive steps.
+template <int L> struct Across {
+    static constexpr int CW = 32 / L;
+    static constexpr int PERM = CW >= 4 ? 4 : CW;               // orders (powers of two; 1: none)
+    static constexpr int REST = CW / PERM;                      // lanes left to sum over after the states
+    static constexpr int SC = REST < SEL_CHUNK ? REST : SEL_CHUNK;
+    static constexpr int KEPT = 4 / PERM;                       // states that a lane is left with
+    static constexpr int COPIES = PERM == 2 ? 4 : PERM;         // of a staged row; the orders 0 and 2 leave two unused
+    // order of a lane's states: its two highest channel bits, the highest exchanges the pairs
+    __device__ static __forceinline__ int order(int cw)
+    {
+        if (PERM == 4) return cw / REST;                        // 0 .. 3
+        if (PERM == 2) return cw * 2;                           // 0 or 2: the halves only
+        return 0;
+    }
+    // sums v over the lanes that the states are halved over; the first KEPT of the four are left
+    __device__ static __forceinline__ void halve_states(Quad &v)
+    {
+        if (PERM >= 2) v.q[0] = add2(v.q[0], make_float2(__shfl_xor_sync(0xffffffffu, v.q[1].x, 16), __shfl_xor_sync(0xffffffffu, v.q[1].y, 16)));
+        if (PERM == 4) v.q[0].x += __shfl_xor_sync(0xffffffffu, v.q[0].y, 8);
+    }
 };
 
-// Gradient that a piece of time sends to the step in front of it when nothing enters from behind, and its sum of step sizes.
-template <typename T, int L, bool VEC>
-__global__ void __launch_bounds__(Geo<L>::NT) sel_backward_state_kernel(const SelArgs a)
+// v[j] = u[j ^ order]
+__device__ __forceinline__ void reorder(float (&v)[4], int order)
 {
-    using Q = Geo<L>;
-    constexpr int CC = Q::CC, NT = Q::NT, NP = Q::NP, COLS = Q::COLS;
-    __shared__ float2 s_in[KB * CC];         // dt, p
-    __shared__ float s_c[KB * NP];
-    const Where w = locate<CC>(a);
-    const int per = a.M / a.G;
-    const int tid = threadIdx.x, c = tid / L, l = tid % L, n0 = 4 * l;
-    const bool alive = w.ch0 + c < per;
-    const int m = w.g * per + w.ch0 + c;
-    const int64_t len = sequence_length(a, w.b);
-    const int64_t t_lo = w.seg * a.seg, t_hi = t_lo + a.seg < a.T ? t_lo + a.seg : a.T;
-    const int64_t t_end = t_hi < len ? t_hi : len;
-    float A2[4] = {0.f, 0.f, 0.f, 0.f}, r[4] = {0.f, 0.f, 0.f, 0.f};
-    if (alive) {
-        load_states(A2, a.A + (int64_t)m * a.N, n0, a.N);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) A2[j] *= LOG2E;
-    }
-    float dt_sum = 0.0f;
-    const int64_t count = t_end > t_lo ? (t_end - t_lo + KB - 1) / KB : 0;
-    for (int64_t k = count - 1; k >= 0; --k) {
-        const int64_t tc = t_lo + k * KB;
-        const int steps = t_end - tc < KB ? (int)(t_end - tc) : KB;
-        __syncthreads();
-        for (int i = tid; i < KB * COLS; i += NT) {
-            const int row = i / COLS, col = (i % COLS) * 4;
-            const int left = row < steps ? per - (w.ch0 + col) : 0;
-            const int ch = w.g * per + w.ch0 + col;
-            Pack<T, 4> pd, pz, pg;
-            load_pack<VEC>(pd, static_cast<const T *>(a.dt.p) + w.b * a.dt.sb + (tc + row) * a.dt.st + ch, left);
-            load_pack<VEC>(pg, static_cast<const T *>(a.dy.p) + w.b * a.dy.sb + (tc + row) * a.dy.st + ch, left);
-            if (a.z.p) load_pack<VEC>(pz, static_cast<const T *>(a.z.p) + w.b * a.z.sb + (tc + row) * a.z.st + ch, left);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float d = 0.0f, p = 0.0f;
-                if (j < left) {
-                    d = step_size(to_f32(pd.v[j]), a.dt_bias ? a.dt_bias[ch + j] : 0.0f, a.softplus);
-                    p = to_f32(pg.v[j]);
-                    if (a.z.p) p *= silu_f(to_f32(pz.v[j]));
-                }
-                s_in[row * CC + col + j] = make_float2(d, p);
-            }
-        }
-        stage_group<T, NT, NP, KB>(s_c, a.Cm, w.b, tc, steps, w.g, a.N);
-        __syncthreads();
-#pragma unroll
-        for (int t = KB - 1; t >= 0; --t) {
-            if (t < steps) {
-                const float2 in = s_in[t * CC + c];
-                const float4 c4 = *reinterpret_cast<const float4 *>(s_c + t * NP + n0);
-                const float cc[4] = {c4.x, c4.y, c4.z, c4.w};
-                dt_sum += in.x;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) r[j] = exp2_fast(in.x * A2[j]) * fmaf(cc[j], in.y, r[j]);
-            }
-        }
-    }
-    if (alive) {
-        store_states(a.seg_h + ((w.b * a.segments + w.seg) * a.M + m) * NP, r, n0, NP);
-        if (l == 0) a.seg_dt[(w.b * a.segments + w.seg) * a.M + m] = dt_sum;
-    }
+    if (order & 1) { float t = v[0]; v[0] = v[1]; v[1] = t; t = v[2]; v[2] = v[3]; v[3] = t; }
+    if (order & 2) { float t = v[0]; v[0] = v[2]; v[2] = t; t = v[1]; v[1] = v[3]; v[3] = t; }
 }
+
+constexpr int KB = SEL_CHUNK, NH_BACKWARD = 128;
 
 template <int L>
 constexpr int backward_smem_bytes()
 {
     using Q = Geo<L>;
-    const int warps = Q::NT / 32;
-    return (int)sizeof(float) * (KB * Q::CC * 6 + KB * Q::NP * 2 + warps * KB * 2 * Q::NP + 8 * Q::NT);
+    return (int)sizeof(float) * 2 * (KB * Q::CC * 12 + 2 * KB * Across<L>::COPIES * Q::NP + Q::WARPS * KB * 2 * Q::NP);
 }
 
-// Walks its piece of time backwards, one chunk of KB steps after the other.  In each it rebuilds the states from the
-// chunk's checkpoint, keeping the decays a_t and the decayed states a_t h_{t-1} in registers, and then runs the reverse
-// recurrence  g_t = C_t p_t + a_{t+1} g_{t+1}  (p = dy silu(z)) on them.
+// Walks its piece of time backwards.  In each chunk it rebuilds the states from the chunk's checkpoint, keeping the
+// decays a_t and the decayed states a_t h_{t-1} in registers, and then runs the reverse recurrence
+// g_t = C_t p_t + a_{t+1} g_{t+1}  (p = dy silu(z)) on them, so that every exponential is formed once.
 template <typename T, int L, bool VEC>
-__global__ void __launch_bounds__(Geo<L>::NT) sel_backward_kernel(const SelArgs a)
+__global__ void __launch_bounds__(Geo<L>::NT + NH_BACKWARD) sel_backward_kernel(const SelArgs a)
 {
     using Q = Geo<L>;
-    constexpr int CC = Q::CC, NT = Q::NT, NP = Q::NP, COLS = Q::COLS, WARPS = NT / 32;
-    constexpr int GS = L < KB ? L : KB;             // steps whose sums over the lanes of a channel are formed together
-    constexpr int CW = 32 / L;                      // channels of a warp
-    constexpr int SC = CW <= 4 ? 1 : (CW / 4 < KB ? CW / 4 : KB);      // steps whose sums over the channels are formed together
-    constexpr int VC = 4 * SC, RC = VC >= CW ? VC / CW : 1;
-    static_assert(KB % GS == 0 && KB % SC == 0, "");
+    using X = Across<L>;
+    constexpr int CC = Q::CC, NT = Q::NT, NP = Q::NP, NH = NH_BACKWARD, COPIES = X::COPIES;
     extern __shared__ float smem[];
-    float2 *s_in = reinterpret_cast<float2 *>(smem);      // dt, dt * x
-    float *s_p = smem + 2 * KB * CC;
-    float *s_y = s_p + KB * CC, *s_gb = s_y + KB * CC, *s_ga = s_gb + KB * CC;
-    float *s_b = s_ga + KB * CC, *s_c = s_b + KB * NP;
-    float *s_bc = s_c + KB * NP;                          // [warp][step][B, C][NP]
-    float *s_d = s_bc + WARPS * KB * 2 * NP;              // [thread][8]
-    const Where w = locate<CC>(a);
-    const int per = a.M / a.G;
-    const int tid = threadIdx.x, c = tid / L, l = tid % L, n0 = 4 * l, warp = tid / 32, cw = (tid % 32) / L;
-    const bool alive = w.ch0 + c < per;
-    const int m = w.g * per + w.ch0 + c;
-    const int64_t len = sequence_length(a, w.b);
-    const int64_t t_lo = w.seg * a.seg, t_hi = t_lo + a.seg < a.T ? t_lo + a.seg : a.T;
-    const int64_t t_end = t_hi < len ? t_hi : len;
+    float4 *s_in = reinterpret_cast<float4 *>(smem);      // [2][KB][CC]: dt twice, dt x twice
+    float2 *s_p = reinterpret_cast<float2 *>(smem + 8 * KB * CC);      // [2][KB][CC]: p twice
+    float *s_x = smem + 12 * KB * CC;                     // [2][KB][CC]: x
+    float *s_s = s_x + 2 * KB * CC;                       // slope of the step size
+    float *s_q = s_s + 2 * KB * CC;                       // dy times the slope of silu(z)
+    float *s_y = s_q + 2 * KB * CC, *s_gb = s_y + 2 * KB * CC, *s_ga = s_gb + 2 * KB * CC;      // sums over the states: C h, g B, g a h A
+    float *s_b = s_ga + 2 * KB * CC, *s_c = s_b + 2 * KB * COPIES * NP;              // [2][KB][COPIES][NP]
+    float *s_bc = s_c + 2 * KB * COPIES * NP;             // [2][warp][KB][B, C][NP]
+    const Block<KB, CC> blk(a);
+    const bool gated = a.z.p != nullptr;
     const int64_t nchunks = (a.T + SEL_CHUNK - 1) / SEL_CHUNK;
-    const int tiles = (per + CC - 1) / CC;
 
-    float A2[4] = {0.f, 0.f, 0.f, 0.f}, A1[4] = {0.f, 0.f, 0.f, 0.f}, g[4] = {0.f, 0.f, 0.f, 0.f}, dA[4] = {0.f, 0.f, 0.f, 0.f};
-    if (alive) {
-        load_states(A1, a.A + (int64_t)m * a.N, n0, a.N);
+    if (threadIdx.x >= NT) {
+        using P = Part<KB, CC, NH>;
+        constexpr int V = P::V, ITEMS = P::I::ITEMS, ROWS = P::I::ROWS, COLS = P::I::COLS;
+        using F = Pack<float, V>;
+        const int tid = threadIdx.x - NT;
+        const P part(blk, tid);
+        float skip[V], bias[V], dD[V], dbias[V];
+        part.channel_values(skip, a.D);
+        part.channel_values(bias, a.dt_bias);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) A2[j] = A1[j] * LOG2E;
-        if (a.segments > 1) load_states(g, a.seg_h + ((w.b * a.segments + w.seg) * a.M + m) * NP, n0, NP);
-        else if (a.dh_last) load_states(g, a.dh_last + (w.b * a.M + m) * a.N, n0, a.N);
-    }
-    float dD[4] = {0.f, 0.f, 0.f, 0.f}, dbias[4] = {0.f, 0.f, 0.f, 0.f};      // of the elementwise part's channels
-
-    const int64_t count = t_end > t_lo ? (t_end - t_lo + KB - 1) / KB : 0;
-    for (int64_t k = count - 1; k >= 0; --k) {
-        const int64_t tc = t_lo + k * KB;
-        const int steps = t_end - tc < KB ? (int)(t_end - tc) : KB;
-        float h[4] = {0.f, 0.f, 0.f, 0.f};
-        if (alive) load_states(h, a.ckpt + ((w.b * nchunks + tc / SEL_CHUNK) * a.M + m) * NP, n0, NP);
-        __syncthreads();
-        for (int i = tid; i < KB * COLS; i += NT) {
-            const int row = i / COLS, col = (i % COLS) * 4;
-            const int left = row < steps ? per - (w.ch0 + col) : 0;
-            const int ch = w.g * per + w.ch0 + col;
-            Pack<T, 4> px, pd, pz, pg;
-            load_pack<VEC>(px, static_cast<const T *>(a.x.p) + w.b * a.x.sb + (tc + row) * a.x.st + ch, left);
-            load_pack<VEC>(pd, static_cast<const T *>(a.dt.p) + w.b * a.dt.sb + (tc + row) * a.dt.st + ch, left);
-            load_pack<VEC>(pg, static_cast<const T *>(a.dy.p) + w.b * a.dy.sb + (tc + row) * a.dy.st + ch, left);
-            if (a.z.p) load_pack<VEC>(pz, static_cast<const T *>(a.z.p) + w.b * a.z.sb + (tc + row) * a.z.st + ch, left);
+        for (int j = 0; j < V; ++j) dD[j] = dbias[j] = 0.0f;
+        struct Raw {
+            RawPack<T, V, VEC> x[ITEMS], dt[ITEMS], z[ITEMS], dy[ITEMS];
+            GroupRows<T, KB, CC, NP, NH, COPIES> b, c;
+        } raw[2];
+        // chunks are numbered in time and walked backwards
+        auto fetch = [&](Raw &f, int64_t k) {
+            if (k < 0) return;
+            part.fetch(f.x, a.x, blk, k);
+            part.fetch(f.dt, a.dt, blk, k);
+            part.fetch(f.dy, a.dy, blk, k);
+            if (gated) part.fetch(f.z, a.z, blk, k);
+            f.b.fetch(blk, a.Bm, a.N, k, tid);
+            f.c.fetch(blk, a.Cm, a.N, k, tid);
+        };
+        auto stage = [&](const Raw &f, int64_t k) {
+            if (k < 0) return;
+            const int buf = (int)(k & 1) * KB * CC, steps = blk.steps(k);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float d = 0.0f, u = 0.0f, p = 0.0f;
-                if (j < left) {
-                    d = step_size(to_f32(pd.v[j]), a.dt_bias ? a.dt_bias[ch + j] : 0.0f, a.softplus);
-                    u = d * to_f32(px.v[j]);
-                    p = to_f32(pg.v[j]);
-                    if (a.z.p) p *= silu_f(to_f32(pz.v[j]));
-                }
-                s_in[row * CC + col + j] = make_float2(d, u);
-                s_p[row * CC + col + j] = p;
-            }
-        }
-        stage_group<T, NT, NP, KB>(s_b, a.Bm, w.b, tc, steps, w.g, a.N);
-        stage_group<T, NT, NP, KB>(s_c, a.Cm, w.b, tc, steps, w.g, a.N);
-        __syncthreads();
-
-        // forward through the chunk: decays, decayed states, readout, gradient of C
-        float av[KB][4], ah[KB][4];
-        {
-            float y[GS], vc[VC];
+            for (int i = 0; i < ITEMS; ++i) {
+                const int r = part.row + i * ROWS, at = buf + r * CC + part.col;
+                if (r >= KB) continue;
+                float d[V], pre[V];
+                step_sizes(d, pre, f.dt[i], bias, a.softplus, part.there(steps, r));
+                F fx, fs, fq;
 #pragma unroll
-            for (int t = 0; t < KB; ++t) {
-                const float2 in = s_in[t * CC + c];
-                const float p = s_p[t * CC + c];
-                const float4 b4 = *reinterpret_cast<const float4 *>(s_b + t * NP + n0);
-                const float4 c4 = *reinterpret_cast<const float4 *>(s_c + t * NP + n0);
-                const float bb[4] = {b4.x, b4.y, b4.z, b4.w}, cc[4] = {c4.x, c4.y, c4.z, c4.w};
-                float sum = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    av[t][j] = t < steps ? exp2_fast(in.x * A2[j]) : 1.0f;
-                    ah[t][j] = av[t][j] * h[j];
-                    h[j] = fmaf(in.y, bb[j], ah[t][j]);
-                    sum = fmaf(cc[j], h[j], sum);
-                    vc[(t % SC) * 4 + j] = p * h[j];
-                }
-                y[t % GS] = sum;
-                if (t % GS == GS - 1 && a.z.p) {
-                    reduce_scatter<GS, L, 1>(y, tid);
-                    if (writes_total<GS, L>(l)) s_y[(t - (GS - 1) + first_of<GS, L>(l)) * CC + c] = y[0];
-                }
-                if (t % SC == SC - 1) {
-                    reduce_scatter<VC, CW, L>(vc, tid);
-                    if (writes_total<VC, CW>(cw)) {
-#pragma unroll
-                        for (int r = 0; r < RC; ++r) {
-                            const int e = first_of<VC, CW>(cw) + r;
-                            s_bc[((warp * KB + t - (SC - 1) + e / 4) * 2 + 1) * NP + n0 + e % 4] = vc[r];
-                        }
+                for (int j = 0; j < V; ++j) {
+                    const float x = f.x[i].get(j), up = f.dy[i].get(j), u = d[j] * x;
+                    s_in[buf + r * CC + place_of(part.col + j)] = make_float4(d[j], d[j], u, u);
+                    fx.v[j] = x;
+                    fs.v[j] = a.softplus ? sigmoid_f(pre[j]) : 1.0f;
+                    float p = up;
+                    if (gated) {
+                        const float z = f.z[i].get(j), sg = sigmoid_f(z), gate = z * sg;
+                        p = up * gate;
+                        fq.v[j] = up * fmaf(gate, 1.0f - sg, sg);
                     }
+                    s_p[at + j] = both(p);
                 }
+                *reinterpret_cast<F *>(s_x + at) = fx;
+                *reinterpret_cast<F *>(s_s + at) = fs;
+                if (gated) *reinterpret_cast<F *>(s_q + at) = fq;
             }
-        }
-        // backward through it
-        {
-            float gb[GS], ga[GS], vb[VC], dA_c[4] = {0.f, 0.f, 0.f, 0.f};
+            f.b.stage(s_b + (k & 1) * KB * COPIES * NP, tid);
+            f.c.stage(s_c + (k & 1) * KB * COPIES * NP, tid);
+        };
+        auto emit = [&](int64_t k) {
+            if (k >= blk.count) return;
+            const int buf = (int)(k & 1) * KB * CC, steps = blk.steps(k);
+            const float *sums = s_bc + (k & 1) * Q::WARPS * KB * 2 * NP;
+            float *to = a.part_bc + (((blk.w.tile * a.B + blk.w.b) * a.T + blk.time(k)) * a.G + blk.w.g) * 2 * NP;
+            for (int i = tid; i < steps * 2 * NP; i += NH) {
+                float s = 0.0f;
 #pragma unroll
-            for (int t = KB - 1; t >= 0; --t) {
-                const float2 in = s_in[t * CC + c];
-                const float p = s_p[t * CC + c];
-                const float4 b4 = *reinterpret_cast<const float4 *>(s_b + t * NP + n0);
-                const float4 c4 = *reinterpret_cast<const float4 *>(s_c + t * NP + n0);
-                const float bb[4] = {b4.x, b4.y, b4.z, b4.w}, cc[4] = {c4.x, c4.y, c4.z, c4.w};
-                float sb = 0.0f, sa = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    g[j] = fmaf(cc[j], p, g[j]);
-                    vb[(t % SC) * 4 + j] = g[j] * in.y;
-                    sb = fmaf(g[j], bb[j], sb);
-                    const float u = g[j] * ah[t][j];
-                    sa = fmaf(u, A1[j], sa);
-                    dA_c[j] = fmaf(u, in.x, dA_c[j]);
-                    g[j] *= av[t][j];
-                }
-                gb[t % GS] = sb;
-                ga[t % GS] = sa;
-                if (t % GS == 0) {
-                    reduce_scatter<GS, L, 1>(gb, tid);
-                    reduce_scatter<GS, L, 1>(ga, tid);
-                    if (writes_total<GS, L>(l)) {
-                        s_gb[(t + first_of<GS, L>(l)) * CC + c] = gb[0];
-                        s_ga[(t + first_of<GS, L>(l)) * CC + c] = ga[0];
-                    }
-                }
-                if (t % SC == 0) {
-                    reduce_scatter<VC, CW, L>(vb, tid);
-                    if (writes_total<VC, CW>(cw)) {
-#pragma unroll
-                        for (int r = 0; r < RC; ++r) {
-                            const int e = first_of<VC, CW>(cw) + r;
-                            s_bc[((warp * KB + t + e / 4) * 2) * NP + n0 + e % 4] = vb[r];
-                        }
-                    }
-                }
+                for (int q = 0; q < Q::WARPS; ++q) s += sums[q * KB * 2 * NP + i];
+                to[(int64_t)(i / (2 * NP)) * a.G * 2 * NP + i % (2 * NP)] = s;
             }
+            int64_t out = (blk.w.b * a.T + blk.time(k) + part.row) * a.M + part.ch;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) dA[j] += dA_c[j];
-        }
-        __syncthreads();
-        for (int i = tid; i < steps * 2 * NP; i += NT) {
-            float s = 0.0f;
-#pragma unroll
-            for (int q = 0; q < WARPS; ++q) s += s_bc[q * KB * 2 * NP + i];
-            const int64_t row = ((w.tile * a.B + w.b) * a.T + tc + i / (2 * NP)) * a.G + w.g;
-            a.part_bc[row * 2 * NP + i % (2 * NP)] = s;
-        }
-        for (int i = tid; i < KB * COLS; i += NT) {
-            const int row = i / COLS, col = (i % COLS) * 4;
-            const int left = row < steps ? per - (w.ch0 + col) : 0;
-            const int ch = w.g * per + w.ch0 + col;
-            if (left <= 0) continue;
-            Pack<T, 4> px, pd, pz, pg, ox, od, oz;
-            load_pack<VEC>(px, static_cast<const T *>(a.x.p) + w.b * a.x.sb + (tc + row) * a.x.st + ch, left);
-            load_pack<VEC>(pd, static_cast<const T *>(a.dt.p) + w.b * a.dt.sb + (tc + row) * a.dt.st + ch, left);
-            if (a.z.p) {
-                load_pack<VEC>(pg, static_cast<const T *>(a.dy.p) + w.b * a.dy.sb + (tc + row) * a.dy.st + ch, left);
-                load_pack<VEC>(pz, static_cast<const T *>(a.z.p) + w.b * a.z.sb + (tc + row) * a.z.st + ch, left);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int at = row * CC + col + j;
-                const float x = to_f32(px.v[j]), p = s_p[at];
-                const float skip = (j < left && a.D) ? a.D[ch + j] : 0.0f;
-                const float pre = to_f32(pd.v[j]) + ((j < left && a.dt_bias) ? a.dt_bias[ch + j] : 0.0f);
-                float d = fmaf(s_gb[at], x, s_ga[at]);
-                if (a.softplus) d *= sigmoid_f(pre);
-                ox.v[j] = from_f32<T>(fmaf(s_in[at].x, s_gb[at], skip * p));
-                od.v[j] = from_f32<T>(d);
-                if (a.z.p) {
-                    const float z = to_f32(pz.v[j]), sg = sigmoid_f(z);
-                    const float raw = fmaf(skip, x, s_y[at]);
-                    oz.v[j] = from_f32<T>(to_f32(pg.v[j]) * raw * (sg * (1.0f + z * (1.0f - sg))));
+            for (int i = 0; i < ITEMS; ++i, out += ROWS * (int64_t)a.M) {
+                const int r = part.row + i * ROWS, have = part.there(steps, r), at = buf + r * CC + part.col;
+                if (have <= 0) continue;
+                const F fx = *reinterpret_cast<const F *>(s_x + at), fs = *reinterpret_cast<const F *>(s_s + at),
+                        fb = *reinterpret_cast<const F *>(s_gb + at), fa = *reinterpret_cast<const F *>(s_ga + at);
+                F fq, fy;
+                if (gated) {
+                    fq = *reinterpret_cast<const F *>(s_q + at);
+                    fy = *reinterpret_cast<const F *>(s_y + at);
                 }
-                if (j < left) {
+                Pack<T, V> ox, od, oz;
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float p = s_p[at + j].x, x = fx.v[j];
+                    const float d = fmaf(fb.v[j], x, fa.v[j]) * fs.v[j];
+                    ox.v[j] = from_f32<T>(fmaf(s_in[buf + r * CC + place_of(part.col + j)].x, fb.v[j], skip[j] * p));
+                    od.v[j] = from_f32<T>(d);
+                    if (gated) oz.v[j] = from_f32<T>(fq.v[j] * fmaf(skip[j], x, fy.v[j]));
                     dD[j] = fmaf(p, x, dD[j]);
                     dbias[j] += d;
                 }
+                store_pack<VEC>(static_cast<T *>(a.dx) + out, ox, have);
+                store_pack<VEC>(static_cast<T *>(a.ddt) + out, od, have);
+                if (gated) store_pack<VEC>(static_cast<T *>(a.dz) + out, oz, have);
             }
-            const int64_t at = (w.b * a.T + tc + row) * a.M + ch;
-            store_pack<VEC>(static_cast<T *>(a.dx) + at, ox, left);
-            store_pack<VEC>(static_cast<T *>(a.ddt) + at, od, left);
-            if (a.z.p) store_pack<VEC>(static_cast<T *>(a.dz) + at, oz, left);
+        };
+        fetch(raw[0], blk.count - 1);
+        fetch(raw[1], blk.count - 2);
+        stage(raw[0], blk.count - 1);
+        fetch(raw[0], blk.count - 3);
+        for (int64_t k = blk.count - 1; k >= 0; k -= 2) {
+            meet<NT + NH>();
+            emit(k + 1);
+            stage(raw[1], k - 1);
+            fetch(raw[1], k - 3);
+            if (k < 1) break;
+            meet<NT + NH>();
+            emit(k);
+            stage(raw[0], k - 2);
+            fetch(raw[0], k - 4);
+        }
+        meet<NT + NH>();
+        emit(0);
+        // sums of the threads that had the same columns; the recurrence is done with all of the shared memory
+        asm volatile("bar.sync 1, %0;" ::"n"(NH) : "memory");
+        float *s_d = smem;      // [thread][2 V]
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            s_d[tid * 2 * V + j] = dD[j];
+            s_d[tid * 2 * V + V + j] = dbias[j];
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(NH) : "memory");
+        for (int i = tid; i < 2 * CC; i += NH) {
+            const int ch = i % CC, which = i / CC;
+            float s = 0.0f;
+            for (int q = ch / V; q < NH; q += COLS) s += s_d[q * 2 * V + which * V + ch % V];
+            if (blk.w.ch0 + ch < blk.per) a.part_d[((blk.w.b * a.segments + blk.w.seg) * 2 + which) * a.M + blk.w.g * blk.per + blk.w.ch0 + ch] = s;
+        }
+        // rows behind the sequence have no gradient
+        const int64_t z_lo = blk.t_end > blk.t_lo ? blk.t_end : blk.t_lo;
+        for (int64_t i = tid; i < (blk.t_hi - z_lo) * CC; i += NH) {
+            const int ch = blk.w.ch0 + (int)(i % CC);
+            if (ch >= blk.per) continue;
+            const int64_t at = (blk.w.b * a.T + z_lo + i / CC) * a.M + blk.w.g * blk.per + ch;
+            static_cast<T *>(a.dx)[at] = from_f32<T>(0.0f);
+            static_cast<T *>(a.ddt)[at] = from_f32<T>(0.0f);
+            if (gated) static_cast<T *>(a.dz)[at] = from_f32<T>(0.0f);
+        }
+        for (int64_t i = tid; i < (blk.t_hi - z_lo) * 2 * NP; i += NH) {
+            const int64_t row = ((blk.w.tile * a.B + blk.w.b) * a.T + z_lo + i / (2 * NP)) * a.G + blk.w.g;
+            a.part_bc[row * 2 * NP + i % (2 * NP)] = 0.0f;
+        }
+        return;
+    }
+
+    constexpr int GS = L < KB ? L : KB;             // steps whose sums over the lanes of a channel are formed together
+    constexpr int SC = X::SC;
+    static_assert(KB % GS == 0 && KB % SC == 0 && X::REST <= SC, "");
+    const int tid = threadIdx.x, c = tid / L, l = tid % L, n0 = 4 * l, warp = tid / 32, cw = tid % 32 / L;
+    const int order = X::order(cw);
+    const bool alive = blk.w.ch0 + c < blk.per;
+    const int m = blk.w.g * blk.per + blk.w.ch0 + c;
+    Quad A1, A2, g, dA;
+    {
+        float r[4] = {0.f, 0.f, 0.f, 0.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
+        if (alive) {
+            load_rates(r, a.A + (int64_t)m * a.N, n0, a.N);
+            if (a.segments > 1) load_states(s, a.seg_h + ((blk.w.b * a.segments + blk.w.seg) * a.M + m) * NP, n0, NP);
+            else if (a.dh_last) load_states(s, a.dh_last + (blk.w.b * a.M + m) * a.N, n0, a.N);
+        }
+        reorder(r, order);
+        reorder(s, order);
+        A1.set(r);
+        g.set(s);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            A2.q[q] = mul2(A1.q[q], both(LOG2E));
+            dA.q[q] = both(0.0f);
         }
     }
-    if (alive) {
-        store_states(a.part_a + ((w.b * a.segments + w.seg) * a.M + m) * NP, dA, n0, NP);
-        if (a.dh0 && w.seg == 0) store_states(a.dh0 + (w.b * a.M + m) * a.N, g, n0, a.N);
-    }
-    // a thread's elementwise part always has the same four columns (NT is a multiple of COLS): sum over the threads
+    float4 state = make_float4(0.f, 0.f, 0.f, 0.f);      // checkpoint of the next chunk
+    auto fetch_state = [&](int64_t k) {
+        if (k >= 0 && alive) state = *reinterpret_cast<const float4 *>(a.ckpt + ((blk.w.b * nchunks + blk.t_lo / SEL_CHUNK + k) * a.M + m) * NP + n0);
+    };
+    fetch_state(blk.count - 1);
+    for (int64_t k = blk.count - 1; k >= 0; --k) {
+        meet<NT + NH>();
+        const float4 *in = s_in + (k & 1) * KB * CC + place_of(c);
+        const float2 *p = s_p + (k & 1) * KB * CC + c;
+        const float *b = s_b + ((k & 1) * KB * COPIES + order) * NP + n0, *cc = s_c + ((k & 1) * KB * COPIES + order) * NP + n0;
+        float *y_out = s_y + (k & 1) * KB * CC + c, *gb_out = s_gb + (k & 1) * KB * CC + c, *ga_out = s_ga + (k & 1) * KB * CC + c;
+        float *bc_out = s_bc + ((k & 1) * Q::WARPS + warp) * KB * 2 * NP + n0;
+        // Leaves the warp's totals of `v`, gathered over SC steps from t on, in row `which` (B, C) of the steps.
+        auto across = [&](Quad (&v)[SC], int t, int which) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        s_d[tid * 8 + j] = dD[j];
-        s_d[tid * 8 + 4 + j] = dbias[j];
+            for (int i = 0; i < SC; ++i) X::halve_states(v[i]);
+            if (X::REST > 1) {
+                float s[SC];
+#pragma unroll
+                for (int i = 0; i < SC; ++i) s[i] = v[i].q[0].x;
+                reduce_scatter<SC, X::REST, L>(s, tid);
+                bc_out[((t + cw % X::REST) * 2 + which) * NP + order] = s[0];
+            } else {
+                float s[4];
+                v[0].get(s);
+#pragma unroll
+                for (int i = 0; i < X::KEPT; ++i) bc_out[(t * 2 + which) * NP + (i ^ order)] = s[i];
+            }
+        };
+
+        Quad av[KB], ah[KB];
+        {      // forward through the chunk: decays, decayed states, readout, gradient of C
+            Quad h;
+            {
+                float s[4] = {state.x, state.y, state.z, state.w};
+                reorder(s, order);
+                h.set(s);
+            }
+            fetch_state(k - 1);
+            float y[GS];
+            Quad vc[SC];
+#pragma unroll
+            for (int t = 0; t < KB; ++t) {
+                const float4 d4 = in[t * CC];
+                const float2 pt = p[t * CC];
+                const float4 b4 = *reinterpret_cast<const float4 *>(b + t * COPIES * NP);
+                const float2 bb[2] = {low(b4), high(b4)};
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const float2 e = mul2(low(d4), A2.q[q]);
+                    av[t].q[q] = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                    ah[t].q[q] = mul2(av[t].q[q], h.q[q]);
+                    h.q[q] = fma2(high(d4), bb[q], ah[t].q[q]);
+                    vc[t % SC].q[q] = mul2(pt, h.q[q]);
+                }
+                if (gated) {
+                    const float4 c4 = *reinterpret_cast<const float4 *>(cc + t * COPIES * NP);
+                    const float2 sum = fma2(high(c4), h.q[1], mul2(low(c4), h.q[0]));
+                    y[t % GS] = sum.x + sum.y;
+                    if (t % GS == GS - 1) {
+                        reduce_scatter<GS, L, 1>(y, tid);
+                        if (writes_total<GS, L>(l)) y_out[(t - (GS - 1) + first_of<GS, L>(l)) * CC] = y[0];
+                    }
+                }
+                if (t % SC == SC - 1) across(vc, t - (SC - 1), 1);
+            }
+        }
+        {      // backward through it
+            float sb[GS], sa[GS];
+            Quad vb[SC], dA_c;
+            dA_c.q[0] = dA_c.q[1] = both(0.0f);
+#pragma unroll
+            for (int t = KB - 1; t >= 0; --t) {
+                const float4 d4 = in[t * CC];
+                const float2 pt = p[t * CC];
+                const float4 b4 = *reinterpret_cast<const float4 *>(b + t * COPIES * NP), c4 = *reinterpret_cast<const float4 *>(cc + t * COPIES * NP);
+                const float2 bb[2] = {low(b4), high(b4)}, ccv[2] = {low(c4), high(c4)};
+                float2 rb, ra;
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    g.q[q] = fma2(ccv[q], pt, g.q[q]);
+                    vb[t % SC].q[q] = mul2(g.q[q], high(d4));
+                    rb = q ? fma2(g.q[q], bb[q], rb) : mul2(g.q[q], bb[q]);
+                    const float2 u = mul2(g.q[q], ah[t].q[q]);
+                    ra = q ? fma2(u, A1.q[q], ra) : mul2(u, A1.q[q]);
+                    dA_c.q[q] = fma2(u, low(d4), dA_c.q[q]);
+                    g.q[q] = mul2(g.q[q], av[t].q[q]);
+                }
+                sb[t % GS] = rb.x + rb.y;
+                sa[t % GS] = ra.x + ra.y;
+                if (t % GS == 0) {
+                    reduce_scatter<GS, L, 1>(sb, tid);
+                    reduce_scatter<GS, L, 1>(sa, tid);
+                    if (writes_total<GS, L>(l)) {
+                        gb_out[(t + first_of<GS, L>(l)) * CC] = sb[0];
+                        ga_out[(t + first_of<GS, L>(l)) * CC] = sa[0];
+                    }
+                }
+                if (t % SC == 0) across(vb, t, 0);
+            }
+#pragma unroll
+            for (int q = 0; q < 2; ++q) dA.q[q] = add2(dA.q[q], dA_c.q[q]);
+        }
     }
-    __syncthreads();
-    for (int i = tid; i < 2 * CC; i += NT) {
-        const int ch = i % CC, which = i / CC;
-        float s = 0.0f;
-        for (int q = ch / 4; q < NT; q += COLS) s += s_d[q * 8 + which * 4 + ch % 4];
-        if (w.ch0 + ch < per) a.part_d[((w.b * a.segments + w.seg) * 2 + which) * a.M + w.g * per + w.ch0 + ch] = s;
+    meet<NT + NH>();
+    if (alive) {
+        float s[4], r[4];
+        dA.get(s);
+        g.get(r);
+        reorder(s, order);
+        reorder(r, order);
+        store_states(a.part_a + ((blk.w.b * a.segments + blk.w.seg) * a.M + m) * NP, s, n0, NP);
+        if (a.dh0 && blk.w.seg == 0) store_states(a.dh0 + (blk.w.b * a.M + m) * a.N, r, n0, a.N);
     }
-    // rows behind the sequence have no gradient
-    const int64_t z_lo = t_end > t_lo ? t_end : t_lo;
-    for (int64_t i = tid; i < (t_hi - z_lo) * CC; i += NT) {
-        const int ch = w.ch0 + (int)(i % CC);
-        if (ch >= per) continue;
-        const int64_t at = (w.b * a.T + z_lo + i / CC) * a.M + w.g * per + ch;
-        static_cast<T *>(a.dx)[at] = from_f32<T>(0.0f);
-        static_cast<T *>(a.ddt)[at] = from_f32<T>(0.0f);
-        if (a.z.p) static_cast<T *>(a.dz)[at] = from_f32<T>(0.0f);
-    }
-    for (int64_t i = tid; i < (t_hi - z_lo) * 2 * NP; i += NT) {
-        const int64_t row = ((w.tile * a.B + w.b) * a.T + z_lo + i / (2 * NP)) * a.G + w.g;
-        a.part_bc[row * 2 * NP + i % (2 * NP)] = 0.0f;
-    }
-    (void)tiles;
 }
 
 // Gradients of B and C: sum over the channel tiles.  One thread per (b, t, g, B or C, n).
@@ -606,7 +926,8 @@ __global__ void __launch_bounds__(256) sel_step_kernel(const SelStepArgs a)
         load_states(h, hp, n0, a.N);
         load_states(A, a.A + (int64_t)m * a.N, n0, a.N);
         x = to_f32(static_cast<const T *>(a.x.p)[b * a.x.sb + m]);
-        const float d = step_size(to_f32(static_cast<const T *>(a.dt.p)[b * a.dt.sb + m]), a.dt_bias ? a.dt_bias[m] : 0.0f, a.softplus);
+        float d = to_f32(static_cast<const T *>(a.dt.p)[b * a.dt.sb + m]) + (a.dt_bias ? a.dt_bias[m] : 0.0f);
+        if (a.softplus) d = softplus_f(d);
         const T *bp = static_cast<const T *>(a.Bm.p) + b * a.Bm.sb + (int64_t)g * a.N;
         const T *cp = static_cast<const T *>(a.Cm.p) + b * a.Cm.sb + (int64_t)g * a.N;
 #pragma unroll
@@ -641,15 +962,33 @@ bool pack_aligned(const View &v)
     return !v.p || (reinterpret_cast<uintptr_t>(v.p) % (4 * sizeof(T)) == 0 && v.sb % 4 == 0 && v.st % 4 == 0);
 }
 
+template <typename K>
+cudaError_t allow_smem(K kernel, int bytes)
+{
+    return bytes > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) : cudaSuccess;
+}
+
+// What enters every piece of time.
+template <typename T, int L, bool VEC, bool REVERSE>
+cudaError_t enter_pieces(const SelArgs &a, const SelPlan &p, unsigned grid, cudaStream_t s)
+{
+    constexpr int smem = state_smem_bytes<L>();
+    cudaError_t e = allow_smem(sel_state_kernel<T, L, VEC, REVERSE>, smem);
+    if (e != cudaSuccess) return e;
+    sel_state_kernel<T, L, VEC, REVERSE><<<grid, Geo<L>::NT + NH_STATE, smem, s>>>(a);
+    sel_carry_kernel<REVERSE><<<(unsigned)ceil_div(a.B * a.M * p.NP, 128), 128, 0, s>>>(a, p.NP);
+    return cudaGetLastError();
+}
+
 template <typename T, int L, bool VEC>
 cudaError_t forward_typed(const SelArgs &a, const SelPlan &p, cudaStream_t s)
 {
     const unsigned grid = (unsigned)(a.B * a.G * p.tiles * p.segments);
-    if (p.segments > 1) {
-        sel_forward_kernel<T, L, VEC, true><<<grid, Geo<L>::NT, 0, s>>>(a);
-        sel_carry_kernel<false><<<(unsigned)ceil_div(a.B * a.M * p.NP, 128), 128, 0, s>>>(a, p.NP);
-    }
-    sel_forward_kernel<T, L, VEC, false><<<grid, Geo<L>::NT, 0, s>>>(a);
+    constexpr int smem = forward_smem_bytes<L>();
+    cudaError_t e = allow_smem(sel_forward_kernel<T, L, VEC>, smem);
+    if (e == cudaSuccess && p.segments > 1) e = enter_pieces<T, L, VEC, false>(a, p, grid, s);
+    if (e != cudaSuccess) return e;
+    sel_forward_kernel<T, L, VEC><<<grid, Geo<L>::NT + NH_FORWARD, smem, s>>>(a);
     return cudaGetLastError();
 }
 
@@ -657,16 +996,11 @@ template <typename T, int L, bool VEC>
 cudaError_t backward_typed(const SelArgs &a, const SelPlan &p, cudaStream_t s)
 {
     const unsigned grid = (unsigned)(a.B * a.G * p.tiles * p.segments);
-    if (p.segments > 1) {
-        sel_backward_state_kernel<T, L, VEC><<<grid, Geo<L>::NT, 0, s>>>(a);
-        sel_carry_kernel<true><<<(unsigned)ceil_div(a.B * a.M * p.NP, 128), 128, 0, s>>>(a, p.NP);
-    }
     constexpr int smem = backward_smem_bytes<L>();
-    if (smem > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(sel_backward_kernel<T, L, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) return e;
-    }
-    sel_backward_kernel<T, L, VEC><<<grid, Geo<L>::NT, smem, s>>>(a);
+    cudaError_t e = allow_smem(sel_backward_kernel<T, L, VEC>, smem);
+    if (e == cudaSuccess && p.segments > 1) e = enter_pieces<T, L, VEC, true>(a, p, grid, s);
+    if (e != cudaSuccess) return e;
+    sel_backward_kernel<T, L, VEC><<<grid, Geo<L>::NT + NH_BACKWARD, smem, s>>>(a);
     return cudaGetLastError();
 }
 
@@ -744,9 +1078,9 @@ SelPlan sel_plan(int64_t B, int64_t T, int M, int N, int G, bool backward)
     p.NP = 4 * p.L;
     p.CC = sel_channels(p.L);
     p.tiles = (int)ceil_div(M / G, p.CC);
-    const int64_t blocks = B * G * p.tiles, unit = KF;
+    const int64_t blocks = B * G * p.tiles, unit = 16;
     // A block per SM at least: split the time axis when there are fewer, down to pieces of 64 steps.
-    int64_t want = blocks >= 148 ? 1 : ceil_div(296, blocks);
+    int64_t want = blocks >= 96 ? 1 : ceil_div(296, blocks);
     const int64_t most = T / 64 > 1 ? T / 64 : 1;
     if (want > most) want = most;
     p.seg = ceil_div(ceil_div(T, want), unit) * unit;

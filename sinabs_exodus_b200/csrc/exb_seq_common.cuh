@@ -21,6 +21,11 @@ __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 
+// The value whose bits stand in the low end of a word.
+__device__ __forceinline__ float word_to_f32(const float *, uint32_t w) { return __uint_as_float(w); }
+__device__ __forceinline__ float word_to_f32(const __nv_bfloat16 *, uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float word_to_f32(const __half *, uint32_t w) { return __half2float(__ushort_as_half((unsigned short)w)); }
+
 template <typename T> __device__ __forceinline__ T from_f32(float v);
 template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
@@ -49,6 +54,45 @@ __device__ __forceinline__ void load_pack(Pack<T, V> &r, const T *p, int n)
     }
 }
 
+// The same kept as the words that were loaded, for loads that stay in flight over much other work: the elements of a
+// Pack would be taken apart, and waited for, where the load stands.
+template <typename T, int V, bool VEC>
+struct RawPack {
+    static constexpr int PER = VEC ? 4 / (int)sizeof(T) : 1;      // elements of a word
+    static constexpr int WORDS = V / PER;
+    uint32_t w[WORDS];
+
+    __device__ __forceinline__ void load(const T *p, int n)
+    {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) w[i] = 0u;
+            if (n > 0) {
+                if constexpr (WORDS == 4) {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(p);
+                    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+                } else if constexpr (WORDS == 2) {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(p);
+                    w[0] = v.x; w[1] = v.y;
+                } else {
+                    w[0] = *reinterpret_cast<const uint32_t *>(p);
+                }
+            }
+        } else if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) w[i] = i < n ? *reinterpret_cast<const unsigned short *>(p + i) : 0u;
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) w[i] = i < n ? *reinterpret_cast<const uint32_t *>(p + i) : 0u;
+        }
+    }
+    __device__ __forceinline__ float get(int j) const
+    {
+        const uint32_t v = PER == 2 && (j & 1) ? w[j / PER] >> 16 : w[j / PER];
+        return word_to_f32((const T *)nullptr, v);
+    }
+};
+
 template <bool VEC, typename T, int V>
 __device__ __forceinline__ void store_pack(T *p, const Pack<T, V> &r, int n)
 {
@@ -61,8 +105,7 @@ __device__ __forceinline__ void store_pack(T *p, const Pack<T, V> &r, int n)
     }
 }
 
-__device__ __forceinline__ float sigmoid_f(float v) { return 1.0f / (1.0f + expf(-v)); }
-__device__ __forceinline__ float silu_f(float v) { return v / (1.0f + expf(-v)); }
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 // 2^v, two units in the last place at worst over the range that matters; results below 2^-126 become 0.
 __device__ __forceinline__ float exp2_fast(float v)
@@ -71,8 +114,60 @@ __device__ __forceinline__ float exp2_fast(float v)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
+// 1 / v to one unit in the last place.
+__device__ __forceinline__ float rcp_fast(float v)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+// The larger of two values, NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b)
+{
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 
-constexpr float LOG2E = 1.4426950408889634f;
+// The exponent's rounding makes these good to (2 + |v|) * 2^-23: at most a few units where the result matters.
+__device__ __forceinline__ float sigmoid_f(float v) { return rcp_fast(1.0f + exp2_fast(-LOG2E * v)); }
+__device__ __forceinline__ float silu_f(float v) { return v * sigmoid_f(v); }
+
+// Two float32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// log(1 + e^v) = max(v, 0) + log(1 + u), u = e^-|v|, and log(1 + u) = 2 artanh(u / (2 + u)) by its series, whose argument is
+// at most 1/3: seven terms leave 1.4e-8.  u keeps the digits that rounding |v| log2(e) would cost (step sizes are the
+// small end of softplus: v = -7 gives 0.001, and they are multiplied over many steps).
+__device__ __forceinline__ float2 softplus2(float2 v)
+{
+    const float2 w = make_float2(min_nan(fabsf(v.x), 87.0f), min_nan(fabsf(v.y), 87.0f));
+    const float2 t = mul2(w, both(-LOG2E));
+    // what the rounding of t lost, with the second word of log2(e)
+    const float2 lost = fma2(w, both(-1.92596299e-8f), fma2(w, both(-LOG2E), make_float2(-t.x, -t.y)));
+    float2 u = make_float2(exp2_fast(t.x), exp2_fast(t.y));
+    u = fma2(u, mul2(lost, both(LN2)), u);
+    const float2 n = add2(u, both(2.0f));
+    const float2 s = mul2(u, make_float2(rcp_fast(n.x), rcp_fast(n.y))), q = mul2(s, s);
+    float2 p = both(2.0f / 13.0f);
+    p = fma2(p, q, both(2.0f / 11.0f));
+    p = fma2(p, q, both(2.0f / 9.0f));
+    p = fma2(p, q, both(2.0f / 7.0f));
+    p = fma2(p, q, both(2.0f / 5.0f));
+    p = fma2(p, q, both(2.0f / 3.0f));
+    p = fma2(p, q, both(2.0f));
+    return fma2(s, p, make_float2(max_nan(v.x, 0.0f), max_nan(v.y, 0.0f)));
+}
+__device__ __forceinline__ float softplus_f(float v) { return softplus2(both(v)).x; }
 
 // Sums v[0..V) over the W lanes that differ in the lane bits W/2*UNIT ... UNIT, by halving: in each exchange a lane
 // passes on the half that it will not end up with, so that V values cost about V exchanges instead of V*log2(W).
