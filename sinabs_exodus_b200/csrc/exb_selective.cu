@@ -815,14 +815,13 @@ __global__ void __launch_bounds__(Geo<L>::NT + NH_BACKWARD) sel_backward_kernel(
                     h.q[q] = fma2(high(d4), bb[q], ah[t].q[q]);
                     vc[t % SC].q[q] = mul2(pt, h.q[q]);
                 }
-                if (gated) {
-                    const float4 c4 = *reinterpret_cast<const float4 *>(cc + t * COPIES * NP);
-                    const float2 sum = fma2(high(c4), h.q[1], mul2(low(c4), h.q[0]));
-                    y[t % GS] = sum.x + sum.y;
-                    if (t % GS == GS - 1) {
-                        reduce_scatter<GS, L, 1>(y, tid);
-                        if (writes_total<GS, L>(l)) y_out[(t - (GS - 1) + first_of<GS, L>(l)) * CC] = y[0];
-                    }
+                // also without a gate: a branch would end the run of instructions that the scheduler can interleave
+                const float4 c4 = *reinterpret_cast<const float4 *>(cc + t * COPIES * NP);
+                const float2 sum = fma2(high(c4), h.q[1], mul2(low(c4), h.q[0]));
+                y[t % GS] = sum.x + sum.y;
+                if (t % GS == GS - 1) {
+                    reduce_scatter<GS, L, 1>(y, tid);
+                    if (writes_total<GS, L>(l)) y_out[(t - (GS - 1) + first_of<GS, L>(l)) * CC] = y[0];
                 }
                 if (t % SC == SC - 1) across(vc, t - (SC - 1), 1);
             }
