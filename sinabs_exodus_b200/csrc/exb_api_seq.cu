@@ -50,8 +50,8 @@ int check_scan_sizes(const char *who, int64_t B, int64_t T, int64_t M, int64_t N
 // Blocks of the scan's kernels (every block has at least 8 channels, every piece of time at least 16 steps).
 int check_scan_grid(const char *who, const exb::SelPlan &p, int64_t B, int64_t T, int64_t M, int64_t N, int64_t G)
 {
-    const double blocks = (double)B * G * p.tiles * p.segments, sums = (double)B * T * G * 2 * N / 256, states = (double)B * M * p.NP / 128;
-    if (blocks > GRID_MAX || sums > GRID_MAX || states > GRID_MAX) return fail(EXB_ERR_ARG, "%s: sizes too large for one launch", who);
+    const double blocks = (double)B * G * p.tiles * p.segments, sums = (double)B * T * G * 2 * N / 256;
+    if (blocks > GRID_MAX || sums > GRID_MAX) return fail(EXB_ERR_ARG, "%s: sizes too large for one launch", who);
     return EXB_OK;
 }
 
@@ -73,7 +73,7 @@ extern "C" {
 int64_t exb_selective_checkpoint_floats(int64_t B, int64_t T, int64_t M, int64_t N)
 {
     if (B <= 0 || T <= 0 || M <= 0 || N < 1 || N > EXB_SELECTIVE_MAX_STATES) return 0;
-    return B * ((T + EXB_SELECTIVE_CHECKPOINT - 1) / EXB_SELECTIVE_CHECKPOINT) * M * 4 * exb::sel_lanes((int)N);
+    return B * ((T + EXB_SELECTIVE_CHECKPOINT - 1) / EXB_SELECTIVE_CHECKPOINT) * M * exb::sel_padded((int)N);
 }
 
 int64_t exb_selective_workspace_bytes(int64_t B, int64_t T, int64_t M, int64_t N, int64_t G, int backward)

@@ -12,12 +12,14 @@ namespace exb {
 
 namespace {
 
+// L lanes of four states each hold a channel, a thread has two channels: with two, the values that all channels share
+// (B, C) are read from shared memory half as often, which is what bounds these kernels next to the exponentials.
 template <int L> struct Geo {
-    static constexpr int CC = L == 1 ? 128 : 256 / L;
-    static constexpr int NT = CC * L;
+    static constexpr int NT = 128;                  // threads of the recurrence
+    static constexpr int CC = 2 * NT / L;           // channels of a block
     static constexpr int NP = 4 * L;
     static constexpr int WARPS = NT / 32;
-    static constexpr int KF = L == 1 ? 8 : 16;      // steps of a chunk in the forward direction
+    static constexpr int KF = L == 2 ? 8 : 16;      // steps of a chunk in the forward direction
 };
 
 // Which tile, piece of time and batch item a block works on.
@@ -200,12 +202,27 @@ struct GroupRows {
     }
 };
 
-// Where a channel's 16 bytes lie in a row: a preparing thread writes four neighbouring channels one after the other, so
-// neighbouring packs use the places in different orders, which halves the bank conflicts of those stores.
-__device__ __forceinline__ int place_of(int c) { return c ^ ((c >> 2) & 3); }
-
 __device__ __forceinline__ float2 low(const float4 &v) { return make_float2(v.x, v.y); }
 __device__ __forceinline__ float2 high(const float4 &v) { return make_float2(v.z, v.w); }
+
+// A thread's two channels, and how sums over their states are formed.  Lanes with odd l have them in the other order
+// (channel k ^ 1 at place k): what a lane keeps in the first exchange and what it sends then always lie at the same
+// places, and no selection is needed.
+template <int L, int STEPS>
+struct Pair {
+    static constexpr int REST = L / 2;                                 // lanes left after the first exchange
+    static constexpr int GS = REST < STEPS ? REST : STEPS;             // steps that share the other exchanges
+    int l, first;      // state lane; first of the two channels (in the block)
+    __device__ __forceinline__ explicit Pair(int tid) : l(tid % L), first(tid / L * 2) {}
+    __device__ __forceinline__ int channel(int k) const { return first + (k ^ (l & 1)); }
+    // Leaves the totals of GS steps from t on in out[step][CC].
+    __device__ __forceinline__ void total(float (&v)[GS], float *out, int CC, int t) const
+    {
+        reduce_scatter<GS, REST, 2>(v, l);
+        if (writes_total<GS, REST>(l >> 1)) out[(t + first_of<GS, REST>(l >> 1)) * CC + first + (l & 1)] = v[0];
+    }
+    __device__ __forceinline__ static float exchange(float keep, float send) { return keep + __shfl_xor_sync(0xffffffffu, send, 1); }
+};
 
 // Four states of a lane as two pairs.
 struct Quad {
@@ -214,25 +231,46 @@ struct Quad {
     __device__ __forceinline__ void get(float (&v)[4]) const { v[0] = q[0].x; v[1] = q[0].y; v[2] = q[1].x; v[3] = q[1].y; }
 };
 
+// State that enters piece `seg` of channel m (four states from n0 on): what the pieces in front of it hand on by
+// themselves, each decayed through those behind it; or (REVERSE) the gradient that enters from behind.  Every block folds
+// that for itself: a launch less, and the loads of several pieces are in flight together.
+template <bool REVERSE, int NP>
+__device__ __forceinline__ void enter(float (&v)[4], const SelArgs &a, const Where &w, int m, int n0, const Quad &A2)
+{
+    const float *start = REVERSE ? a.dh_last : a.h0;
+    if (start) load_states(v, start + (w.b * a.M + m) * a.N, n0, a.N);
+    const int count = REVERSE ? a.segments - 1 - w.seg : w.seg;
+#pragma unroll 8
+    for (int k = 0; k < count; ++k) {
+        const int64_t at = (w.b * a.segments + (REVERSE ? a.segments - 1 - k : k)) * a.M + m;
+        const float4 own = *reinterpret_cast<const float4 *>(a.seg_h + at * NP + n0);
+        const float sum = a.seg_dt[at];
+        v[0] = fmaf(exp2_fast(sum * A2.q[0].x), v[0], own.x);
+        v[1] = fmaf(exp2_fast(sum * A2.q[0].y), v[1], own.y);
+        v[2] = fmaf(exp2_fast(sum * A2.q[1].x), v[2], own.z);
+        v[3] = fmaf(exp2_fast(sum * A2.q[1].y), v[3], own.w);
+    }
+}
+
 // ---------------------------------------------------------------------------------------------- forward
 
-constexpr int NH_FORWARD = 256;
+constexpr int NH_FORWARD = 128;
 
 template <int L>
 constexpr int forward_smem_bytes()
 {
     using Q = Geo<L>;
-    return (int)sizeof(float) * 2 * (Q::KF * Q::CC * 7 + 2 * Q::KF * Q::NP);
+    return (int)sizeof(float) * 2 * (Q::KF * Q::CC * 5 + 2 * Q::KF * Q::NP);
 }
 
 template <typename T, int L, bool VEC>
-__global__ void __launch_bounds__(Geo<L>::NT + NH_FORWARD) sel_forward_kernel(const SelArgs a)
+__global__ void __launch_bounds__(Geo<L>::NT + NH_FORWARD, 2) sel_forward_kernel(const SelArgs a)
 {
     using Q = Geo<L>;
     constexpr int K = Q::KF, CC = Q::CC, NT = Q::NT, NP = Q::NP, NH = NH_FORWARD;
     extern __shared__ float smem[];
-    float4 *s_in = reinterpret_cast<float4 *>(smem);       // [2][K][CC]: dt twice, dt x twice (pairs as the arithmetic takes them)
-    float *s_skip = smem + 8 * K * CC, *s_gate = s_skip + 2 * K * CC;      // [2][K][CC]: D x, silu(z)
+    float2 *s_in = reinterpret_cast<float2 *>(smem);       // [2][K][CC]: dt, dt x
+    float *s_skip = smem + 4 * K * CC, *s_gate = s_skip + 2 * K * CC;      // [2][K][CC]: D x, silu(z)
     float *s_y = s_gate + 2 * K * CC;                      // [2][K][CC]
     float *s_b = s_y + 2 * K * CC, *s_c = s_b + 2 * K * NP;      // [2][K][NP]
     const Block<K, CC> blk(a);
@@ -270,7 +308,7 @@ __global__ void __launch_bounds__(Geo<L>::NT + NH_FORWARD) sel_forward_kernel(co
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     const float x = f.x[i].get(j), u = d[j] * x;
-                    s_in[buf + r * CC + place_of(part.col + j)] = make_float4(d[j], d[j], u, u);
+                    s_in[at + j] = make_float2(d[j], u);
                     sk.v[j] = skip[j] * x;
                     ga.v[j] = a.z.p ? silu_f(f.z[i].get(j)) : 1.0f;
                 }
@@ -322,86 +360,99 @@ __global__ void __launch_bounds__(Geo<L>::NT + NH_FORWARD) sel_forward_kernel(co
         return;
     }
 
-    constexpr int GS = L < SEL_CHUNK ? L : SEL_CHUNK;      // steps whose readouts are summed over the lanes together
-    const int tid = threadIdx.x, c = tid / L, l = tid % L, n0 = 4 * l;
-    const bool alive = blk.w.ch0 + c < blk.per;
-    const int m = blk.w.g * blk.per + blk.w.ch0 + c;
+    using R = Pair<L, SEL_CHUNK>;
+    constexpr int GS = R::GS;
+    const R pair(threadIdx.x);
+    const int n0 = 4 * pair.l;
     const int64_t nchunks = (a.T + SEL_CHUNK - 1) / SEL_CHUNK;
-    Quad A2, h;
-    {
-        float r[4] = {0.f, 0.f, 0.f, 0.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
-        if (alive) {
-            load_rates(r, a.A + (int64_t)m * a.N, n0, a.N);
-            if (a.segments > 1) load_states(s, a.seg_h + ((blk.w.b * a.segments + blk.w.seg) * a.M + m) * NP, n0, NP);
-            else if (a.h0) load_states(s, a.h0 + (blk.w.b * a.M + m) * a.N, n0, a.N);
-        }
-        A2.set(r);
-        h.set(s);
+    Quad A2[2], h[2];
+    float *ckpt[2];
 #pragma unroll
-        for (int q = 0; q < 2; ++q) A2.q[q] = mul2(A2.q[q], both(LOG2E));
+    for (int k = 0; k < 2; ++k) {
+        const int c = pair.channel(k), m = blk.w.g * blk.per + blk.w.ch0 + c;
+        const bool alive = blk.w.ch0 + c < blk.per;
+        float r[4] = {0.f, 0.f, 0.f, 0.f}, v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (alive) load_rates(r, a.A + (int64_t)m * a.N, n0, a.N);
+        A2[k].set(r);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) A2[k].q[q] = mul2(A2[k].q[q], both(LOG2E));
+        if (alive) enter<false, NP>(v, a, blk.w, m, n0, A2[k]);
+        h[k].set(v);
+        ckpt[k] = a.ckpt && alive ? a.ckpt + ((blk.w.b * nchunks + blk.t_lo / SEL_CHUNK) * a.M + m) * NP + n0 : nullptr;
     }
-    float *ckpt = a.ckpt ? a.ckpt + ((blk.w.b * nchunks + blk.t_lo / SEL_CHUNK) * a.M + m) * NP : nullptr;
-    for (int64_t k = 0; k < blk.count; ++k) {
+    for (int64_t j = 0; j < blk.count; ++j) {
         meet<NT + NH>();
-        const float4 *in = s_in + (k & 1) * K * CC + place_of(c);
-        const float *b = s_b + (k & 1) * K * NP + n0, *cc = s_c + (k & 1) * K * NP + n0;
-        float *y = s_y + (k & 1) * K * CC + c;
-        const int steps = blk.steps(k);
+        const float2 *in = s_in + (j & 1) * K * CC;
+        const float *b = s_b + (j & 1) * K * NP + n0, *cc = s_c + (j & 1) * K * NP + n0;
+        float *y = s_y + (j & 1) * K * CC;
+        const int steps = blk.steps(j);
 #pragma unroll
         for (int t0 = 0; t0 < K; t0 += GS) {
-            if (t0 % SEL_CHUNK == 0 && ckpt) {
-                if (alive && t0 < steps) *reinterpret_cast<float4 *>(ckpt + n0) = make_float4(h.q[0].x, h.q[0].y, h.q[1].x, h.q[1].y);
-                ckpt += (int64_t)a.M * NP;
+            if (t0 % SEL_CHUNK == 0) {
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    if (ckpt[k]) {
+                        if (t0 < steps) *reinterpret_cast<float4 *>(ckpt[k]) = make_float4(h[k].q[0].x, h[k].q[0].y, h[k].q[1].x, h[k].q[1].y);
+                        ckpt[k] += (int64_t)a.M * NP;
+                    }
             }
             float v[GS];
 #pragma unroll
             for (int i = 0; i < GS; ++i) {
                 const int t = t0 + i;
-                const float4 d4 = in[t * CC];
                 const float4 b4 = *reinterpret_cast<const float4 *>(b + t * NP), c4 = *reinterpret_cast<const float4 *>(cc + t * NP);
                 const float2 bb[2] = {low(b4), high(b4)}, ccv[2] = {low(c4), high(c4)};
-                float2 sum;
+                float sum[2];
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const float2 e = mul2(low(d4), A2.q[q]);
-                    h.q[q] = fma2(make_float2(exp2_fast(e.x), exp2_fast(e.y)), h.q[q], mul2(high(d4), bb[q]));
-                    sum = q ? fma2(ccv[q], h.q[q], sum) : mul2(ccv[q], h.q[q]);
+                for (int k = 0; k < 2; ++k) {
+                    const float2 d = in[t * CC + pair.channel(k)];
+                    float2 s;
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const float2 e = mul2(both(d.x), A2[k].q[q]);
+                        h[k].q[q] = fma2(make_float2(exp2_fast(e.x), exp2_fast(e.y)), h[k].q[q], mul2(both(d.y), bb[q]));
+                        s = q ? fma2(ccv[q], h[k].q[q], s) : mul2(ccv[q], h[k].q[q]);
+                    }
+                    sum[k] = s.x + s.y;
                 }
-                v[i] = sum.x + sum.y;
+                v[i] = R::exchange(sum[0], sum[1]);
             }
-            reduce_scatter<GS, L, 1>(v, tid);
-            if (writes_total<GS, L>(l)) y[(t0 + first_of<GS, L>(l)) * CC] = v[0];
+            pair.total(v, y, CC, t0);
         }
     }
     meet<NT + NH>();
-    if (alive && blk.w.seg == a.segments - 1) {
-        float s[4];
-        h.get(s);
-        store_states(a.h_last + (blk.w.b * a.M + m) * a.N, s, n0, a.N);
+    if (blk.w.seg == a.segments - 1) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int c = blk.w.ch0 + pair.channel(k);
+            float v[4];
+            h[k].get(v);
+            if (c < blk.per) store_states(a.h_last + (blk.w.b * a.M + blk.w.g * blk.per + c) * a.N, v, n0, a.N);
+        }
     }
 }
 
 // ---------------------------------------------------------------------------------------------- time split
 
-constexpr int NH_STATE = 256;
+constexpr int NH_STATE = 128;
 
 template <int L>
 constexpr int state_smem_bytes()
 {
     using Q = Geo<L>;
-    return (int)sizeof(float) * 2 * (Q::KF * Q::CC * 4 + Q::KF * Q::NP);
+    return (int)sizeof(float) * 2 * (Q::KF * Q::CC * 2 + Q::KF * Q::NP);
 }
 
 // What a piece of time hands on when nothing enters it, and its sum of step sizes: the state behind its last step, or
 // (REVERSE) the gradient that goes to the step in front of its first one.
 template <typename T, int L, bool VEC, bool REVERSE>
-__global__ void __launch_bounds__(Geo<L>::NT + NH_STATE) sel_state_kernel(const SelArgs a)
+__global__ void __launch_bounds__(Geo<L>::NT + NH_STATE, 2) sel_state_kernel(const SelArgs a)
 {
     using Q = Geo<L>;
     constexpr int K = Q::KF, CC = Q::CC, NT = Q::NT, NP = Q::NP, NH = NH_STATE;
     extern __shared__ float smem[];
-    float4 *s_in = reinterpret_cast<float4 *>(smem);      // [2][K][CC]: dt twice, and dt x or p twice
-    float *s_w = smem + 8 * K * CC;                       // [2][K][NP]: B or C
+    float2 *s_in = reinterpret_cast<float2 *>(smem);      // [2][K][CC]: dt, and dt x or p
+    float *s_w = smem + 4 * K * CC;                       // [2][K][NP]: B or C
     const Block<K, CC> blk(a);
     if (blk.w.seg == (REVERSE ? 0 : a.segments - 1)) return;      // nobody comes after it
 
@@ -440,7 +491,7 @@ __global__ void __launch_bounds__(Geo<L>::NT + NH_STATE) sel_state_kernel(const 
                     float v = f.w[i].get(j);
                     if (!REVERSE) v *= d[j];
                     else if (gated) v *= silu_f(f.z[i].get(j));
-                    s_in[buf + r * CC + place_of(part.col + j)] = make_float4(d[j], d[j], v, v);
+                    s_in[buf + r * CC + part.col + j] = make_float2(d[j], v);
                 }
             }
             f.g.stage(s_w + (k & 1) * K * NP, tid);
@@ -461,67 +512,52 @@ __global__ void __launch_bounds__(Geo<L>::NT + NH_STATE) sel_state_kernel(const 
         return;
     }
 
-    const int tid = threadIdx.x, c = tid / L, l = tid % L, n0 = 4 * l;
-    const bool alive = blk.w.ch0 + c < blk.per;
-    const int m = blk.w.g * blk.per + blk.w.ch0 + c;
-    Quad A2, h;
-    {
+    const Pair<L, K> pair(threadIdx.x);
+    const int n0 = 4 * pair.l;
+    Quad A2[2], h[2];
+    float dt_sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int c = blk.w.ch0 + pair.channel(k);
         float r[4] = {0.f, 0.f, 0.f, 0.f};
-        if (alive) load_rates(r, a.A + (int64_t)m * a.N, n0, a.N);
-        A2.set(r);
+        if (c < blk.per) load_rates(r, a.A + (int64_t)(blk.w.g * blk.per + c) * a.N, n0, a.N);
+        A2[k].set(r);
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-            A2.q[q] = mul2(A2.q[q], both(LOG2E));
-            h.q[q] = both(0.0f);
+            A2[k].q[q] = mul2(A2[k].q[q], both(LOG2E));
+            h[k].q[q] = both(0.0f);
         }
     }
-    float dt_sum = 0.0f;
-    for (int64_t k = 0; k < blk.count; ++k) {
+    for (int64_t j = 0; j < blk.count; ++j) {
         meet<NT + NH>();
-        const float4 *in = s_in + (k & 1) * K * CC + place_of(c);
-        const float *w = s_w + (k & 1) * K * NP + n0;
+        const float2 *in = s_in + (j & 1) * K * CC;
+        const float *w = s_w + (j & 1) * K * NP + n0;
 #pragma unroll
         for (int i = 0; i < K; ++i) {
             const int t = REVERSE ? K - 1 - i : i;
-            const float4 d4 = in[t * CC];
             const float4 w4 = *reinterpret_cast<const float4 *>(w + t * NP);
             const float2 ww[2] = {low(w4), high(w4)};
-            dt_sum += d4.x;
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const float2 e = mul2(low(d4), A2.q[q]), f = make_float2(exp2_fast(e.x), exp2_fast(e.y));
-                h.q[q] = REVERSE ? mul2(f, fma2(ww[q], high(d4), h.q[q])) : fma2(f, h.q[q], mul2(high(d4), ww[q]));
+            for (int k = 0; k < 2; ++k) {
+                const float2 d = in[t * CC + pair.channel(k)];
+                dt_sum[k] += d.x;
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const float2 e = mul2(both(d.x), A2[k].q[q]), f = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                    h[k].q[q] = REVERSE ? mul2(f, fma2(ww[q], both(d.y), h[k].q[q])) : fma2(f, h[k].q[q], mul2(both(d.y), ww[q]));
+                }
             }
         }
     }
-    if (alive) {
-        float s[4];
-        h.get(s);
-        store_states(a.seg_h + ((blk.w.b * a.segments + blk.w.seg) * a.M + m) * NP, s, n0, NP);
-        if (l == 0) a.seg_dt[(blk.w.b * a.segments + blk.w.seg) * a.M + m] = dt_sum;
-    }
-}
-
-// Turns what every piece hands on by itself into what enters it, in place: from the first piece to the last, or
-// (REVERSE, gradients) the other way.  One thread per state.
-template <bool REVERSE>
-__global__ void sel_carry_kernel(const SelArgs a, int NP)
-{
-    const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
-    if (i >= a.B * a.M * NP) return;
-    const int n = (int)(i % NP);
-    const int64_t bm = i / NP, b = bm / a.M, m = bm % a.M;
-    const float *start = REVERSE ? a.dh_last : a.h0;
-    float carry = (start && n < a.N) ? start[bm * a.N + n] : 0.0f;
-    const float A2 = n < a.N ? min_nan(max_nan(a.A[m * a.N + n], -2.0e38f), 2.0e38f) * LOG2E : 0.0f;
-#pragma unroll 4
-    for (int k = 0; k < a.segments; ++k) {
-        const int s = REVERSE ? a.segments - 1 - k : k;
-        const int64_t at = (b * a.segments + s) * a.M + m;
-        const bool more = k < a.segments - 1;
-        const float own = more ? a.seg_h[at * NP + n] : 0.0f, sum = more ? a.seg_dt[at] : 0.0f;
-        a.seg_h[at * NP + n] = carry;
-        carry = fmaf(exp2_fast(sum * A2), carry, own);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int c = blk.w.ch0 + pair.channel(k);
+        if (c >= blk.per) continue;
+        const int64_t at = (blk.w.b * a.segments + blk.w.seg) * a.M + blk.w.g * blk.per + c;
+        float v[4];
+        h[k].get(v);
+        store_states(a.seg_h + at * NP, v, n0, NP);
+        if (pair.l == 0) a.seg_dt[at] = dt_sum[k];
     }
 }
 
@@ -535,7 +571,7 @@ template <int L> struct Across {
     static constexpr int CW = 32 / L;
     static constexpr int PERM = CW >= 4 ? 4 : CW;               // orders (powers of two; 1: none)
     static constexpr int REST = CW / PERM;                      // lanes left to sum over after the states
-    static constexpr int SC = REST < SEL_CHUNK ? REST : SEL_CHUNK;
+    static constexpr int SC = REST;                             // consecutive steps whose sums share the other exchanges
     static constexpr int KEPT = 4 / PERM;                       // states that a lane is left with
     static constexpr int COPIES = PERM == 2 ? 4 : PERM;         // of a staged row; the orders 0 and 2 leave two unused
     // order of a lane's states: its two highest channel bits, the highest exchanges the pairs
@@ -561,30 +597,33 @@ __device__ __forceinline__ void reorder(float (&v)[4], int order)
 }
 
 constexpr int KB = SEL_CHUNK, NH_BACKWARD = 128;
+constexpr int KH = KB / 2;      // steps whose decays and states are in registers at a time
 
 template <int L>
 constexpr int backward_smem_bytes()
 {
     using Q = Geo<L>;
-    return (int)sizeof(float) * 2 * (KB * Q::CC * 12 + 2 * KB * Across<L>::COPIES * Q::NP + Q::WARPS * KB * 2 * Q::NP);
+    return (int)sizeof(float) * 2 * (KB * Q::CC * 9 + 2 * KB * Across<L>::COPIES * Q::NP + Q::WARPS * KB * 2 * Q::NP);
 }
 
-// Walks its piece of time backwards.  In each chunk it rebuilds the states from the chunk's checkpoint, keeping the
-// decays a_t and the decayed states a_t h_{t-1} in registers, and then runs the reverse recurrence
-// g_t = C_t p_t + a_{t+1} g_{t+1}  (p = dy silu(z)) on them, so that every exponential is formed once.
+// Walks its piece of time backwards.  It rebuilds the states of half a chunk from the chunk's checkpoint, keeping them and
+// the decays a_t in registers, and runs the reverse recurrence  g_t = C_t p_t + a_{t+1} g_{t+1}  (p = dy silu(z)) on them.
+// The chunk's later half comes first, for which its earlier half is run through once more: a quarter more exponentials,
+// and registers for two blocks on an SM, whose barriers then do not stop all of it.  The launch gives every thread 128
+// registers, of which the preparing warps hand 40 to those of the recurrence.
 template <typename T, int L, bool VEC>
-__global__ void __launch_bounds__(Geo<L>::NT + NH_BACKWARD) sel_backward_kernel(const SelArgs a)
+__global__ void __launch_bounds__(Geo<L>::NT + NH_BACKWARD, 2) sel_backward_kernel(const SelArgs a)
 {
     using Q = Geo<L>;
     using X = Across<L>;
     constexpr int CC = Q::CC, NT = Q::NT, NP = Q::NP, NH = NH_BACKWARD, COPIES = X::COPIES;
     extern __shared__ float smem[];
-    float4 *s_in = reinterpret_cast<float4 *>(smem);      // [2][KB][CC]: dt twice, dt x twice
-    float2 *s_p = reinterpret_cast<float2 *>(smem + 8 * KB * CC);      // [2][KB][CC]: p twice
-    float *s_x = smem + 12 * KB * CC;                     // [2][KB][CC]: x
+    float2 *s_in = reinterpret_cast<float2 *>(smem);      // [2][KB][CC]: dt, dt x
+    float *s_p = smem + 4 * KB * CC;                      // [2][KB][CC]: p
+    float *s_x = s_p + 2 * KB * CC;                       // x
     float *s_s = s_x + 2 * KB * CC;                       // slope of the step size
     float *s_q = s_s + 2 * KB * CC;                       // dy times the slope of silu(z)
-    float *s_y = s_q + 2 * KB * CC, *s_gb = s_y + 2 * KB * CC, *s_ga = s_gb + 2 * KB * CC;      // sums over the states: C h, g B, g a h A
+    float *s_y = s_q + 2 * KB * CC, *s_gb = s_y + 2 * KB * CC, *s_ga = s_gb + 2 * KB * CC;      // sums over the states: C h, g B, g a h A log2(e)
     float *s_b = s_ga + 2 * KB * CC, *s_c = s_b + 2 * KB * COPIES * NP;              // [2][KB][COPIES][NP]
     float *s_bc = s_c + 2 * KB * COPIES * NP;             // [2][warp][KB][B, C][NP]
     const Block<KB, CC> blk(a);
@@ -595,6 +634,7 @@ __global__ void __launch_bounds__(Geo<L>::NT + NH_BACKWARD) sel_backward_kernel(
         using P = Part<KB, CC, NH>;
         constexpr int V = P::V, ITEMS = P::I::ITEMS, ROWS = P::I::ROWS, COLS = P::I::COLS;
         using F = Pack<float, V>;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         const int tid = threadIdx.x - NT;
         const P part(blk, tid);
         float skip[V], bias[V], dD[V], dbias[V];
@@ -625,11 +665,11 @@ __global__ void __launch_bounds__(Geo<L>::NT + NH_BACKWARD) sel_backward_kernel(
                 if (r >= KB) continue;
                 float d[V], pre[V];
                 step_sizes(d, pre, f.dt[i], bias, a.softplus, part.there(steps, r));
-                F fx, fs, fq;
+                F fx, fs, fq, fp;
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     const float x = f.x[i].get(j), up = f.dy[i].get(j), u = d[j] * x;
-                    s_in[buf + r * CC + place_of(part.col + j)] = make_float4(d[j], d[j], u, u);
+                    s_in[at + j] = make_float2(d[j], u);
                     fx.v[j] = x;
                     fs.v[j] = a.softplus ? sigmoid_f(pre[j]) : 1.0f;
                     float p = up;
@@ -638,8 +678,9 @@ __global__ void __launch_bounds__(Geo<L>::NT + NH_BACKWARD) sel_backward_kernel(
                         p = up * gate;
                         fq.v[j] = up * fmaf(gate, 1.0f - sg, sg);
                     }
-                    s_p[at + j] = both(p);
+                    fp.v[j] = p;
                 }
+                *reinterpret_cast<F *>(s_p + at) = fp;
                 *reinterpret_cast<F *>(s_x + at) = fx;
                 *reinterpret_cast<F *>(s_s + at) = fs;
                 if (gated) *reinterpret_cast<F *>(s_q + at) = fq;
@@ -664,7 +705,8 @@ __global__ void __launch_bounds__(Geo<L>::NT + NH_BACKWARD) sel_backward_kernel(
                 const int r = part.row + i * ROWS, have = part.there(steps, r), at = buf + r * CC + part.col;
                 if (have <= 0) continue;
                 const F fx = *reinterpret_cast<const F *>(s_x + at), fs = *reinterpret_cast<const F *>(s_s + at),
-                        fb = *reinterpret_cast<const F *>(s_gb + at), fa = *reinterpret_cast<const F *>(s_ga + at);
+                        fb = *reinterpret_cast<const F *>(s_gb + at), fa = *reinterpret_cast<const F *>(s_ga + at),
+                        fp = *reinterpret_cast<const F *>(s_p + at);
                 F fq, fy;
                 if (gated) {
                     fq = *reinterpret_cast<const F *>(s_q + at);
@@ -673,9 +715,9 @@ __global__ void __launch_bounds__(Geo<L>::NT + NH_BACKWARD) sel_backward_kernel(
                 Pack<T, V> ox, od, oz;
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    const float p = s_p[at + j].x, x = fx.v[j];
-                    const float d = fmaf(fb.v[j], x, fa.v[j]) * fs.v[j];
-                    ox.v[j] = from_f32<T>(fmaf(s_in[buf + r * CC + place_of(part.col + j)].x, fb.v[j], skip[j] * p));
+                    const float p = fp.v[j], x = fx.v[j];
+                    const float d = fmaf(fb.v[j], x, fa.v[j] * LN2) * fs.v[j];
+                    ox.v[j] = from_f32<T>(fmaf(s_in[at + j].x, fb.v[j], skip[j] * p));
                     od.v[j] = from_f32<T>(d);
                     if (gated) oz.v[j] = from_f32<T>(fq.v[j] * fmaf(skip[j], x, fy.v[j]));
                     dD[j] = fmaf(p, x, dD[j]);
@@ -735,43 +777,53 @@ __global__ void __launch_bounds__(Geo<L>::NT + NH_BACKWARD) sel_backward_kernel(
         return;
     }
 
-    constexpr int GS = L < KB ? L : KB;             // steps whose sums over the lanes of a channel are formed together
-    constexpr int SC = X::SC;
-    static_assert(KB % GS == 0 && KB % SC == 0 && X::REST <= SC, "");
-    const int tid = threadIdx.x, c = tid / L, l = tid % L, n0 = 4 * l, warp = tid / 32, cw = tid % 32 / L;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    using R = Pair<L, KH>;
+    constexpr int GS = R::GS, SC = X::SC;
+    static_assert(KH % GS == 0 && KH % SC == 0 && X::REST <= SC, "");
+    const R pair(threadIdx.x);
+    const int n0 = 4 * pair.l, warp = threadIdx.x / 32, cw = threadIdx.x % 32 / L;
     const int order = X::order(cw);
-    const bool alive = blk.w.ch0 + c < blk.per;
-    const int m = blk.w.g * blk.per + blk.w.ch0 + c;
-    Quad A1, A2, g, dA;
-    {
-        float r[4] = {0.f, 0.f, 0.f, 0.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
-        if (alive) {
-            load_rates(r, a.A + (int64_t)m * a.N, n0, a.N);
-            if (a.segments > 1) load_states(s, a.seg_h + ((blk.w.b * a.segments + blk.w.seg) * a.M + m) * NP, n0, NP);
-            else if (a.dh_last) load_states(s, a.dh_last + (blk.w.b * a.M + m) * a.N, n0, a.N);
-        }
+    Quad A2[2], g[2], dA[2];
+    float4 state[2];      // the chunk's checkpoint
+    const float *ckpt[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int c = blk.w.ch0 + pair.channel(k), m = blk.w.g * blk.per + c;
+        float r[4] = {0.f, 0.f, 0.f, 0.f}, v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (c < blk.per) load_rates(r, a.A + (int64_t)m * a.N, n0, a.N);
+        Quad A2_here;
+        A2_here.set(r);
         reorder(r, order);
-        reorder(s, order);
-        A1.set(r);
-        g.set(s);
+        A2[k].set(r);
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-            A2.q[q] = mul2(A1.q[q], both(LOG2E));
-            dA.q[q] = both(0.0f);
+            A2_here.q[q] = mul2(A2_here.q[q], both(LOG2E));
+            A2[k].q[q] = mul2(A2[k].q[q], both(LOG2E));
+            dA[k].q[q] = both(0.0f);
         }
+        if (c < blk.per) enter<true, NP>(v, a, blk.w, m, n0, A2_here);
+        reorder(v, order);
+        g[k].set(v);
+        state[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        ckpt[k] = c < blk.per ? a.ckpt + ((blk.w.b * nchunks + blk.t_lo / SEL_CHUNK + blk.count - 1) * a.M + m) * NP + n0 : nullptr;
     }
-    float4 state = make_float4(0.f, 0.f, 0.f, 0.f);      // checkpoint of the next chunk
-    auto fetch_state = [&](int64_t k) {
-        if (k >= 0 && alive) state = *reinterpret_cast<const float4 *>(a.ckpt + ((blk.w.b * nchunks + blk.t_lo / SEL_CHUNK + k) * a.M + m) * NP + n0);
+    auto fetch_state = [&](bool there) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (there && ckpt[k]) {
+                state[k] = *reinterpret_cast<const float4 *>(ckpt[k]);
+                ckpt[k] -= (int64_t)a.M * NP;
+            }
     };
-    fetch_state(blk.count - 1);
-    for (int64_t k = blk.count - 1; k >= 0; --k) {
+    fetch_state(blk.count > 0);
+    for (int64_t j = blk.count - 1; j >= 0; --j) {
         meet<NT + NH>();
-        const float4 *in = s_in + (k & 1) * KB * CC + place_of(c);
-        const float2 *p = s_p + (k & 1) * KB * CC + c;
-        const float *b = s_b + ((k & 1) * KB * COPIES + order) * NP + n0, *cc = s_c + ((k & 1) * KB * COPIES + order) * NP + n0;
-        float *y_out = s_y + (k & 1) * KB * CC + c, *gb_out = s_gb + (k & 1) * KB * CC + c, *ga_out = s_ga + (k & 1) * KB * CC + c;
-        float *bc_out = s_bc + ((k & 1) * Q::WARPS + warp) * KB * 2 * NP + n0;
+        const float2 *in = s_in + (j & 1) * KB * CC;
+        const float *p = s_p + (j & 1) * KB * CC;
+        const float *b = s_b + ((j & 1) * KB * COPIES + order) * NP + n0, *cc = s_c + ((j & 1) * KB * COPIES + order) * NP + n0;
+        float *y_out = s_y + (j & 1) * KB * CC, *gb_out = s_gb + (j & 1) * KB * CC, *ga_out = s_ga + (j & 1) * KB * CC;
+        float *bc_out = s_bc + ((j & 1) * Q::WARPS + warp) * KB * 2 * NP + n0;
         // Leaves the warp's totals of `v`, gathered over SC steps from t on, in row `which` (B, C) of the steps.
         auto across = [&](Quad (&v)[SC], int t, int which) {
 #pragma unroll
@@ -780,7 +832,7 @@ __global__ void __launch_bounds__(Geo<L>::NT + NH_BACKWARD) sel_backward_kernel(
                 float s[SC];
 #pragma unroll
                 for (int i = 0; i < SC; ++i) s[i] = v[i].q[0].x;
-                reduce_scatter<SC, X::REST, L>(s, tid);
+                reduce_scatter<SC, X::REST, L>(s, threadIdx.x);
                 bc_out[((t + cw % X::REST) * 2 + which) * NP + order] = s[0];
             } else {
                 float s[4];
@@ -789,88 +841,111 @@ __global__ void __launch_bounds__(Geo<L>::NT + NH_BACKWARD) sel_backward_kernel(
                 for (int i = 0; i < X::KEPT; ++i) bc_out[(t * 2 + which) * NP + (i ^ order)] = s[i];
             }
         };
-
-        Quad av[KB], ah[KB];
-        {      // forward through the chunk: decays, decayed states, readout, gradient of C
-            Quad h;
-            {
-                float s[4] = {state.x, state.y, state.z, state.w};
-                reorder(s, order);
-                h.set(s);
+#pragma unroll 1      // unrolled, the halves are interleaved beyond what the registers hold
+        for (int half = 1; half >= 0; --half) {
+            Quad h[2], av[KH][2], before[KH][2];      // decays, and the states in front of the steps
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                float v[4] = {state[k].x, state[k].y, state[k].z, state[k].w};
+                reorder(v, order);
+                h[k].set(v);
             }
-            fetch_state(k - 1);
-            float y[GS];
-            Quad vc[SC];
+            if (half == 1) {
 #pragma unroll
-            for (int t = 0; t < KB; ++t) {
-                const float4 d4 = in[t * CC];
-                const float2 pt = p[t * CC];
-                const float4 b4 = *reinterpret_cast<const float4 *>(b + t * COPIES * NP);
-                const float2 bb[2] = {low(b4), high(b4)};
+                for (int t = 0; t < KH; ++t) {
+                    const float4 b4 = *reinterpret_cast<const float4 *>(b + t * COPIES * NP);
+                    const float2 bb[2] = {low(b4), high(b4)};
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const float2 e = mul2(low(d4), A2.q[q]);
-                    av[t].q[q] = make_float2(exp2_fast(e.x), exp2_fast(e.y));
-                    ah[t].q[q] = mul2(av[t].q[q], h.q[q]);
-                    h.q[q] = fma2(high(d4), bb[q], ah[t].q[q]);
-                    vc[t % SC].q[q] = mul2(pt, h.q[q]);
-                }
-                // also without a gate: a branch would end the run of instructions that the scheduler can interleave
-                const float4 c4 = *reinterpret_cast<const float4 *>(cc + t * COPIES * NP);
-                const float2 sum = fma2(high(c4), h.q[1], mul2(low(c4), h.q[0]));
-                y[t % GS] = sum.x + sum.y;
-                if (t % GS == GS - 1) {
-                    reduce_scatter<GS, L, 1>(y, tid);
-                    if (writes_total<GS, L>(l)) y_out[(t - (GS - 1) + first_of<GS, L>(l)) * CC] = y[0];
-                }
-                if (t % SC == SC - 1) across(vc, t - (SC - 1), 1);
-            }
-        }
-        {      // backward through it
-            float sb[GS], sa[GS];
-            Quad vb[SC], dA_c;
-            dA_c.q[0] = dA_c.q[1] = both(0.0f);
+                    for (int k = 0; k < 2; ++k) {
+                        const float2 d = in[t * CC + pair.channel(k)];
 #pragma unroll
-            for (int t = KB - 1; t >= 0; --t) {
-                const float4 d4 = in[t * CC];
-                const float2 pt = p[t * CC];
-                const float4 b4 = *reinterpret_cast<const float4 *>(b + t * COPIES * NP), c4 = *reinterpret_cast<const float4 *>(cc + t * COPIES * NP);
-                const float2 bb[2] = {low(b4), high(b4)}, ccv[2] = {low(c4), high(c4)};
-                float2 rb, ra;
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    g.q[q] = fma2(ccv[q], pt, g.q[q]);
-                    vb[t % SC].q[q] = mul2(g.q[q], high(d4));
-                    rb = q ? fma2(g.q[q], bb[q], rb) : mul2(g.q[q], bb[q]);
-                    const float2 u = mul2(g.q[q], ah[t].q[q]);
-                    ra = q ? fma2(u, A1.q[q], ra) : mul2(u, A1.q[q]);
-                    dA_c.q[q] = fma2(u, low(d4), dA_c.q[q]);
-                    g.q[q] = mul2(g.q[q], av[t].q[q]);
-                }
-                sb[t % GS] = rb.x + rb.y;
-                sa[t % GS] = ra.x + ra.y;
-                if (t % GS == 0) {
-                    reduce_scatter<GS, L, 1>(sb, tid);
-                    reduce_scatter<GS, L, 1>(sa, tid);
-                    if (writes_total<GS, L>(l)) {
-                        gb_out[(t + first_of<GS, L>(l)) * CC] = sb[0];
-                        ga_out[(t + first_of<GS, L>(l)) * CC] = sa[0];
+                        for (int q = 0; q < 2; ++q) {
+                            const float2 e = mul2(both(d.x), A2[k].q[q]);
+                            h[k].q[q] = fma2(make_float2(exp2_fast(e.x), exp2_fast(e.y)), h[k].q[q], mul2(both(d.y), bb[q]));
+                        }
                     }
                 }
-                if (t % SC == 0) across(vb, t, 0);
+            } else {
+                fetch_state(j > 0);
             }
+            {      // forward: decays, states, readout (also without a gate, a branch would keep the steps apart), gradient of C
+                float y[GS];
+                Quad vc[SC];
 #pragma unroll
-            for (int q = 0; q < 2; ++q) dA.q[q] = add2(dA.q[q], dA_c.q[q]);
+                for (int i = 0; i < KH; ++i) {
+                    const int t = half * KH + i;
+                    const float4 b4 = *reinterpret_cast<const float4 *>(b + t * COPIES * NP), c4 = *reinterpret_cast<const float4 *>(cc + t * COPIES * NP);
+                    const float2 bb[2] = {low(b4), high(b4)};
+                    float sum[2];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const float2 d = in[t * CC + pair.channel(k)];
+                        const float pt = p[t * CC + pair.channel(k)];
+                        before[i][k] = h[k];
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            const float2 e = mul2(both(d.x), A2[k].q[q]);
+                            av[i][k].q[q] = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                            h[k].q[q] = fma2(av[i][k].q[q], h[k].q[q], mul2(both(d.y), bb[q]));
+                            vc[i % SC].q[q] = k ? fma2(both(pt), h[k].q[q], vc[i % SC].q[q]) : mul2(both(pt), h[k].q[q]);
+                        }
+                        const float2 s = fma2(high(c4), h[k].q[1], mul2(low(c4), h[k].q[0]));
+                        sum[k] = s.x + s.y;
+                    }
+                    y[i % GS] = R::exchange(sum[0], sum[1]);
+                    if (i % GS == GS - 1) pair.total(y, y_out, CC, t - (GS - 1));
+                    if (i % SC == SC - 1) across(vc, t - (SC - 1), 1);
+                }
+            }
+            {      // backward
+                float sb[GS], sa[GS];
+                Quad vb[SC];
+#pragma unroll
+                for (int i = KH - 1; i >= 0; --i) {
+                    const int t = half * KH + i;
+                    const float4 b4 = *reinterpret_cast<const float4 *>(b + t * COPIES * NP), c4 = *reinterpret_cast<const float4 *>(cc + t * COPIES * NP);
+                    const float2 bb[2] = {low(b4), high(b4)}, ccv[2] = {low(c4), high(c4)};
+                    float tb[2], ta[2];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const float2 d = in[t * CC + pair.channel(k)];
+                        const float pt = p[t * CC + pair.channel(k)];
+                        float2 rb, ra;
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            g[k].q[q] = fma2(ccv[q], both(pt), g[k].q[q]);
+                            vb[i % SC].q[q] = k ? fma2(g[k].q[q], both(d.y), vb[i % SC].q[q]) : mul2(g[k].q[q], both(d.y));
+                            rb = q ? fma2(g[k].q[q], bb[q], rb) : mul2(g[k].q[q], bb[q]);
+                            g[k].q[q] = mul2(g[k].q[q], av[i][k].q[q]);
+                            const float2 u = mul2(g[k].q[q], before[i][k].q[q]);
+                            ra = q ? fma2(u, A2[k].q[q], ra) : mul2(u, A2[k].q[q]);
+                            dA[k].q[q] = fma2(u, both(d.x), dA[k].q[q]);
+                        }
+                        tb[k] = rb.x + rb.y;
+                        ta[k] = ra.x + ra.y;
+                    }
+                    sb[i % GS] = R::exchange(tb[0], tb[1]);
+                    sa[i % GS] = R::exchange(ta[0], ta[1]);
+                    if (i % GS == 0) {
+                        pair.total(sb, gb_out, CC, t);
+                        pair.total(sa, ga_out, CC, t);
+                    }
+                    if (i % SC == 0) across(vb, t, 0);
+                }
+            }
         }
     }
     meet<NT + NH>();
-    if (alive) {
-        float s[4], r[4];
-        dA.get(s);
-        g.get(r);
-        reorder(s, order);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int c = blk.w.ch0 + pair.channel(k), m = blk.w.g * blk.per + c;
+        if (c >= blk.per) continue;
+        float v[4], r[4];
+        dA[k].get(v);
+        g[k].get(r);
+        reorder(v, order);
         reorder(r, order);
-        store_states(a.part_a + ((blk.w.b * a.segments + blk.w.seg) * a.M + m) * NP, s, n0, NP);
+        store_states(a.part_a + ((blk.w.b * a.segments + blk.w.seg) * a.M + m) * NP, v, n0, NP);
         if (a.dh0 && blk.w.seg == 0) store_states(a.dh0 + (blk.w.b * a.M + m) * a.N, r, n0, a.N);
     }
 }
@@ -967,15 +1042,14 @@ cudaError_t allow_smem(K kernel, int bytes)
     return bytes > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) : cudaSuccess;
 }
 
-// What enters every piece of time.
+// What every piece of time hands on.
 template <typename T, int L, bool VEC, bool REVERSE>
-cudaError_t enter_pieces(const SelArgs &a, const SelPlan &p, unsigned grid, cudaStream_t s)
+cudaError_t piece_states(const SelArgs &a, unsigned grid, cudaStream_t s)
 {
     constexpr int smem = state_smem_bytes<L>();
     cudaError_t e = allow_smem(sel_state_kernel<T, L, VEC, REVERSE>, smem);
     if (e != cudaSuccess) return e;
     sel_state_kernel<T, L, VEC, REVERSE><<<grid, Geo<L>::NT + NH_STATE, smem, s>>>(a);
-    sel_carry_kernel<REVERSE><<<(unsigned)ceil_div(a.B * a.M * p.NP, 128), 128, 0, s>>>(a, p.NP);
     return cudaGetLastError();
 }
 
@@ -985,7 +1059,7 @@ cudaError_t forward_typed(const SelArgs &a, const SelPlan &p, cudaStream_t s)
     const unsigned grid = (unsigned)(a.B * a.G * p.tiles * p.segments);
     constexpr int smem = forward_smem_bytes<L>();
     cudaError_t e = allow_smem(sel_forward_kernel<T, L, VEC>, smem);
-    if (e == cudaSuccess && p.segments > 1) e = enter_pieces<T, L, VEC, false>(a, p, grid, s);
+    if (e == cudaSuccess && p.segments > 1) e = piece_states<T, L, VEC, false>(a, grid, s);
     if (e != cudaSuccess) return e;
     sel_forward_kernel<T, L, VEC><<<grid, Geo<L>::NT + NH_FORWARD, smem, s>>>(a);
     return cudaGetLastError();
@@ -997,7 +1071,7 @@ cudaError_t backward_typed(const SelArgs &a, const SelPlan &p, cudaStream_t s)
     const unsigned grid = (unsigned)(a.B * a.G * p.tiles * p.segments);
     constexpr int smem = backward_smem_bytes<L>();
     cudaError_t e = allow_smem(sel_backward_kernel<T, L, VEC>, smem);
-    if (e == cudaSuccess && p.segments > 1) e = enter_pieces<T, L, VEC, true>(a, p, grid, s);
+    if (e == cudaSuccess && p.segments > 1) e = piece_states<T, L, VEC, true>(a, grid, s);
     if (e != cudaSuccess) return e;
     sel_backward_kernel<T, L, VEC><<<grid, Geo<L>::NT + NH_BACKWARD, smem, s>>>(a);
     return cudaGetLastError();
@@ -1009,7 +1083,6 @@ cudaError_t forward_dispatch(const SelArgs &a, const SelPlan &p, cudaStream_t s)
     const bool vec = (a.M / a.G) % 4 == 0 && pack_aligned<T>(a.x) && pack_aligned<T>(a.dt) && pack_aligned<T>(a.z) &&
                      reinterpret_cast<uintptr_t>(a.y) % (4 * sizeof(T)) == 0;
     switch (p.L) {
-    case 1: return vec ? forward_typed<T, 1, true>(a, p, s) : forward_typed<T, 1, false>(a, p, s);
     case 2: return vec ? forward_typed<T, 2, true>(a, p, s) : forward_typed<T, 2, false>(a, p, s);
     case 4: return vec ? forward_typed<T, 4, true>(a, p, s) : forward_typed<T, 4, false>(a, p, s);
     case 8: return vec ? forward_typed<T, 8, true>(a, p, s) : forward_typed<T, 8, false>(a, p, s);
@@ -1026,7 +1099,6 @@ cudaError_t backward_dispatch(const SelArgs &a, const SelPlan &p, void *dB, void
                       (4 * sizeof(T))) == 0;
     cudaError_t e;
     switch (p.L) {
-    case 1: e = vec ? backward_typed<T, 1, true>(a, p, s) : backward_typed<T, 1, false>(a, p, s); break;
     case 2: e = vec ? backward_typed<T, 2, true>(a, p, s) : backward_typed<T, 2, false>(a, p, s); break;
     case 4: e = vec ? backward_typed<T, 4, true>(a, p, s) : backward_typed<T, 4, false>(a, p, s); break;
     case 8: e = vec ? backward_typed<T, 8, true>(a, p, s) : backward_typed<T, 8, false>(a, p, s); break;
@@ -1073,15 +1145,16 @@ void place(SelArgs &a, const SelPlan &p, void *ws)
 SelPlan sel_plan(int64_t B, int64_t T, int M, int N, int G, bool backward)
 {
     SelPlan p{};
-    p.L = sel_lanes(N);
-    p.NP = 4 * p.L;
-    p.CC = sel_channels(p.L);
+    p.NP = sel_padded(N);
+    p.L = p.NP / 4;
+    p.CC = 256 / p.L;
     p.tiles = (int)ceil_div(M / G, p.CC);
     const int64_t blocks = B * G * p.tiles, unit = 16;
-    // A block per SM at least: split the time axis when there are fewer, down to pieces of 64 steps.
-    int64_t want = blocks >= 96 ? 1 : ceil_div(296, blocks);
-    const int64_t most = T / 64 > 1 ? T / 64 : 1;
-    if (want > most) want = most;
+    // Splitting the time axis costs a pass over the states of all pieces (half of the forward pass, a quarter of the
+    // backward one), so it has to bring more than 1.5 times the blocks: two on each of 148 SMs.  A piece is no shorter
+    // than 32 steps and than the number of pieces that its block has to fold.
+    int64_t want = blocks >= 96 ? 1 : 296 / blocks;
+    while (want > 1 && (T / want < 32 || T / want < want)) --want;
     p.seg = ceil_div(ceil_div(T, want), unit) * unit;
     p.segments = (int)ceil_div(T, p.seg);
     p.chunks = ceil_div(T, SEL_CHUNK);

@@ -26,7 +26,7 @@ struct SelArgs {
     float *part_bc;                      // [tiles][B][T][G][2][NP]
     float *part_a;                       // [B * segments][M][NP]
     float *part_d;                       // [B * segments][2][M]   (D, dt_bias)
-    // time split: `segments` pieces of `seg` steps; state (or gradient) entering each piece
+    // time split: `segments` pieces of `seg` steps; what each hands on (state or gradient), and its sum of step sizes
     int segments;
     int64_t seg;
     float *seg_h;                        // [B][segments][M][NP]
@@ -40,7 +40,9 @@ inline int sel_lanes(int N)
     while (4 * l < N) l *= 2;
     return l;
 }
-inline int sel_channels(int L) { return L == 1 ? 128 : 256 / L; }      // channels of a block
+
+// States of a channel as the scan's kernels keep them (the single step has no use for a second lane of padding).
+inline int sel_padded(int N) { const int l = sel_lanes(N); return 4 * (l < 2 ? 2 : l); }
 
 struct SelPlan {
     int L, NP, CC, tiles, segments;
