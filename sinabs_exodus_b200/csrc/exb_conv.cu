@@ -2,8 +2,9 @@
 //
 //   y_t[m] = act(bias[m] + sum_k w[m,k] x_{t-W+1+k}[m]),   x_{-1}, x_{-2}, ... from the state of the call before.
 //
-// Bound by memory: a thread owns a pack of neighbouring channels and a run of time steps, keeps the last W - 1 rows in
-// registers and so reads every row once, W - 1 rows per run twice.
+// Bound by memory: a thread owns V neighbouring channels and a run of time steps.  It takes STEP rows at a time, with the
+// next STEP already on their way, and keeps the W - 1 rows in front of them in registers, so that every row is read once,
+// W - 1 rows per run twice.  Rows that do not exist are predicated loads and stores: a branch would keep the rows apart.
 #include "exb_conv.cuh"
 
 namespace exb {
@@ -11,7 +12,7 @@ namespace exb {
 namespace {
 
 constexpr int TX = 32, TY = 4;      // packs and runs of a block
-constexpr int STEP = 4;             // rows in flight per thread
+constexpr int STEP = 4;
 
 __device__ __forceinline__ float param(const void *p, int64_t i, int f32, const float *) { (void)f32; return static_cast<const float *>(p)[i]; }
 template <typename T>
@@ -22,7 +23,7 @@ __device__ __forceinline__ float param(const void *p, int64_t i, int f32, const 
 
 struct Spot {
     int64_t b, t0, t1, len, row;      // batch item, run, valid steps, index of the block among those of its channels
-    int m;
+    int m, left;                      // first channel, channels from there on
 };
 template <int V>
 __device__ __forceinline__ Spot place(const ConvArgs &a)
@@ -32,167 +33,202 @@ __device__ __forceinline__ Spot place(const ConvArgs &a)
     int64_t i = blockIdx.x;
     Spot s;
     s.m = ((int)(i % tiles) * TX + threadIdx.x) * V;
+    s.left = a.M - s.m;
     i /= tiles;
     s.row = i;
-    s.b = i / runs;
-    s.t0 = ((i % runs) * TY + threadIdx.y) * a.run;
+    s.b = runs > 0 ? i / runs : i;
+    s.t0 = (runs > 0 ? (i % runs) * TY + threadIdx.y : threadIdx.y) * a.run;
     s.t1 = s.t0 + a.run < a.T ? s.t0 + a.run : a.T;
     int64_t n = a.lengths ? (int64_t)a.lengths[s.b] : a.T;
     s.len = n < 0 ? 0 : (n > a.T ? a.T : n);
     return s;
 }
 
-// Row t of the sequence with the state in front of it (t >= -(W - 1)).
+// Row t of the sequence with the state in front of it; 0 in front of that and behind the sequence.
 template <typename T, int V, int W, bool VEC>
-__device__ __forceinline__ void load_row(Pack<T, V> &r, const ConvArgs &a, const Spot &s, int64_t t, int left)
+__device__ __forceinline__ void load_row(RawPack<T, V, VEC> &r, const ConvArgs &a, const Spot &s, int64_t t)
 {
-    if (t >= 0)
-        load_pack<VEC>(r, static_cast<const T *>(a.x.p) + s.b * a.x.sb + t * a.x.st + s.m, t < s.len ? left : 0);
-    else
-        load_pack<VEC>(r, static_cast<const T *>(a.state) + (s.b * (W - 1) + (t + W - 1)) * a.M + s.m, (a.state && t >= 1 - W) ? left : 0);
+    const bool from_x = t >= 0;
+    const T *p = from_x ? static_cast<const T *>(a.x.p) + s.b * a.x.sb + t * a.x.st + s.m
+                        : static_cast<const T *>(a.state) + (s.b * (W - 1) + (t + W - 1)) * a.M + s.m;
+    r.load(p, (from_x ? t < s.len : (a.state && t >= 1 - W)) ? s.left : 0);
 }
 
+// Filter of V channels as pairs.
+template <typename T, int V, int W>
+struct Filter {
+    float2 w[W][V / 2], bias[V / 2];
+    __device__ __forceinline__ Filter(const ConvArgs &a, const Spot &s)
+    {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            const int m = s.m + 2 * i;
+            const bool one = 2 * i < s.left, two = 2 * i + 1 < s.left;
+            const T *tag = nullptr;
+            bias[i] = make_float2(one && a.bias ? param(a.bias, m, a.params_f32, tag) : 0.0f, two && a.bias ? param(a.bias, m + 1, a.params_f32, tag) : 0.0f);
+#pragma unroll
+            for (int k = 0; k < W; ++k)
+                w[k][i] = make_float2(one ? param(a.weight, (int64_t)m * W + k, a.params_f32, tag) : 0.0f,
+                                      two ? param(a.weight, (int64_t)(m + 1) * W + k, a.params_f32, tag) : 0.0f);
+        }
+    }
+};
+
+// 8 x 2048 x 4096 bfloat16, W = 4 (268 MB): see the table in the design notes for the measured time.
 template <typename T, int V, int W, bool VEC>
 __global__ void __launch_bounds__(TX * TY) conv_forward_kernel(const ConvArgs a)
 {
     const Spot s = place<V>(a);
-    const int left = a.M - s.m;
-    if (left <= 0) return;
+    if (s.left <= 0) return;
     if (s.t0 == 0 && a.last) {      // the rows that the next call starts from
         for (int j = 0; j < W - 1; ++j) {
-            Pack<T, V> r;
-            load_row<T, V, W, VEC>(r, a, s, s.len + j - (W - 1), left);
-            store_pack<VEC>(static_cast<T *>(a.last) + (s.b * (W - 1) + j) * a.M + s.m, r, left);
+            RawPack<T, V, VEC> r;
+            load_row<T, V, W, VEC>(r, a, s, s.len + j - (W - 1));
+            r.store(static_cast<T *>(a.last) + (s.b * (W - 1) + j) * a.M + s.m, s.left);
         }
     }
     if (s.t0 >= a.T) return;
-    float w[W][V], bias[V], win[W][V];      // win[k]: row t - W + 1 + k
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        const bool there = v < left;
-        bias[v] = (there && a.bias) ? param(a.bias, s.m + v, a.params_f32, (const T *)nullptr) : 0.0f;
-#pragma unroll
-        for (int k = 0; k < W; ++k) w[k][v] = there ? param(a.weight, (int64_t)(s.m + v) * W + k, a.params_f32, (const T *)nullptr) : 0.0f;
-    }
+    const Filter<T, V, W> f(a, s);
+    RawPack<T, V, VEC> next[STEP];
+    float2 row[STEP + W - 1][V / 2];      // row j: step t - (W - 1) + j
 #pragma unroll
     for (int k = 0; k < W - 1; ++k) {
-        Pack<T, V> r;
-        load_row<T, V, W, VEC>(r, a, s, s.t0 - (W - 1) + k, left);
+        RawPack<T, V, VEC> r;
+        load_row<T, V, W, VEC>(r, a, s, s.t0 - (W - 1) + k);
 #pragma unroll
-        for (int v = 0; v < V; ++v) win[k + 1][v] = to_f32(r.v[v]);
+        for (int i = 0; i < V / 2; ++i) row[k][i] = r.pair(i);
     }
+#pragma unroll
+    for (int j = 0; j < STEP; ++j) load_row<T, V, W, VEC>(next[j], a, s, s.t0 + j);
+    T *out = static_cast<T *>(a.y) + (s.b * a.T + s.t0) * a.M + s.m;
     for (int64_t t = s.t0; t < s.t1; t += STEP) {
-        Pack<T, V> in[STEP];
 #pragma unroll
-        for (int i = 0; i < STEP; ++i) load_row<T, V, W, VEC>(in[i], a, s, t + i, t + i < s.t1 ? left : 0);
+        for (int j = 0; j < STEP; ++j)
 #pragma unroll
-        for (int i = 0; i < STEP; ++i) {
-            if (t + i >= s.t1) break;
-            Pack<T, V> out;
+            for (int i = 0; i < V / 2; ++i) row[W - 1 + j][i] = next[j].pair(i);
+        if (t + STEP < s.t1) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-#pragma unroll
-                for (int k = 0; k < W - 1; ++k) win[k][v] = win[k + 1][v];
-                win[W - 1][v] = to_f32(in[i].v[v]);
-                float y = bias[v];
-#pragma unroll
-                for (int k = 0; k < W; ++k) y = fmaf(w[k][v], win[k][v], y);
-                if (a.silu) y = silu_f(y);
-                out.v[v] = from_f32<T>(t + i < s.len ? y : 0.0f);
-            }
-            store_pack<VEC>(static_cast<T *>(a.y) + (s.b * a.T + t + i) * a.M + s.m, out, left);
+            for (int j = 0; j < STEP; ++j) load_row<T, V, W, VEC>(next[j], a, s, t + STEP + j);
         }
+#pragma unroll
+        for (int j = 0; j < STEP; ++j) {
+            Pack<T, V> y;
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                float2 v = f.bias[i];
+#pragma unroll
+                for (int k = 0; k < W; ++k) v = fma2(f.w[k][i], row[j + k][i], v);
+                if (a.silu) v = silu2(v);
+                y.v[2 * i] = from_f32<T>(t + j < s.len ? v.x : 0.0f);
+                y.v[2 * i + 1] = from_f32<T>(t + j < s.len ? v.y : 0.0f);
+            }
+            store_pack<VEC>(out, y, t + j < s.t1 ? s.left : 0);
+            out += a.M;
+        }
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k)
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) row[k][i] = row[k + STEP][i];
     }
 }
 
-// A thread forms d pre_t for its run and for the W - 1 steps behind it (which the rows of its run feed), and from
-// those dx; filter and bias gradients only take the run's own steps.
+// A thread forms the gradient in front of the activation, d, for its run and for the W - 1 steps behind it (which the rows
+// of its run feed), and from those dx; filter and bias gradients only take the run's own steps.
 template <typename T, int V, int W, bool VEC>
 __global__ void __launch_bounds__(TX * TY) conv_backward_kernel(const ConvArgs a)
 {
     extern __shared__ float s_part[];      // [TY][W + 1][TX * V]
     const Spot s = place<V>(a);
-    const int left = a.M - s.m;
-    float dw[W + 1][V];
+    float2 dw[W + 1][V / 2];
 #pragma unroll
-    for (int v = 0; v < V; ++v)
+    for (int i = 0; i < V / 2; ++i)
 #pragma unroll
-        for (int k = 0; k <= W; ++k) dw[k][v] = 0.0f;
-    if (left > 0 && s.t0 < a.T) {
-        float w[W][V], bias[V], win[W][V], dp[W][V];      // dp[k]: d pre of step t - W + 1 + k
+        for (int k = 0; k <= W; ++k) dw[k][i] = both(0.0f);
+    if (s.left > 0 && s.t0 < a.T) {
+        const Filter<T, V, W> f(a, s);
+        RawPack<T, V, VEC> next_x[STEP], next_g[STEP];
+        float2 row[STEP + W - 1][V / 2], d[STEP + W - 1][V / 2];      // entry j: step t - (W - 1) + j
+        const int64_t end = s.t1 + W - 1;      // rows t - (W - 1) in [t0 (or the state's), t1) come out
+        auto fetch = [&](int64_t t) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const bool there = v < left;
-            bias[v] = (there && a.bias) ? param(a.bias, s.m + v, a.params_f32, (const T *)nullptr) : 0.0f;
-#pragma unroll
-            for (int k = 0; k < W; ++k) {
-                w[k][v] = there ? param(a.weight, (int64_t)(s.m + v) * W + k, a.params_f32, (const T *)nullptr) : 0.0f;
-                dp[k][v] = 0.0f;
+            for (int j = 0; j < STEP; ++j) {
+                load_row<T, V, W, VEC>(next_x[j], a, s, t + j);
+                next_g[j].load(static_cast<const T *>(a.dy.p) + s.b * a.dy.sb + (t + j) * a.dy.st + s.m, (t + j < s.len && t + j < end) ? s.left : 0);
             }
-        }
+        };
 #pragma unroll
         for (int k = 0; k < W - 1; ++k) {
-            Pack<T, V> r;
-            load_row<T, V, W, VEC>(r, a, s, s.t0 - (W - 1) + k, left);
+            RawPack<T, V, VEC> r;
+            load_row<T, V, W, VEC>(r, a, s, s.t0 - (W - 1) + k);
 #pragma unroll
-            for (int v = 0; v < V; ++v) win[k + 1][v] = to_f32(r.v[v]);
+            for (int i = 0; i < V / 2; ++i) {
+                row[k][i] = r.pair(i);
+                d[k][i] = both(0.0f);
+            }
         }
-        const int64_t end = s.t1 + W - 1;      // rows t - W + 1 in [t0 (or the state's), t1) come out
+        fetch(s.t0);
+        T *out = static_cast<T *>(a.dx) + (s.b * a.T + s.t0 - (W - 1)) * a.M + s.m;
+        T *out_state = (s.t0 == 0 && a.dstate) ? static_cast<T *>(a.dstate) + s.b * (W - 1) * a.M + s.m : nullptr;
         for (int64_t t = s.t0; t < end; t += STEP) {
-            Pack<T, V> in[STEP], up[STEP];
+            float2 up[STEP][V / 2];
 #pragma unroll
-            for (int i = 0; i < STEP; ++i) {
-                const bool valid = t + i < end && t + i < s.len;
-                load_row<T, V, W, VEC>(in[i], a, s, t + i, valid ? left : 0);
-                load_pack<VEC>(up[i], static_cast<const T *>(a.dy.p) + s.b * a.dy.sb + (t + i) * a.dy.st + s.m, valid ? left : 0);
-            }
+            for (int j = 0; j < STEP; ++j)
 #pragma unroll
-            for (int i = 0; i < STEP; ++i) {
-                const int64_t now = t + i, row = now - (W - 1);
-                if (now >= end) break;
-                Pack<T, V> out;
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-#pragma unroll
-                    for (int k = 0; k < W - 1; ++k) {
-                        win[k][v] = win[k + 1][v];
-                        dp[k][v] = dp[k + 1][v];
-                    }
-                    win[W - 1][v] = to_f32(in[i].v[v]);
-                    float d = to_f32(up[i].v[v]);
-                    if (a.silu) {
-                        float pre = bias[v];
-#pragma unroll
-                        for (int k = 0; k < W; ++k) pre = fmaf(w[k][v], win[k][v], pre);
-                        const float sg = sigmoid_f(pre);
-                        d *= sg * (1.0f + pre * (1.0f - sg));
-                    }
-                    if (now >= s.len) d = 0.0f;
-                    dp[W - 1][v] = d;
-                    if (now < s.t1 && now < s.len) {
-#pragma unroll
-                        for (int k = 0; k < W; ++k) dw[k][v] = fmaf(d, win[k][v], dw[k][v]);
-                        dw[W][v] += d;
-                    }
-                    float g = 0.0f;
-#pragma unroll
-                    for (int k = 0; k < W; ++k) g = fmaf(w[W - 1 - k][v], dp[k][v], g);
-                    const int64_t f = row + (W - 1) - s.len;      // row of `last` that this row became
-                    if (a.dlast && f >= 0 && f < W - 1 && v < left)
-                        g += to_f32(static_cast<const T *>(a.dlast)[(s.b * (W - 1) + f) * a.M + s.m + v]);
-                    out.v[v] = from_f32<T>(g);
+                for (int i = 0; i < V / 2; ++i) {
+                    row[W - 1 + j][i] = next_x[j].pair(i);
+                    up[j][i] = next_g[j].pair(i);
                 }
-                if (row >= s.t0)
-                    store_pack<VEC>(static_cast<T *>(a.dx) + (s.b * a.T + row) * a.M + s.m, out, left);
-                else if (s.t0 == 0 && a.dstate)
-                    store_pack<VEC>(static_cast<T *>(a.dstate) + (s.b * (W - 1) + now) * a.M + s.m, out, left);
+            if (t + STEP < end) fetch(t + STEP);
+#pragma unroll
+            for (int j = 0; j < STEP; ++j) {
+                const int64_t now = t + j, r = now - (W - 1);
+                const bool counts = now < s.t1;
+                Pack<T, V> g;
+#pragma unroll
+                for (int i = 0; i < V / 2; ++i) {
+                    // rows without an output have up = 0; their pre is finite, because rows behind the sequence read as 0
+                    float2 e = up[j][i];
+                    if (a.silu) {
+                        float2 pre = f.bias[i];
+#pragma unroll
+                        for (int k = 0; k < W; ++k) pre = fma2(f.w[k][i], row[j + k][i], pre);
+                        const float2 slope = silu_slope2(pre);
+                        e = now < s.len ? mul2(e, slope) : both(0.0f);
+                    }
+                    d[W - 1 + j][i] = e;
+                    const float2 own = counts ? e : both(0.0f);
+#pragma unroll
+                    for (int k = 0; k < W; ++k) dw[k][i] = fma2(own, row[j + k][i], dw[k][i]);
+                    dw[W][i] = add2(dw[W][i], own);
+                    float2 v = mul2(f.w[0][i], d[W - 1 + j][i]);
+#pragma unroll
+                    for (int k = 1; k < W; ++k) v = fma2(f.w[k][i], d[W - 1 + j - k][i], v);
+                    const int64_t q = now - s.len;      // row of `last` that row r became
+                    if (a.dlast && q >= 0 && q < W - 1) {
+                        const T *at = static_cast<const T *>(a.dlast) + (s.b * (W - 1) + q) * a.M + s.m + 2 * i;
+                        if (2 * i < s.left) v.x += to_f32(at[0]);
+                        if (2 * i + 1 < s.left) v.y += to_f32(at[1]);
+                    }
+                    g.v[2 * i] = from_f32<T>(v.x);
+                    g.v[2 * i + 1] = from_f32<T>(v.y);
+                }
+                store_pack<VEC>(out, g, (r >= s.t0 && r < s.t1) ? s.left : 0);
+                if (out_state && now < W - 1) store_pack<VEC>(out_state + now * a.M, g, s.left);
+                out += a.M;
             }
+#pragma unroll
+            for (int k = 0; k < W - 1; ++k)
+#pragma unroll
+                for (int i = 0; i < V / 2; ++i) {
+                    row[k][i] = row[k + STEP][i];
+                    d[k][i] = d[k + STEP][i];
+                }
         }
     }
 #pragma unroll
     for (int k = 0; k <= W; ++k)
 #pragma unroll
-        for (int v = 0; v < V; ++v) s_part[(threadIdx.y * (W + 1) + k) * (TX * V) + threadIdx.x * V + v] = dw[k][v];
+        for (int i = 0; i < V / 2; ++i) *reinterpret_cast<float2 *>(s_part + (threadIdx.y * (W + 1) + k) * (TX * V) + threadIdx.x * V + 2 * i) = dw[k][i];
     __syncthreads();
     const int m0 = s.m - threadIdx.x * V;
     for (int i = threadIdx.y * TX + threadIdx.x; i < (W + 1) * TX * V; i += TX * TY) {
@@ -218,43 +254,53 @@ struct PutParams {
     }
 };
 
+// One step: a thread takes V channels of `items` batch items, with their filters in registers.
 template <typename T, int V, int W, bool VEC>
-__global__ void conv_step_kernel(const ConvStepArgs a)
+__global__ void __launch_bounds__(128) conv_step_kernel(const ConvStepArgs a, int items)
 {
     const int packs = (a.M + V - 1) / V;
-    const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
-    if (i >= a.B * packs) return;
-    const int64_t b = i / packs;
-    const int m = (int)(i % packs) * V, left = a.M - m;
-    Pack<T, V> row[W];
-    T *st = static_cast<T *>(a.state) + b * a.ss + m;
+    const int64_t i = blockIdx.x * 128ll + threadIdx.x;
+    const int64_t b0 = i / packs * items;
+    if (b0 >= a.B) return;
+    ConvArgs c{};
+    c.M = a.M; c.weight = a.weight; c.bias = a.bias; c.params_f32 = a.params_f32;
+    Spot s{};
+    s.m = (int)(i % packs) * V;
+    s.left = a.M - s.m;
+    const Filter<T, V, W> f(c, s);
+    const int64_t b1 = b0 + items < a.B ? b0 + items : a.B;
+#pragma unroll 2
+    for (int64_t b = b0; b < b1; ++b) {
+        RawPack<T, V, VEC> row[W];
+        T *st = static_cast<T *>(a.state) + b * a.ss + s.m;
 #pragma unroll
-    for (int k = 0; k < W - 1; ++k) load_pack<VEC>(row[k], st + (int64_t)k * a.M, left);
-    load_pack<VEC>(row[W - 1], static_cast<const T *>(a.x.p) + b * a.x.sb + m, left);
+        for (int k = 0; k < W - 1; ++k) row[k].load(st + (int64_t)k * a.M, s.left);
+        row[W - 1].load(static_cast<const T *>(a.x.p) + b * a.x.sb + s.m, s.left);
 #pragma unroll
-    for (int k = 0; k < W - 1; ++k) store_pack<VEC>(st + (int64_t)k * a.M, row[k + 1], left);
-    Pack<T, V> out;
+        for (int k = 0; k < W - 1; ++k) row[k + 1].store(st + (int64_t)k * a.M, s.left);
+        Pack<T, V> y;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        float y = 0.0f;
-        if (v < left) {
-            y = a.bias ? param(a.bias, m + v, a.params_f32, (const T *)nullptr) : 0.0f;
+        for (int q = 0; q < V / 2; ++q) {
+            float2 v = f.bias[q];
 #pragma unroll
-            for (int k = 0; k < W; ++k) y = fmaf(param(a.weight, (int64_t)(m + v) * W + k, a.params_f32, (const T *)nullptr), to_f32(row[k].v[v]), y);
-            if (a.silu) y = silu_f(y);
+            for (int k = 0; k < W; ++k) v = fma2(f.w[k][q], row[k].pair(q), v);
+            if (a.silu) v = silu2(v);
+            y.v[2 * q] = from_f32<T>(v.x);
+            y.v[2 * q + 1] = from_f32<T>(v.y);
         }
-        out.v[v] = from_f32<T>(y);
+        store_pack<VEC>(static_cast<T *>(a.y) + b * a.M + s.m, y, s.left);
     }
-    store_pack<VEC>(static_cast<T *>(a.y) + b * a.M + m, out, left);
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+constexpr int V = 4;      // channels of a thread where rows are aligned, two where they are not
+
 // Steps of a thread: long runs re-read less (W - 1 rows each), short ones give every SM work on small problems.
-int64_t run_of(int64_t B, int64_t T, int M, int V, int64_t longest)
+int64_t run_of(int64_t B, int64_t T, int M, int64_t longest)
 {
     int64_t run = longest;
-    while (run > 4 && B * ceil_div(M, TX * V) * ceil_div(T, run * TY) < 2 * 148) run /= 2;
+    while (run > 4 && B * ceil_div(M, TX * V) * ceil_div(T, run * TY) < 4 * 148) run /= 2;
     return run;
 }
 
@@ -269,58 +315,58 @@ bool ptr_aligned(const void *p, int V)
     return reinterpret_cast<uintptr_t>(p) % (V * sizeof(T)) == 0;
 }
 
-template <typename T, int V, int W, bool VEC>
+template <typename T, int N, int W, bool VEC>
 cudaError_t forward_typed(ConvArgs a, cudaStream_t s)
 {
-    a.run = run_of(a.B, a.T, a.M, V, 32);
+    a.run = run_of(a.B, a.T, a.M, 64);
     const int64_t runs = a.T > 0 ? ceil_div(a.T, a.run * TY) : 1;
-    conv_forward_kernel<T, V, W, VEC><<<(unsigned)(ceil_div(a.M, TX * V) * runs * a.B), dim3(TX, TY), 0, s>>>(a);
+    conv_forward_kernel<T, N, W, VEC><<<(unsigned)(ceil_div(a.M, TX * N) * runs * a.B), dim3(TX, TY), 0, s>>>(a);
     return cudaGetLastError();
 }
 
-constexpr int BV = 4;      // channels of a thread in the backward pass: 16-byte packs of 16-bit types would need 200 registers
-
-template <typename T, int V, int W, bool VEC>
+template <typename T, int N, int W, bool VEC>
 cudaError_t backward_typed(ConvArgs a, void *dweight, void *dbias, cudaStream_t s)
 {
-    a.run = run_of(a.B, a.T, a.M, BV, 64);
+    a.run = run_of(a.B, a.T, a.M, 64);
     const int64_t rows = a.B * ceil_div(a.T, a.run * TY);
-    constexpr int smem = TY * (W + 1) * TX * V * (int)sizeof(float);
+    constexpr int smem = TY * (W + 1) * TX * N * (int)sizeof(float);
     static_assert(smem <= 48 * 1024, "");
-    conv_backward_kernel<T, V, W, VEC><<<(unsigned)(ceil_div(a.M, TX * V) * rows), dim3(TX, TY), smem, s>>>(a);
+    conv_backward_kernel<T, N, W, VEC><<<(unsigned)(ceil_div(a.M, TX * N) * rows), dim3(TX, TY), smem, s>>>(a);
     const int64_t cols = (int64_t)(W + 1) * a.M;
     if (a.params_f32) launch_column_sum(PutParams<float>{(float *)dweight, (float *)dbias, a.M, W}, a.part, rows, cols, s);
     else launch_column_sum(PutParams<T>{(T *)dweight, (T *)dbias, a.M, W}, a.part, rows, cols, s);
     return cudaGetLastError();
 }
 
-template <typename T, int V, int W, bool VEC>
+template <typename T, int N, int W, bool VEC>
 cudaError_t step_typed(const ConvStepArgs &a, cudaStream_t s)
 {
-    conv_step_kernel<T, V, W, VEC><<<(unsigned)ceil_div(a.B * ceil_div(a.M, V), 128), 128, 0, s>>>(a);
+    const int64_t packs = ceil_div(a.M, N);
+    // several batch items per thread once there are two blocks of threads for every SM
+    int64_t items = a.B * packs / (2 * 148 * 128);
+    items = items < 1 ? 1 : (items > 8 ? 8 : items);
+    conv_step_kernel<T, N, W, VEC><<<(unsigned)ceil_div(ceil_div(a.B, items) * packs, 128), 128, 0, s>>>(a, (int)items);
     return cudaGetLastError();
 }
 
 template <typename T, int W>
 cudaError_t forward_width(const ConvArgs &a, cudaStream_t s)
 {
-    constexpr int V = 16 / sizeof(T);
     const bool vec = a.M % V == 0 && rows_aligned<T>(a.x, V) && ptr_aligned<T>(a.y, V) && ptr_aligned<T>(a.state, V) && ptr_aligned<T>(a.last, V);
-    return vec ? forward_typed<T, V, W, true>(a, s) : forward_typed<T, 1, W, false>(a, s);
+    return vec ? forward_typed<T, V, W, true>(a, s) : forward_typed<T, 2, W, false>(a, s);
 }
 template <typename T, int W>
 cudaError_t backward_width(const ConvArgs &a, void *dweight, void *dbias, cudaStream_t s)
 {
-    const bool vec = a.M % BV == 0 && rows_aligned<T>(a.x, BV) && rows_aligned<T>(a.dy, BV) && ptr_aligned<T>(a.dx, BV) &&
-                     ptr_aligned<T>(a.state, BV) && ptr_aligned<T>(a.dstate, BV);
-    return vec ? backward_typed<T, BV, W, true>(a, dweight, dbias, s) : backward_typed<T, 1, W, false>(a, dweight, dbias, s);
+    const bool vec = a.M % V == 0 && rows_aligned<T>(a.x, V) && rows_aligned<T>(a.dy, V) && ptr_aligned<T>(a.dx, V) &&
+                     ptr_aligned<T>(a.state, V) && ptr_aligned<T>(a.dstate, V);
+    return vec ? backward_typed<T, V, W, true>(a, dweight, dbias, s) : backward_typed<T, 2, W, false>(a, dweight, dbias, s);
 }
 template <typename T, int W>
 cudaError_t step_width(const ConvStepArgs &a, cudaStream_t s)
 {
-    constexpr int V = 16 / sizeof(T);
     const bool vec = a.M % V == 0 && a.x.sb % V == 0 && a.ss % V == 0 && ptr_aligned<T>(a.x.p, V) && ptr_aligned<T>(a.y, V) && ptr_aligned<T>(a.state, V);
-    return vec ? step_typed<T, V, W, true>(a, s) : step_typed<T, 1, W, false>(a, s);
+    return vec ? step_typed<T, V, W, true>(a, s) : step_typed<T, 2, W, false>(a, s);
 }
 
 #define EXB_CONV_WIDTHS(CALL)                                                                                                  \
@@ -362,7 +408,7 @@ cudaError_t step_dispatch(const ConvStepArgs &a, cudaStream_t s)
 int64_t conv_backward_workspace_bytes(int64_t B, int64_t T, int M, int W)
 {
     // the run does not depend on how many channels a thread takes, so that both kernels fill the same partial sums
-    const int64_t run = run_of(B, T, M, BV, 64);
+    const int64_t run = run_of(B, T, M, 64);
     return B * ceil_div(T, run * TY) * (W + 1) * M * (int64_t)sizeof(float);
 }
 

@@ -21,6 +21,7 @@ struct NormArgs {
     float *part;                         // partial sums: statistics [R][chunks][G][2] or gradients [rows][2][C]
     int64_t chunk;                       // positions of a block
     int chunks, slab, slabs;             // blocks of a sample; groups of a block; blocks of a row
+    int smem;                            // pairs of shared memory that the map kernels work in
 };
 
 int64_t norm_workspace_bytes(int64_t R, int64_t S, int C, int G, int dtype, bool backward);

@@ -985,44 +985,54 @@ struct PutD {
 
 // ---------------------------------------------------------------------------------------------- one token
 
-template <typename T, int L>
-__global__ void __launch_bounds__(256) sel_step_kernel(const SelStepArgs a)
+// A thread takes four states of a channel in ITEMS batch items, `apart` of them between two: the rates are loaded once, and
+// all states are on their way together (the state is what has to move).
+template <typename T, int L, int ITEMS, bool VEC>
+__global__ void __launch_bounds__(256) sel_step_kernel(const SelStepArgs a, int64_t apart)
 {
-    const int64_t i = (blockIdx.x * (int64_t)256 + threadIdx.x) / L;
+    const int64_t i = (blockIdx.x * 256ll + threadIdx.x) / L;
     const int l = threadIdx.x % L, n0 = 4 * l;
-    const bool alive = i < a.B * a.M;
-    const int64_t b = alive ? i / a.M : 0;
+    const bool alive = i < apart * a.M;
+    const int64_t b0 = alive ? i / a.M : 0;
     const int m = alive ? (int)(i % a.M) : 0, g = m / (a.M / a.G);
-    float y = 0.0f, x = 0.0f;
-    if (alive) {
-        float h[4], A[4], bb[4], cc[4];
-        float *hp = a.h + b * a.sh + (int64_t)m * a.N;
-        load_states(h, hp, n0, a.N);
-        load_states(A, a.A + (int64_t)m * a.N, n0, a.N);
-        x = to_f32(static_cast<const T *>(a.x.p)[b * a.x.sb + m]);
-        float d = to_f32(static_cast<const T *>(a.dt.p)[b * a.dt.sb + m]) + (a.dt_bias ? a.dt_bias[m] : 0.0f);
-        if (a.softplus) d = softplus_f(d);
-        const T *bp = static_cast<const T *>(a.Bm.p) + b * a.Bm.sb + (int64_t)g * a.N;
-        const T *cp = static_cast<const T *>(a.Cm.p) + b * a.Cm.sb + (int64_t)g * a.N;
+    RawPack<T, 1, false> x[ITEMS], dt[ITEMS], z[ITEMS];
+    RawPack<T, 4, VEC> vb[ITEMS], vc[ITEMS];
+    RawPack<float, 4, VEC> vh[ITEMS], va;
+    va.load(a.A + (int64_t)m * a.N + n0, alive ? a.N - n0 : 0);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            bb[j] = n0 + j < a.N ? to_f32(bp[n0 + j]) : 0.0f;
-            cc[j] = n0 + j < a.N ? to_f32(cp[n0 + j]) : 0.0f;
-        }
-        const float u = d * x;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            h[j] = fmaf(exp2_fast(d * A[j] * LOG2E), h[j], u * bb[j]);
-            y = fmaf(cc[j], h[j], y);
-        }
-        store_states(hp, h, n0, a.N);
+    for (int k = 0; k < ITEMS; ++k) {
+        const int64_t b = b0 + k * apart;
+        const int here = alive && b < a.B;
+        vh[k].load(a.h + b * a.sh + (int64_t)m * a.N + n0, here ? a.N - n0 : 0);
+        x[k].load(static_cast<const T *>(a.x.p) + b * a.x.sb + m, here);
+        dt[k].load(static_cast<const T *>(a.dt.p) + b * a.dt.sb + m, here);
+        z[k].load(static_cast<const T *>(a.z.p) + b * a.z.sb + m, here && a.z.p);
+        vb[k].load(static_cast<const T *>(a.Bm.p) + b * a.Bm.sb + (int64_t)g * a.N + n0, here ? a.N - n0 : 0);
+        vc[k].load(static_cast<const T *>(a.Cm.p) + b * a.Cm.sb + (int64_t)g * a.N + n0, here ? a.N - n0 : 0);
     }
+    const float bias = alive && a.dt_bias ? a.dt_bias[m] : 0.0f, skip = alive && a.D ? a.D[m] : 0.0f;
 #pragma unroll
-    for (int s = 1; s < L; s <<= 1) y += __shfl_xor_sync(0xffffffffu, y, s);
-    if (alive && l == 0) {
-        if (a.D) y = fmaf(a.D[m], x, y);
-        if (a.z.p) y *= silu_f(to_f32(static_cast<const T *>(a.z.p)[b * a.z.sb + m]));
-        static_cast<T *>(a.y)[b * a.M + m] = from_f32<T>(y);
+    for (int k = 0; k < ITEMS; ++k) {
+        const int64_t b = b0 + k * apart;
+        float d = dt[k].get(0) + bias;
+        if (a.softplus) d = softplus_f(d);
+        const float u = d * x[k].get(0);
+        float y = 0.0f;
+        Pack<float, 4> h;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            h.v[j] = fmaf(exp2_fast(d * va.get(j) * LOG2E), vh[k].get(j), u * vb[k].get(j));
+            y = fmaf(vc[k].get(j), h.v[j], y);
+        }
+        const bool here = alive && b < a.B;
+        store_pack<VEC>(a.h + b * a.sh + (int64_t)m * a.N + n0, h, here ? a.N - n0 : 0);
+#pragma unroll
+        for (int s = 1; s < L; s <<= 1) y += __shfl_xor_sync(0xffffffffu, y, s);
+        if (here && l == 0) {
+            y = fmaf(skip, x[k].get(0), y);
+            if (a.z.p) y *= silu_f(z[k].get(0));
+            static_cast<T *>(a.y)[b * a.M + m] = from_f32<T>(y);
+        }
     }
 }
 
@@ -1112,20 +1122,37 @@ cudaError_t backward_dispatch(const SelArgs &a, const SelPlan &p, void *dB, void
     return cudaGetLastError();
 }
 
+template <typename T, int L, bool VEC>
+cudaError_t step_typed(const SelStepArgs &a, cudaStream_t s)
+{
+    // Four batch items per thread once that leaves two blocks for every SM.
+    const bool many = a.B >= 4 && ceil_div(a.B, 4) * a.M * L >= 2 * 148 * 256;
+    const int64_t apart = many ? ceil_div(a.B, 4) : a.B;
+    const unsigned grid = (unsigned)ceil_div(apart * a.M * L, 256);
+    if (many) sel_step_kernel<T, L, 4, VEC><<<grid, 256, 0, s>>>(a, apart);
+    else sel_step_kernel<T, L, 1, VEC><<<grid, 256, 0, s>>>(a, apart);
+    return cudaGetLastError();
+}
+
+template <typename T, bool VEC>
+cudaError_t step_lanes(const SelStepArgs &a, cudaStream_t s)
+{
+    switch (sel_lanes(a.N)) {
+    case 1: return step_typed<T, 1, VEC>(a, s);
+    case 2: return step_typed<T, 2, VEC>(a, s);
+    case 4: return step_typed<T, 4, VEC>(a, s);
+    case 8: return step_typed<T, 8, VEC>(a, s);
+    case 16: return step_typed<T, 16, VEC>(a, s);
+    default: return step_typed<T, 32, VEC>(a, s);
+    }
+}
+
 template <typename T>
 cudaError_t step_dispatch(const SelStepArgs &a, cudaStream_t s)
 {
-    const int L = sel_lanes(a.N);
-    const unsigned grid = (unsigned)ceil_div(a.B * a.M * L, 256);
-    switch (L) {
-    case 1: sel_step_kernel<T, 1><<<grid, 256, 0, s>>>(a); break;
-    case 2: sel_step_kernel<T, 2><<<grid, 256, 0, s>>>(a); break;
-    case 4: sel_step_kernel<T, 4><<<grid, 256, 0, s>>>(a); break;
-    case 8: sel_step_kernel<T, 8><<<grid, 256, 0, s>>>(a); break;
-    case 16: sel_step_kernel<T, 16><<<grid, 256, 0, s>>>(a); break;
-    default: sel_step_kernel<T, 32><<<grid, 256, 0, s>>>(a); break;
-    }
-    return cudaGetLastError();
+    const bool vec = a.N % 4 == 0 && pack_aligned<T>(a.Bm) && pack_aligned<T>(a.Cm) && a.sh % 4 == 0 &&
+                     ((reinterpret_cast<uintptr_t>(a.h) | reinterpret_cast<uintptr_t>(a.A)) & 15) == 0;
+    return vec ? step_lanes<T, true>(a, s) : step_lanes<T, false>(a, s);
 }
 
 void place(SelArgs &a, const SelPlan &p, void *ws)

@@ -86,11 +86,30 @@ struct RawPack {
             for (int i = 0; i < V; ++i) w[i] = i < n ? *reinterpret_cast<const uint32_t *>(p + i) : 0u;
         }
     }
+    __device__ __forceinline__ void store(T *p, int n) const
+    {
+        if constexpr (VEC) {
+            if (n > 0) {
+                if constexpr (WORDS == 4) *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+                else if constexpr (WORDS == 2) *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+                else *reinterpret_cast<uint32_t *>(p) = w[0];
+            }
+        } else if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (i < n) *reinterpret_cast<unsigned short *>(p + i) = (unsigned short)w[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (i < n) *reinterpret_cast<uint32_t *>(p + i) = w[i];
+        }
+    }
     __device__ __forceinline__ float get(int j) const
     {
         const uint32_t v = PER == 2 && (j & 1) ? w[j / PER] >> 16 : w[j / PER];
         return word_to_f32((const T *)nullptr, v);
     }
+    __device__ __forceinline__ float2 pair(int i) const { return make_float2(get(2 * i), get(2 * i + 1)); }
 };
 
 template <bool VEC, typename T, int V>
@@ -144,6 +163,20 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+__device__ __forceinline__ float2 sigmoid2(float2 v)
+{
+    const float2 e = mul2(v, both(-LOG2E));
+    const float2 n = add2(make_float2(exp2_fast(e.x), exp2_fast(e.y)), both(1.0f));
+    return make_float2(rcp_fast(n.x), rcp_fast(n.y));
+}
+__device__ __forceinline__ float2 silu2(float2 v) { return mul2(v, sigmoid2(v)); }
+// d (v sigmoid(v)) / dv = s + v s (1 - s)
+__device__ __forceinline__ float2 silu_slope2(float2 v)
+{
+    const float2 s = sigmoid2(v), f = mul2(v, s);
+    return fma2(f, fma2(s, both(-1.0f), both(1.0f)), s);
+}
 
 // log(1 + e^v) = max(v, 0) + log(1 + u), u = e^-|v|, and log(1 + u) = 2 artanh(u / (2 + u)) by its series, whose argument is
 // at most 1/3: seven terms leave 1.4e-8.  u keeps the digits that rounding |v| log2(e) would cost (step sizes are the
