@@ -189,7 +189,8 @@ int exb_selective_step(void *y, float *h, int64_t h_stride, const exb_rows *x, c
     EXB_TRY(check_ptr(who, "D", D, 4, false));
     EXB_TRY(check_rows(who, "z", z, es, false));
     EXB_TRY(check_ptr(who, "dt_bias", dt_bias, 4, false));
-    if ((double)B * M * exb::sel_lanes((int)N) / 256 > GRID_MAX) return fail(EXB_ERR_ARG, "%s: sizes too large for one launch", who);
+    if ((double)B * M * exb::sel_lanes((int)N) > 4.0e9)      // threads are counted in 32 bits
+        return fail(EXB_ERR_ARG, "%s: sizes too large for one launch", who);
     DeviceGuard guard(device);
     if (!guard.ok) return fail(EXB_ERR_DEVICE, "%s: cannot select device %d", who, device);
     exb::SelStepArgs a{};
@@ -308,7 +309,8 @@ int check_norm_sizes(const char *who, int64_t R, int64_t S, int64_t C, int64_t G
     if (G < 1 || C % G) return fail(EXB_ERR_ARG, "%s: the %lld groups must divide the %lld channels", who, (long long)G, (long long)C);
     if (C / G > exb::NORM_MAX_GROUP) return fail(EXB_ERR_ARG, "%s: at most %d channels in a group, got %lld", who, exb::NORM_MAX_GROUP, (long long)(C / G));
     if (!dtype_ok(dtype)) return fail(EXB_ERR_ARG, "%s: unknown element type %d", who, dtype);
-    if (C > 0x7fffffffll / 4 || (double)R * (double)G > GRID_MAX) return fail(EXB_ERR_ARG, "%s: sizes too large for one launch", who);
+    // 32 lanes per sample and group at most, blocks of 256; a sample's positions are counted in int
+    if (C > 0x7fffffffll / 4 || S > 0x7fffffffll - 1024 || (double)R * (double)G > GRID_MAX) return fail(EXB_ERR_ARG, "%s: sizes too large for one launch", who);
     return EXB_OK;
 }
 

@@ -22,46 +22,91 @@ __device__ __forceinline__ float param(const void *p, int64_t i, int f32)
     return f32 ? static_cast<const float *>(p)[i] : to_f32(static_cast<const T *>(p)[i]);
 }
 
-__device__ __forceinline__ float2 activate2(float2 v, int act)
+// The activation of all pairs, and d times its slope; one branch for all of them.
+template <int P>
+__device__ __forceinline__ void activate(float2 (&v)[P], int act)
 {
-    if (act == EXB_ACT_SILU) return silu2(v);
-    if (act == EXB_ACT_RELU) return make_float2(max_nan(v.x, 0.0f), max_nan(v.y, 0.0f));
-    return v;
+    if (act == EXB_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) v[i] = silu2(v[i]);
+    } else if (act == EXB_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) v[i] = make_float2(max_nan(v[i].x, 0.0f), max_nan(v[i].y, 0.0f));
+    }
 }
-__device__ __forceinline__ float2 activate_slope2(float2 v, int act)
+template <int P>
+__device__ __forceinline__ void activate_backward(float2 (&d)[P], const float2 (&pre)[P], int act)
 {
-    if (act == EXB_ACT_SILU) return silu_slope2(v);
-    if (act == EXB_ACT_RELU) return make_float2(v.x > 0.0f ? 1.0f : 0.0f, v.y > 0.0f ? 1.0f : 0.0f);
-    return both(1.0f);
+    if (act == EXB_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) d[i] = mul2(d[i], silu_slope2(pre[i]));
+    } else if (act == EXB_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) d[i] = make_float2(pre[i].x > 0.0f ? d[i].x : 0.0f, pre[i].y > 0.0f ? d[i].y : 0.0f);
+    }
+}
+
+// Weight or bias of V channels from c on (the first `left` of them exist), `absent` where there is none.
+template <typename T, int V, bool VEC>
+__device__ __forceinline__ void load_params(float (&v)[V], const void *p, int64_t c, int left, int f32, float absent)
+{
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = absent;
+    if (!p) return;
+    if (VEC && f32 && V % 4 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+#pragma unroll
+        for (int i = 0; i + 3 < V; i += 4) {
+            const float4 q = left > 0 ? *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + c + i) : make_float4(absent, absent, absent, absent);
+            v[i] = q.x; v[i + 1] = q.y; v[i + 2] = q.z; v[i + 3] = q.w;
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (i < left) v[i] = param<T>(p, c + i, f32);
+}
+
+// 1 / sqrt(v), the approximation refined once.
+__device__ __forceinline__ float inverse_sqrt(float v)
+{
+    const float r = rsqrtf(v);
+    return v > 0.0f && r < 1e18f ? r * fmaf(-0.5f * v * r, r, 1.5f) : r;
+}
+
+__device__ __forceinline__ float warp_sum(float v)
+{
+#pragma unroll
+    for (int m = 16; m >= 1; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+    return v;
 }
 
 // Number of values, their mean and the sum of their squared distances from it.
 struct Moments {
     float n, mean, m2;
 };
-__device__ __forceinline__ Moments merge(const Moments &a, const Moments &b)
+
+// Moments of `count` sets of values together, by one warp: the mean about the first set's, then every set's distances with
+// n (mean - total mean)^2, so that a large common offset costs no digits.  get(i): the i-th set; the same in all lanes.
+template <typename Get>
+__device__ __forceinline__ Moments join(int count, const Get &get)
 {
-    Moments r;
-    r.n = a.n + b.n;
-    if (b.n == 0.0f) return a;
-    if (a.n == 0.0f) return b;
-    const float d = b.mean - a.mean, f = b.n / r.n;
-    r.mean = fmaf(d, f, a.mean);
-    r.m2 = a.m2 + b.m2 + d * d * (a.n * f);
-    return r;
-}
-__device__ __forceinline__ Moments merge_lanes(Moments v)
-{
-#pragma unroll
-    for (int m = 16; m >= 1; m >>= 1) {
-        Moments o;
-        o.n = __shfl_xor_sync(0xffffffffu, v.n, m);
-        o.mean = __shfl_xor_sync(0xffffffffu, v.mean, m);
-        o.m2 = __shfl_xor_sync(0xffffffffu, v.m2, m);
-        // the same order in both lanes, so that they agree to the last bit
-        v = (threadIdx.x & m) ? merge(o, v) : merge(v, o);
+    const int lane = threadIdx.x % 32;
+    const float base = get(0).mean;
+    float n = 0.0f, sum = 0.0f;
+    for (int i = lane; i < count; i += 32) {
+        const Moments m = get(i);
+        n += m.n;
+        sum = fmaf(m.n, m.mean - base, sum);
     }
-    return v;
+    n = warp_sum(n);
+    const float off = warp_sum(sum) / n, mean = base + off;
+    float m2 = 0.0f;
+    for (int i = lane; i < count; i += 32) {
+        const Moments m = get(i);
+        const float d = (m.mean - base) - off;
+        m2 += fmaf(m.n * d, d, m.m2);
+    }
+    return Moments{n, mean, warp_sum(m2)};
 }
 
 // ---------------------------------------------------------------------------------------------- tokens
@@ -72,6 +117,7 @@ __device__ __forceinline__ Moments merge_lanes(Moments v)
 template <typename T, int V, int L, int K, bool VEC>
 struct Token {
     static constexpr int P = V > 1 ? V / 2 : 1;      // pairs of a pack
+    static constexpr int ROWS = K * V <= 8 ? 4 : (K * V <= 16 ? 2 : 1);      // samples at a time
     int64_t first;
     int l, per, g;
     bool alive;
@@ -86,10 +132,11 @@ struct Token {
         alive = first < strides;
     }
     __device__ __forceinline__ int channel(int k) const { return (k * L + l) * V; }
-    __device__ __forceinline__ void fetch(RawPack<T, V, VEC> (&r)[K], const View &v, int64_t row, bool here) const
+    // x points to the group's first channel of a sample
+    __device__ __forceinline__ void fetch(RawPack<T, V, VEC> (&r)[K], const T *x, bool here) const
     {
 #pragma unroll
-        for (int k = 0; k < K; ++k) r[k].load(static_cast<const T *>(v.p) + row * v.sb + g * per + channel(k), here ? per - channel(k) : 0);
+        for (int k = 0; k < K; ++k) r[k].load(x + channel(k), here ? per - channel(k) : 0);
     }
     __device__ __forceinline__ static float2 pair(const RawPack<T, V, VEC> &r, int i)
     {
@@ -107,13 +154,20 @@ struct Token {
                 v[k][i].y = (p && V > 1 && c + 1 < per) ? param<T>(p, g * per + c + 1, f32) : absent;
             }
     }
-    // 1 where the pair's channels exist
-    __device__ __forceinline__ float2 there(int k, int i) const
+    // 0 for channels that do not exist
+    __device__ __forceinline__ void mask(float2 (&v)[K][P]) const
     {
-        const int c = channel(k) + 2 * i;
-        return make_float2(c < per ? 1.0f : 0.0f, V > 1 && c + 1 < per ? 1.0f : 0.0f);
+        if (per == L * K * V && V > 1) return;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                const int c = channel(k) + 2 * i;
+                if (c >= per) v[k][i].x = 0.0f;
+                if (V == 1 || c + 1 >= per) v[k][i].y = 0.0f;
+            }
     }
-    __device__ __forceinline__ void store(T *p, int64_t row, int C, const float2 (&v)[K][P]) const
+    __device__ __forceinline__ void store(T *y, const float2 (&v)[K][P]) const
     {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -123,7 +177,7 @@ struct Token {
                 out.v[2 * i] = from_f32<T>(v[k][i].x);
                 if constexpr (V > 1) out.v[2 * i + 1] = from_f32<T>(v[k][i].y);
             }
-            store_pack<VEC>(p + row * C + g * per + channel(k), out, per - channel(k));
+            store_pack<VEC>(y + channel(k), out, per - channel(k));
         }
     }
 };
@@ -136,55 +190,81 @@ __device__ __forceinline__ float lane_sum(float v)
 }
 
 template <typename T, int V, int L, int K, bool VEC>
-__global__ void __launch_bounds__(NT) norm_token_forward_kernel(const NormArgs a, int64_t strides)
+__global__ void __launch_bounds__(NT, K * V <= 8 ? 4 : 1) norm_token_forward_kernel(const NormArgs a, int64_t strides)
 {
     using U = Token<T, V, L, K, VEC>;
-    constexpr int P = U::P;
+    constexpr int P = U::P, ROWS = U::ROWS;
     const U u(a, strides);
     float2 w[K][P], b[K][P];
     u.values(w, a.weight, a.params_f32, 1.0f);
     u.values(b, a.bias, a.params_f32, 0.0f);
-    RawPack<T, V, VEC> next[K];
-    u.fetch(next, a.x, u.first, u.alive && u.first < a.R);
-    const int64_t rounds = (a.R + strides - 1) / strides;      // the same for every lane of the warp
+    RawPack<T, V, VEC> next[ROWS][K];
+    // samples of this lane group; rounds of ROWS samples, as many for every lane of the warp
+    const int mine = u.alive && u.first < a.R ? (int)((a.R - u.first + strides - 1) / strides) : 0;
+    const int rounds = (int)((a.R + ROWS * strides - 1) / (ROWS * strides));
+    const int64_t first = u.alive ? u.first : 0;
+    const T *x = static_cast<const T *>(a.x.p) + first * a.x.sb + u.g * u.per;
+    T *y = static_cast<T *>(a.y) + first * a.C + u.g * u.per;
+    float *stat = (u.l == 0 ? a.mean : a.rstd) + first * a.G + u.g;      // lane 0 keeps the mean, lane 1 (or 0 too) the rest
+    const int64_t dx = strides * a.x.sb, dy = strides * a.C, ds = strides * a.G;
+#pragma unroll
+    for (int q = 0; q < ROWS; ++q, x += dx) u.fetch(next[q], x, q < mine);
     const float inv = 1.0f / u.per;
-    for (int64_t j = 0; j < rounds; ++j) {
-        const int64_t r = u.first + j * strides;
-        const bool here = u.alive && r < a.R;
-        float2 v[K][P], sum = both(0.0f), sq = both(0.0f);
+    for (int j = 0; j < rounds; ++j) {
+        float2 v[ROWS][K][P];
+        float mean[ROWS], rstd[ROWS];
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+        for (int q = 0; q < ROWS; ++q) {
+            float2 sum = both(0.0f);
 #pragma unroll
-            for (int i = 0; i < P; ++i) {
-                v[k][i] = U::pair(next[k], i);
-                sum = add2(sum, v[k][i]);
-            }
-        u.fetch(next, a.x, r + strides, u.alive && r + strides < a.R);
-        const float mean = lane_sum<L>(sum.x + sum.y) * inv;
+            for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-            for (int i = 0; i < P; ++i) {
-                v[k][i] = add2(v[k][i], both(-mean));
-                const float2 d = mul2(v[k][i], u.there(k, i));
-                sq = fma2(d, d, sq);
-            }
-        const float rstd = 1.0f / sqrtf(lane_sum<L>(sq.x + sq.y) * inv + a.eps);
-        if (!here) continue;
-        if (u.l == 0) {
-            a.mean[r * a.G + u.g] = mean;
-            a.rstd[r * a.G + u.g] = rstd;
+                for (int i = 0; i < P; ++i) {
+                    v[q][k][i] = U::pair(next[q][k], i);
+                    sum = add2(sum, v[q][k][i]);
+                }
+            mean[q] = sum.x + sum.y;
         }
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+        for (int q = 0; q < ROWS; ++q, x += dx) u.fetch(next[q], x, (j + 1) * ROWS + q < mine);
 #pragma unroll
-            for (int i = 0; i < P; ++i) v[k][i] = activate2(fma2(mul2(v[k][i], both(rstd)), w[k][i], b[k][i]), a.act);
-        u.store(static_cast<T *>(a.y), r, a.C, v);
+        for (int q = 0; q < ROWS; ++q) {
+            mean[q] = lane_sum<L>(mean[q]) * inv;
+            float2 sq = both(0.0f);
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int i = 0; i < P; ++i) v[q][k][i] = add2(v[q][k][i], both(-mean[q]));
+            u.mask(v[q]);
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int i = 0; i < P; ++i) sq = fma2(v[q][k][i], v[q][k][i], sq);
+            rstd[q] = sq.x + sq.y;
+        }
+#pragma unroll
+        for (int q = 0; q < ROWS; ++q) rstd[q] = inverse_sqrt(lane_sum<L>(rstd[q]) * inv + a.eps);
+#pragma unroll
+        for (int q = 0; q < ROWS; ++q) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+#pragma unroll
+                for (int i = 0; i < P; ++i) v[q][k][i] = fma2(mul2(v[q][k][i], both(rstd[q])), w[k][i], b[k][i]);
+                activate(v[q][k], a.act);
+            }
+            if (j * ROWS + q < mine) {
+                u.store(y, v[q]);
+                if (u.l < 2) *stat = u.l == 0 ? mean[q] : rstd[q];
+                if (L == 1) a.rstd[stat - a.mean] = rstd[q];
+            }
+            y += dy;
+            stat += ds;
+        }
     }
 }
 
 template <typename T, int V, int L, int K, bool VEC>
-__global__ void __launch_bounds__(NT) norm_token_backward_kernel(const NormArgs a, int64_t strides)
+__global__ void __launch_bounds__(NT, K * V <= 8 ? 2 : 1) norm_token_backward_kernel(const NormArgs a, int64_t strides)
 {
     using U = Token<T, V, L, K, VEC>;
     constexpr int P = U::P;
@@ -196,36 +276,75 @@ __global__ void __launch_bounds__(NT) norm_token_backward_kernel(const NormArgs 
     for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int i = 0; i < P; ++i) dw[k][i] = db[k][i] = both(0.0f);
-    const int64_t rounds = (a.R + strides - 1) / strides;      // the same for every lane of the warp
+    constexpr int ROWS = U::ROWS > 2 ? 2 : U::ROWS;
+    const int mine = u.alive && u.first < a.R ? (int)((a.R - u.first + strides - 1) / strides) : 0;
+    const int rounds = (int)((a.R + ROWS * strides - 1) / (ROWS * strides));      // the same for every lane of the warp
+    const int64_t first = u.alive ? u.first : 0;
+    const T *x = static_cast<const T *>(a.x.p) + first * a.x.sb + u.g * u.per, *dy = static_cast<const T *>(a.dy.p) + first * a.dy.sb + u.g * u.per;
+    T *out = static_cast<T *>(a.dx) + first * a.C + u.g * u.per;
+    int64_t stat = first * a.G + u.g;
+    const int64_t step_x = strides * a.x.sb, step_dy = strides * a.dy.sb, step_out = strides * a.C, step_stat = strides * a.G;
     const float inv = 1.0f / u.per;
-    for (int64_t j = 0; j < rounds; ++j) {
-        const int64_t r = u.first + j * strides;
-        const bool here = u.alive && r < a.R;
-        RawPack<T, V, VEC> px[K], pg[K];
-        u.fetch(px, a.x, r, here);
-        u.fetch(pg, a.dy, r, here);
-        const float mean = here ? a.mean[r * a.G + u.g] : 0.0f, rstd = here ? a.rstd[r * a.G + u.g] : 0.0f;
-        float2 n[K][P], e[K][P], s1 = both(0.0f), s2 = both(0.0f);
+    RawPack<T, V, VEC> px[ROWS][K], pg[ROWS][K];
+    float next_mean[ROWS], next_rstd[ROWS];
+    auto fetch = [&](int q, bool here) {
+        u.fetch(px[q], x, here);
+        u.fetch(pg[q], dy, here);
+        next_mean[q] = here ? a.mean[stat] : 0.0f;
+        next_rstd[q] = here ? a.rstd[stat] : 0.0f;
+        x += step_x;
+        dy += step_dy;
+        stat += step_stat;
+    };
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+    for (int q = 0; q < ROWS; ++q) fetch(q, q < mine);
+    for (int j = 0; j < rounds; ++j) {
+        float2 n[ROWS][K][P], e[ROWS][K][P];
+        float u1[ROWS], u2[ROWS], rstd[ROWS];
 #pragma unroll
-            for (int i = 0; i < P; ++i) {
-                n[k][i] = mul2(mul2(add2(U::pair(px[k], i), both(-mean)), both(rstd)), u.there(k, i));
-                float2 d = U::pair(pg[k], i);      // 0 where there is no channel
-                if (a.act) d = mul2(d, activate_slope2(fma2(n[k][i], w[k][i], b[k][i]), a.act));
-                dw[k][i] = fma2(d, n[k][i], dw[k][i]);
-                db[k][i] = add2(db[k][i], d);
-                e[k][i] = mul2(d, w[k][i]);
-                s1 = add2(s1, e[k][i]);
-                s2 = fma2(e[k][i], n[k][i], s2);
+        for (int q = 0; q < ROWS; ++q) {
+            const float mean = next_mean[q];
+            rstd[q] = next_rstd[q];
+            float2 s1 = both(0.0f), s2 = both(0.0f);
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    n[q][k][i] = mul2(add2(U::pair(px[q][k], i), both(-mean)), both(rstd[q]));
+                    e[q][k][i] = U::pair(pg[q][k], i);      // 0 where there is no channel
+                }
+            fetch(q, (j + 1) * ROWS + q < mine);
+            u.mask(n[q]);
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                float2 pre[P];
+#pragma unroll
+                for (int i = 0; i < P; ++i) pre[i] = fma2(n[q][k][i], w[k][i], b[k][i]);
+                activate_backward(e[q][k], pre, a.act);
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    const float2 d = e[q][k][i];
+                    dw[k][i] = fma2(d, n[q][k][i], dw[k][i]);
+                    db[k][i] = add2(db[k][i], d);
+                    e[q][k][i] = mul2(d, w[k][i]);
+                    s1 = add2(s1, e[q][k][i]);
+                    s2 = fma2(e[q][k][i], n[q][k][i], s2);
+                }
             }
-        const float u1 = lane_sum<L>(s1.x + s1.y) * inv, u2 = lane_sum<L>(s2.x + s2.y) * inv;
-        if (!here) continue;
+            u1[q] = s1.x + s1.y;
+            u2[q] = s2.x + s2.y;
+        }
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+        for (int q = 0; q < ROWS; ++q) {
+            u1[q] = lane_sum<L>(u1[q]) * inv;
+            u2[q] = lane_sum<L>(u2[q]) * inv;
 #pragma unroll
-            for (int i = 0; i < P; ++i) e[k][i] = mul2(both(rstd), fma2(n[k][i], both(-u2), add2(e[k][i], both(-u1))));
-        u.store(static_cast<T *>(a.dx), r, a.C, e);
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int i = 0; i < P; ++i) e[q][k][i] = mul2(both(rstd[q]), fma2(n[q][k][i], both(-u2[q]), add2(e[q][k][i], both(-u1[q]))));
+            if (j * ROWS + q < mine) u.store(out, e[q]);
+            out += step_out;
+        }
     }
     if (!u.alive) return;
 #pragma unroll
@@ -246,66 +365,77 @@ __global__ void __launch_bounds__(NT) norm_token_backward_kernel(const NormArgs 
 // A block's sample, positions and channels; its threads as columns of packs times rows of positions.
 struct Spot {
     int64_t r, p0, p1;
-    int g0, groups, c0, chans, chunk, packs, px, ty, rows;
+    int g0, groups, c0, chans, chunk, packs, wide, px, ty, rows, count;
 };
 template <int V>
 __device__ __forceinline__ Spot place(const NormArgs &a)
 {
     Spot s;
-    int64_t i = blockIdx.x;
-    s.chunk = (int)(i % a.chunks);      // neighbours: the blocks of a cluster
-    i /= a.chunks;
-    const int sl = (int)(i % a.slabs);
-    s.r = i / a.slabs;
+    unsigned i = blockIdx.x;
+    s.chunk = (int)(i % (unsigned)a.chunks);      // neighbours: the blocks of a cluster
+    i /= (unsigned)a.chunks;
+    const int sl = (int)(i % (unsigned)a.slabs);
+    s.r = i / (unsigned)a.slabs;
     s.g0 = sl * a.slab;
     s.groups = s.g0 + a.slab < a.G ? a.slab : a.G - s.g0;
-    const int per = a.C / a.G;
-    s.c0 = s.g0 * per;
-    s.chans = s.groups * per;
+    s.c0 = s.g0 * a.per;
+    s.chans = s.groups * a.per;
     s.packs = (s.chans + V - 1) / V;
-    const int wide = s.packs < NT ? s.packs : NT;
-    s.px = threadIdx.x % wide;
-    s.ty = threadIdx.x / wide;
-    s.rows = NT / wide;
-    if (s.ty >= s.rows) s.packs = 0;      // threads left over
+    s.wide = s.packs < NT ? s.packs : NT;
+    s.rows = NT / s.wide;
+    s.ty = threadIdx.x / s.wide;
+    s.px = threadIdx.x - s.ty * s.wide;
     s.p0 = s.chunk * a.chunk;
     s.p1 = s.p0 + a.chunk < a.S ? s.p0 + a.chunk : a.S;
+    s.count = s.ty < s.rows ? ((int)(s.p1 - s.p0) - s.ty + s.rows - 1) / s.rows : 0;      // positions of the thread
+    if (s.ty >= s.rows) s.packs = 0;      // threads left over
     return s;
 }
-__device__ __forceinline__ int columns(const Spot &s, int V) { const int p = (s.chans + V - 1) / V; return p < NT ? p : NT; }
-
-__device__ __forceinline__ float warp_sum(float v)
+// Number of positions that the threads of row `ty` have.
+__device__ __forceinline__ float positions(const Spot &s, int ty)
 {
-#pragma unroll
-    for (int m = 16; m >= 1; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
-    return v;
+    const int n = (int)(s.p1 - s.p0), each = n / s.rows;
+    return (float)(each + (ty < n - each * s.rows ? 1 : 0));
 }
 
-// Calls f(pack of x, pack of dy, position) for the positions of a thread, AHEAD of them on their way.
-template <typename T, int V, bool VEC, bool TWO, typename F>
-__device__ __forceinline__ void walk(const NormArgs &a, const Spot &s, int p, const F &f)
+// Calls f(pack of x, pack of dy, index) for the positions of a thread, AHEAD of them on their way.
+// peek(pack of x) sees the first of them before.
+struct Nothing {
+    template <typename R> __device__ __forceinline__ void operator()(const R &) const {}
+};
+template <typename T, int V, bool VEC, bool TWO, typename F, typename Peek = Nothing>
+__device__ __forceinline__ void walk(const NormArgs &a, const Spot &s, int p, const F &f, const Peek &peek = Peek())
 {
     using R = RawPack<T, V, VEC>;
     constexpr int AHEAD = TWO ? 2 : 4;
     const int left = s.chans - p * V;
-    const T *x = static_cast<const T *>(a.x.p) + s.r * a.x.sb + s.c0 + p * V;
-    const T *g = TWO ? static_cast<const T *>(a.dy.p) + s.r * a.dy.sb + s.c0 + p * V : nullptr;
+    const T *x = static_cast<const T *>(a.x.p) + s.r * a.x.sb + s.c0 + p * V + (s.p0 + s.ty) * a.x.st;
+    const T *g = TWO ? static_cast<const T *>(a.dy.p) + s.r * a.dy.sb + s.c0 + p * V + (s.p0 + s.ty) * a.dy.st : nullptr;
+    const int64_t dx = s.rows * a.x.st, dg = TWO ? s.rows * a.dy.st : 0;
     R px[AHEAD], pg[AHEAD];
-    auto fetch = [&](int i, int64_t q) {
-        px[i].load(x + q * a.x.st, q < s.p1 ? left : 0);
-        if (TWO) pg[i].load(g + q * a.dy.st, q < s.p1 ? left : 0);
+    auto fetch = [&](int i, bool there) {
+        px[i].load(x, there ? left : 0);
+        x += dx;
+        if (TWO) {
+            pg[i].load(g, there ? left : 0);
+            g += dg;
+        }
     };
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) fetch(i, s.p0 + s.ty + (int64_t)i * s.rows);
-    for (int64_t q = s.p0 + s.ty; q < s.p1; q += (int64_t)AHEAD * s.rows) {
+    for (int i = 0; i < AHEAD; ++i) fetch(i, i < s.count);
+    peek(px[0]);
+    int q = 0;
+    for (; q + AHEAD <= s.count; q += AHEAD) {
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            const int64_t at = q + (int64_t)i * s.rows;
             const R cx = px[i], cg = pg[i];
-            fetch(i, at + (int64_t)AHEAD * s.rows);
-            if (at < s.p1) f(cx, cg, at);
+            fetch(i, q + i + AHEAD < s.count);
+            f(cx, cg, q + i);
         }
     }
+#pragma unroll
+    for (int i = 0; i < AHEAD - 1; ++i)
+        if (q + i < s.count) f(px[i], pg[i], q + i);
 }
 template <typename T, int V, bool VEC>
 __device__ __forceinline__ float2 pair_of(const RawPack<T, V, VEC> &r, int i)
@@ -315,121 +445,162 @@ __device__ __forceinline__ float2 pair_of(const RawPack<T, V, VEC> &r, int i)
 }
 
 // Moments of every group over the block's positions, in s_m (see map_smem), passed to out(group of the block, moments).
-// A thread takes the moments of its channels about their first value, so that a large common offset costs no digits.
+// A thread takes the moments of its channels about their first value, so that a large common offset costs no digits; where
+// whole packs belong to one group, it joins those of a pack.
 template <typename T, int V, bool VEC, typename Out>
 __device__ __forceinline__ void block_moments(const NormArgs &a, const Spot &s, float2 *s_m, const Out &out)
 {
     constexpr int P = V > 1 ? V / 2 : 1;
-    for (int p = s.px; p < s.packs; p += columns(s, V)) {
+    const bool whole = V > 1 && a.per % V == 0;
+    const int entries = whole ? s.chans / V : s.chans;      // of a row in s_m
+    for (int p = s.px; p < s.packs; p += s.wide) {
         float2 k[P], sum[P], sq[P];
-        int count = 0;
         const int left = s.chans - p * V;
 #pragma unroll
         for (int i = 0; i < P; ++i) k[i] = sum[i] = sq[i] = both(0.0f);
-        if (s.p0 + s.ty < s.p1) {
-            RawPack<T, V, VEC> head;
-            head.load(static_cast<const T *>(a.x.p) + s.r * a.x.sb + s.c0 + p * V + (s.p0 + s.ty) * a.x.st, left);
-#pragma unroll
-            for (int i = 0; i < P; ++i) k[i] = pair_of(head, i);
-        }
-        walk<T, V, VEC, false>(a, s, p, [&](const RawPack<T, V, VEC> &x, const RawPack<T, V, VEC> &, int64_t) {
+        walk<T, V, VEC, false>(a, s, p, [&](const RawPack<T, V, VEC> &x, const RawPack<T, V, VEC> &, int) {
 #pragma unroll
             for (int i = 0; i < P; ++i) {
-                const float2 f = pair_of(x, i), d = make_float2(f.x - k[i].x, f.y - k[i].y);
+                const float2 d = add2(pair_of(x, i), k[i]);
                 sum[i] = add2(sum[i], d);
                 sq[i] = fma2(d, d, sq[i]);
             }
-            ++count;
-        });
-        const float inv = count ? 1.0f / count : 0.0f;
+        }, [&](const RawPack<T, V, VEC> &x) {
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-            float2 *to = s_m + s.ty * s.chans + p * V + 2 * i;
-            if (2 * i < left) to[0] = make_float2(fmaf(sum[i].x, inv, k[i].x), max_nan(sq[i].x - sum[i].x * sum[i].x * inv, 0.0f));
-            if (V > 1 && 2 * i + 1 < left) to[1] = make_float2(fmaf(sum[i].y, inv, k[i].y), max_nan(sq[i].y - sum[i].y * sum[i].y * inv, 0.0f));
+            for (int i = 0; i < P; ++i) {
+                const float2 f = pair_of(x, i);
+                k[i] = make_float2(-f.x, -f.y);
+            }
+        });
+        const float n = (float)s.count, inv = s.count > 0 ? 1.0f / n : 0.0f;
+        float mean[V], m2[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float t = (i & 1) ? sum[i / 2].y : sum[i / 2].x, u = (i & 1) ? sq[i / 2].y : sq[i / 2].x, b = (i & 1) ? k[i / 2].y : k[i / 2].x;
+            mean[i] = fmaf(t, inv, -b);
+            m2[i] = max_nan(fmaf(-t * inv, t, u), 0.0f);
+        }
+        if (whole) {
+            float off = 0.0f, total = 0.0f;
+#pragma unroll
+            for (int i = 1; i < V; ++i) off += mean[i] - mean[0];
+            off *= 1.0f / V;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float d = (mean[i] - mean[0]) - off;
+                total += fmaf(n * d, d, m2[i]);
+            }
+            s_m[s.ty * entries + p] = make_float2(mean[0] + off, total);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (i < left) s_m[s.ty * entries + p * V + i] = make_float2(mean[i], m2[i]);
         }
     }
     __syncthreads();
-    const int per = a.C / a.G, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int64_t n = s.p1 - s.p0;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int each = whole ? a.per / V : a.per;             // entries of a group in a row
+    const int rows = s.p1 - s.p0 < s.rows ? (int)(s.p1 - s.p0) : s.rows;
+    const float weight = whole ? (float)V : 1.0f;
     for (int g = warp; g < s.groups; g += NT / 32) {
-        Moments m = {0.f, 0.f, 0.f};
-        int row = lane / per, c = lane % per;
-        const int step_row = 32 / per, step_c = 32 % per;
-        while (row < s.rows && row < n) {
-            const float2 f = s_m[row * s.chans + g * per + c];
-            m = merge(m, Moments{(float)((n - row + s.rows - 1) / s.rows), f.x, f.y});
-            row += step_row;
-            c += step_c;
-            if (c >= per) {
-                c -= per;
-                ++row;
-            }
-        }
-        m = merge_lanes(m);
+        const Moments m = join(rows * each, [&](int i) {
+            const int row = i / each;
+            const float2 f = s_m[row * entries + g * each + i - row * each];
+            return Moments{positions(s, row) * weight, f.x, f.y};
+        });
         if (lane == 0) out(g, m);
     }
 }
+
+// Group of a channel, for channels one after the other.
+struct GroupOf {
+    int g, rest;      // group, channels of it that are left
+    __device__ __forceinline__ GroupOf(int c, int per) : g(c / per) { rest = per - (c - g * per); }
+    __device__ __forceinline__ void step(int per)
+    {
+        if (--rest == 0) {
+            rest = per;
+            ++g;
+        }
+    }
+};
 
 // y from x with the groups' mean and rstd in s_m.
 template <typename T, int V, bool VEC>
 __device__ __forceinline__ void block_apply(const NormArgs &a, const Spot &s, const float2 *s_m)
 {
     constexpr int P = V > 1 ? V / 2 : 1;
-    const int per = a.C / a.G;
-    for (int p = s.px; p < s.packs; p += columns(s, V)) {
+    for (int p = s.px; p < s.packs; p += s.wide) {
         const int left = s.chans - p * V;
         float2 mean[P], scale[P], shift[P];
+        float wv[V], bv[V];
+        load_params<T, V, VEC>(wv, a.weight, s.c0 + p * V, left, a.params_f32, 1.0f);
+        load_params<T, V, VEC>(bv, a.bias, s.c0 + p * V, left, a.params_f32, 0.0f);
+        GroupOf group(p * V, a.per);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int c = p * V + i;
-            float m = 0.0f, sc = 0.0f, sh = 0.0f;
-            if (c < s.chans) {
-                const float2 f = s_m[c / per];
-                m = f.x;
-                sc = a.weight ? f.y * param<T>(a.weight, s.c0 + c, a.params_f32) : f.y;
-                sh = a.bias ? param<T>(a.bias, s.c0 + c, a.params_f32) : 0.0f;
-            }
-            if (i % 2 == 0) { mean[i / 2] = both(-m); scale[i / 2] = both(sc); shift[i / 2] = both(sh); }
-            else { mean[i / 2].y = -m; scale[i / 2].y = sc; shift[i / 2].y = sh; }
+        for (int i = 0; i < V; ++i, group.step(a.per)) {
+            const float2 f = p * V + i < s.chans ? s_m[group.g] : both(0.0f);
+            const float m = -f.x, sc = f.y * wv[i], sh = bv[i];
+            if (i % 2 == 0) { mean[i / 2] = both(m); scale[i / 2] = both(sc); shift[i / 2] = both(sh); }
+            else { mean[i / 2].y = m; scale[i / 2].y = sc; shift[i / 2].y = sh; }
         }
-        T *out = static_cast<T *>(a.y) + s.r * a.S * a.C + s.c0 + p * V;
-        walk<T, V, VEC, false>(a, s, p, [&](const RawPack<T, V, VEC> &x, const RawPack<T, V, VEC> &, int64_t q) {
+        T *out = static_cast<T *>(a.y) + (s.r * a.S + s.p0 + s.ty) * a.C + s.c0 + p * V;
+        const int64_t step = (int64_t)s.rows * a.C;
+        walk<T, V, VEC, false>(a, s, p, [&](const RawPack<T, V, VEC> &x, const RawPack<T, V, VEC> &, int) {
             Pack<T, V> y;
+            float2 v[P];
+#pragma unroll
+            for (int i = 0; i < P; ++i) v[i] = fma2(add2(pair_of(x, i), mean[i]), scale[i], shift[i]);
+            activate(v, a.act);
 #pragma unroll
             for (int i = 0; i < P; ++i) {
-                const float2 v = activate2(fma2(add2(pair_of(x, i), mean[i]), scale[i], shift[i]), a.act);
-                y.v[2 * i] = from_f32<T>(v.x);
-                if constexpr (V > 1) y.v[2 * i + 1] = from_f32<T>(v.y);
+                y.v[2 * i] = from_f32<T>(v[i].x);
+                if constexpr (V > 1) y.v[2 * i + 1] = from_f32<T>(v[i].y);
             }
-            store_pack<VEC>(out + q * a.C, y, left);
+            store_pack<VEC>(out, y, left);
+            out += step;
         });
     }
 }
 
 // What the backward needs of a pack's channels: (x - mean) rstd = x rstd + centre would lose digits, so both are kept.
-template <typename T, int V>
+template <typename T, int V, bool VEC>
 struct Channels {
     static constexpr int P = V > 1 ? V / 2 : 1;
     float2 mean[P], rstd[P], w[P], b[P];
     __device__ __forceinline__ Channels(const NormArgs &a, const Spot &s, int p)
     {
-        const int per = a.C / a.G;
+        float wv[V], bv[V];
+        load_params<T, V, VEC>(wv, a.weight, s.c0 + p * V, s.chans - p * V, a.params_f32, 1.0f);
+        load_params<T, V, VEC>(bv, a.bias, s.c0 + p * V, s.chans - p * V, a.params_f32, 0.0f);
+        GroupOf group(p * V, a.per);
+        const int64_t at = s.r * a.G + s.g0;
+        float m = -a.mean[at + group.g], r = a.rstd[at + group.g];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const int c = p * V + i;
-            const bool there = c < s.chans;
-            const int64_t g = s.r * a.G + (there ? (s.c0 + c) / per : s.g0);
-            const float m = -a.mean[g], r = a.rstd[g];
-            const float wv = (there && a.weight) ? param<T>(a.weight, s.c0 + c, a.params_f32) : 1.0f;
-            const float bv = (there && a.bias) ? param<T>(a.bias, s.c0 + c, a.params_f32) : 0.0f;
-            if (i % 2 == 0) { mean[i / 2] = both(m); rstd[i / 2] = both(r); w[i / 2] = both(wv); b[i / 2] = both(bv); }
-            else { mean[i / 2].y = m; rstd[i / 2].y = r; w[i / 2].y = wv; b[i / 2].y = bv; }
+            if (i % 2 == 0) { mean[i / 2] = both(m); rstd[i / 2] = both(r); w[i / 2] = both(wv[i]); b[i / 2] = both(bv[i]); }
+            else { mean[i / 2].y = m; rstd[i / 2].y = r; w[i / 2].y = wv[i]; b[i / 2].y = bv[i]; }
+            const int before = group.g;
+            group.step(a.per);
+            if (i + 1 < V && group.g != before && p * V + i + 1 < s.chans) {
+                m = -a.mean[at + group.g];
+                r = a.rstd[at + group.g];
+            }
         }
     }
-    __device__ __forceinline__ float2 normed(float2 x, int i) const { return mul2(add2(x, mean[i]), rstd[i]); }
-    // gradient in front of the activation
-    __device__ __forceinline__ float2 inner(float2 n, float2 up, int act, int i) const { return act ? mul2(up, activate_slope2(fma2(n, w[i], b[i]), act)) : up; }
+    // normed x, and the gradient in front of the activation
+    template <typename R>
+    __device__ __forceinline__ void get(float2 (&n)[P], float2 (&d)[P], const R &x, const R &up, int act) const
+    {
+        float2 pre[P];
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            n[i] = mul2(add2(pair_of(x, i), mean[i]), rstd[i]);
+            d[i] = pair_of(up, i);
+            pre[i] = fma2(n[i], w[i], b[i]);
+        }
+        activate_backward(d, pre, act);
+    }
 };
 
 // Per channel, over the block's positions: the sums of d n and of d (d: gradient in front of the activation, n: normed x),
@@ -438,18 +609,19 @@ template <typename T, int V, bool VEC>
 __device__ __forceinline__ void block_gradient_sums(const NormArgs &a, const Spot &s, float2 *s_m, float2 *s_c)
 {
     constexpr int P = V > 1 ? V / 2 : 1;
-    for (int p = s.px; p < s.packs; p += columns(s, V)) {
+    for (int p = s.px; p < s.packs; p += s.wide) {
         const int left = s.chans - p * V;
-        const Channels<T, V> h(a, s, p);
+        const Channels<T, V, VEC> h(a, s, p);
         float2 s1[P], s2[P];
 #pragma unroll
         for (int i = 0; i < P; ++i) s1[i] = s2[i] = both(0.0f);
-        walk<T, V, VEC, true>(a, s, p, [&](const RawPack<T, V, VEC> &x, const RawPack<T, V, VEC> &g, int64_t) {
+        walk<T, V, VEC, true>(a, s, p, [&](const RawPack<T, V, VEC> &x, const RawPack<T, V, VEC> &g, int) {
+            float2 n[P], d[P];
+            h.get(n, d, x, g, a.act);
 #pragma unroll
             for (int i = 0; i < P; ++i) {
-                const float2 n = h.normed(pair_of(x, i), i), d = h.inner(n, pair_of(g, i), a.act, i);
-                s1[i] = add2(s1[i], d);
-                s2[i] = fma2(d, n, s2[i]);
+                s1[i] = add2(s1[i], d[i]);
+                s2[i] = fma2(d[i], n[i], s2[i]);
             }
         });
 #pragma unroll
@@ -475,7 +647,7 @@ __device__ __forceinline__ void block_gradient_sums(const NormArgs &a, const Spo
 template <typename T, typename Get, typename Out>
 __device__ __forceinline__ void group_sums(const NormArgs &a, const Spot &s, const Get &get, const Out &out)
 {
-    const int per = a.C / a.G, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int per = a.per, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     for (int g = warp; g < s.groups; g += NT / 32) {
         float2 t = both(0.0f);
         for (int i = lane; i < per; i += 32) {
@@ -492,28 +664,31 @@ template <typename T, int V, bool VEC>
 __device__ __forceinline__ void block_gradient(const NormArgs &a, const Spot &s, const float2 *s_g)
 {
     constexpr int P = V > 1 ? V / 2 : 1;
-    const int per = a.C / a.G;
-    for (int p = s.px; p < s.packs; p += columns(s, V)) {
+    for (int p = s.px; p < s.packs; p += s.wide) {
         const int left = s.chans - p * V;
-        const Channels<T, V> h(a, s, p);
+        const Channels<T, V, VEC> h(a, s, p);
         float2 u[P], v[P];
+        GroupOf group(p * V, a.per);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float2 f = s_g[p * V + i < s.chans ? (p * V + i) / per : 0];
+        for (int i = 0; i < V; ++i, group.step(a.per)) {
+            const float2 f = s_g[p * V + i < s.chans ? group.g : 0];
             if (i % 2 == 0) { u[i / 2] = both(-f.x); v[i / 2] = both(-f.y); }
             else { u[i / 2].y = -f.x; v[i / 2].y = -f.y; }
         }
-        T *out = static_cast<T *>(a.dx) + s.r * a.S * a.C + s.c0 + p * V;
-        walk<T, V, VEC, true>(a, s, p, [&](const RawPack<T, V, VEC> &x, const RawPack<T, V, VEC> &g, int64_t q) {
+        T *out = static_cast<T *>(a.dx) + (s.r * a.S + s.p0 + s.ty) * a.C + s.c0 + p * V;
+        const int64_t step = (int64_t)s.rows * a.C;
+        walk<T, V, VEC, true>(a, s, p, [&](const RawPack<T, V, VEC> &x, const RawPack<T, V, VEC> &g, int) {
             Pack<T, V> o;
+            float2 n[P], d[P];
+            h.get(n, d, x, g, a.act);
 #pragma unroll
             for (int i = 0; i < P; ++i) {
-                const float2 n = h.normed(pair_of(x, i), i), d = h.inner(n, pair_of(g, i), a.act, i);
-                const float2 e = mul2(h.rstd[i], fma2(n, v[i], fma2(d, h.w[i], u[i])));
+                const float2 e = mul2(h.rstd[i], fma2(n[i], v[i], fma2(d[i], h.w[i], u[i])));
                 o.v[2 * i] = from_f32<T>(e.x);
                 if constexpr (V > 1) o.v[2 * i + 1] = from_f32<T>(e.y);
             }
-            store_pack<VEC>(out + q * a.C, o, left);
+            store_pack<VEC>(out, o, left);
+            out += step;
         });
     }
 }
@@ -521,7 +696,7 @@ __device__ __forceinline__ void block_gradient(const NormArgs &a, const Spot &s,
 // Final mean and rstd of a group.
 __device__ __forceinline__ void finish_group(const NormArgs &a, const Spot &s, float2 *s_m, int g, const Moments &m, bool write)
 {
-    const float rstd = 1.0f / sqrtf(m.m2 / m.n + a.eps);
+    const float rstd = inverse_sqrt(m.m2 / m.n + a.eps);
     s_m[g] = make_float2(m.mean, rstd);
     if (write) {
         a.mean[s.r * a.G + s.g0 + g] = m.mean;
@@ -541,10 +716,9 @@ __global__ void __launch_bounds__(NT, 3) norm_cluster_forward_kernel(const NormA
     Moments *own = reinterpret_cast<Moments *>(s_m + a.smem);
     block_moments<T, V, VEC>(a, s, s_m, [&](int g, const Moments &m) { own[g] = m; });
     cluster.sync();
-    for (int g = threadIdx.x; g < s.groups; g += NT) {
-        Moments m = {0.f, 0.f, 0.f};
-        for (int r = 0; r < a.chunks; ++r) m = merge(m, cluster.map_shared_rank(own, r)[g]);
-        finish_group(a, s, s_m, g, m, s.chunk == 0);
+    for (int g = threadIdx.x / 32; g < s.groups; g += NT / 32) {
+        const Moments m = join(a.chunks, [&](int r) { return cluster.map_shared_rank(own, r)[g]; });
+        if (threadIdx.x % 32 == 0) finish_group(a, s, s_m, g, m, s.chunk == 0);
     }
     cluster.sync();      // nobody reads another block's moments any more; s_m is written
     block_apply<T, V, VEC>(a, s, s_m);
@@ -557,11 +731,11 @@ __global__ void __launch_bounds__(NT, 3) norm_cluster_backward_kernel(const Norm
     namespace cg = cooperative_groups;
     const cg::cluster_group cluster = cg::this_cluster();
     const Spot s = place<V>(a);
-    float2 *s_c = s_m + a.smem, *own = s_c + a.slab * (a.C / a.G);
+    float2 *s_c = s_m + a.smem, *own = s_c + a.slab * a.per;
     block_gradient_sums<T, V, VEC>(a, s, s_m, s_c);
     group_sums<T>(a, s, [&](int c) { return s_c[c]; }, [&](int g, float2 t) { own[g] = t; });
     cluster.sync();
-    const float inv = 1.0f / ((float)a.S * (float)(a.C / a.G));
+    const float inv = 1.0f / ((float)a.S * (float)a.per);
     for (int g = threadIdx.x; g < s.groups; g += NT) {
         float2 t = both(0.0f);
         for (int r = 0; r < a.chunks; ++r) t = add2(t, cluster.map_shared_rank(own, r)[g]);
@@ -590,16 +764,13 @@ __global__ void __launch_bounds__(NT, 3) norm_apply_kernel(const NormArgs a)
 {
     extern __shared__ float2 s_m[];      // [groups]
     const Spot s = place<V>(a);
-    const int per = a.C / a.G, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    for (int g = warp; g < s.groups; g += NT / 32) {
-        Moments m = {0.f, 0.f, 0.f};
-        for (int i = lane; i < a.chunks; i += 32) {
+    for (int g = threadIdx.x / 32; g < s.groups; g += NT / 32) {
+        const Moments m = join(a.chunks, [&](int i) {
             const int64_t lo = i * a.chunk, hi = lo + a.chunk < a.S ? lo + a.chunk : a.S;
             const float *in = a.part + ((s.r * a.chunks + i) * a.G + s.g0 + g) * 2;
-            m = merge(m, Moments{(float)((hi - lo) * per), in[0], in[1]});
-        }
-        m = merge_lanes(m);
-        if (lane == 0) finish_group(a, s, s_m, g, m, s.chunk == 0);
+            return Moments{(float)((hi - lo) * a.per), in[0], in[1]};
+        });
+        if (threadIdx.x % 32 == 0) finish_group(a, s, s_m, g, m, s.chunk == 0);
     }
     __syncthreads();
     block_apply<T, V, VEC>(a, s, s_m);
@@ -618,7 +789,7 @@ __global__ void __launch_bounds__(NT, 3) norm_backward_apply_kernel(const NormAr
 {
     extern __shared__ float2 s_m[];      // [groups]
     const Spot s = place<V>(a);
-    const float inv = 1.0f / ((float)a.S * (float)(a.C / a.G));
+    const float inv = 1.0f / ((float)a.S * (float)a.per);
     group_sums<T>(a, s, [&](int c) {
         float2 t = both(0.0f);
 #pragma unroll 4
@@ -687,10 +858,12 @@ Plan plan_of(int64_t R, int64_t S, int C, int G, int dtype, bool backward)
     }
     p.chunk = ceil_div(S, chunks);
     p.chunks = p.cluster ? cluster : (int)ceil_div(S, p.chunk);
-    // tokens: half of the threads that the GPU holds; backward at least four samples each, which leave one partial sum
+    // tokens: as many threads as are resident at once, so that no block waits for another's end; backward at least four
+    // samples each, which leave one partial sum
     int L, K;
     token_shape(per, V, &L, &K);
-    int64_t strides = ceil_div(148 * 1024, (int64_t)G * L);
+    int64_t strides = (148ll * NT * (K * V > 8 ? 1 : (backward ? 2 : 4))) / ((int64_t)G * L);
+    if (strides < 1) strides = 1;
     if (backward && strides > R / 4) strides = R / 4 > 64 ? R / 4 : 64;
     p.strides = strides < R ? strides : R;
     p.forward_bytes = p.tokens || p.cluster ? 0 : R * p.chunks * G * 2 * 4;
@@ -872,6 +1045,7 @@ Plan apply_plan(NormArgs &a, int dtype, void *ws, bool backward)
     a.chunks = p.chunks;
     a.slab = p.slab;
     a.slabs = p.slabs;
+    a.per = a.C / a.G;
     a.part = static_cast<float *>(ws);
     return p;
 }

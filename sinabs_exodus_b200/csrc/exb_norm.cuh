@@ -21,6 +21,7 @@ struct NormArgs {
     float *part;                         // partial sums: statistics [R][chunks][G][2] or gradients [rows][2][C]
     int64_t chunk;                       // positions of a block
     int chunks, slab, slabs;             // blocks of a sample; groups of a block; blocks of a row
+    int per;                             // channels of a group
     int smem;                            // pairs of shared memory that the map kernels work in
 };
 

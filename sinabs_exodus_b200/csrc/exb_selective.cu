@@ -986,53 +986,65 @@ struct PutD {
 // ---------------------------------------------------------------------------------------------- one token
 
 // A thread takes four states of a channel in ITEMS batch items, `apart` of them between two: the rates are loaded once, and
-// all states are on their way together (the state is what has to move).
+// all states are on their way together (the state is what has to move).  The channel's first ITEMS lanes do the work that is
+// not per state for one batch item each.
 template <typename T, int L, int ITEMS, bool VEC>
-__global__ void __launch_bounds__(256) sel_step_kernel(const SelStepArgs a, int64_t apart)
+__global__ void __launch_bounds__(256) sel_step_kernel(const SelStepArgs a, unsigned apart)
 {
-    const int64_t i = (blockIdx.x * 256ll + threadIdx.x) / L;
-    const int l = threadIdx.x % L, n0 = 4 * l;
-    const bool alive = i < apart * a.M;
-    const int64_t b0 = alive ? i / a.M : 0;
-    const int m = alive ? (int)(i % a.M) : 0, g = m / (a.M / a.G);
-    RawPack<T, 1, false> x[ITEMS], dt[ITEMS], z[ITEMS];
-    RawPack<T, 4, VEC> vb[ITEMS], vc[ITEMS];
+    const unsigned i = (blockIdx.x * 256u + threadIdx.x) / L;
+    const int l = threadIdx.x % L, n0 = 4 * l, lane = threadIdx.x % 32;
+    const unsigned tiles = a.M;
+    const unsigned b0 = i / tiles;
+    const bool alive = b0 < apart;
+    const int m = (int)(i - b0 * tiles), g = m / (a.M / a.G);
     RawPack<float, 4, VEC> vh[ITEMS], va;
+    RawPack<T, 4, VEC> vb[ITEMS], vc[ITEMS];
     va.load(a.A + (int64_t)m * a.N + n0, alive ? a.N - n0 : 0);
+    float *h0 = a.h + b0 * a.sh + (int64_t)m * a.N + n0;
+    const int64_t hs = apart * a.sh, bs = apart * a.Bm.sb, cs = apart * a.Cm.sb;
+    const T *bp = static_cast<const T *>(a.Bm.p) + b0 * a.Bm.sb + g * a.N + n0, *cp = static_cast<const T *>(a.Cm.p) + b0 * a.Cm.sb + g * a.N + n0;
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
-        const int64_t b = b0 + k * apart;
-        const int here = alive && b < a.B;
-        vh[k].load(a.h + b * a.sh + (int64_t)m * a.N + n0, here ? a.N - n0 : 0);
-        x[k].load(static_cast<const T *>(a.x.p) + b * a.x.sb + m, here);
-        dt[k].load(static_cast<const T *>(a.dt.p) + b * a.dt.sb + m, here);
-        z[k].load(static_cast<const T *>(a.z.p) + b * a.z.sb + m, here && a.z.p);
-        vb[k].load(static_cast<const T *>(a.Bm.p) + b * a.Bm.sb + (int64_t)g * a.N + n0, here ? a.N - n0 : 0);
-        vc[k].load(static_cast<const T *>(a.Cm.p) + b * a.Cm.sb + (int64_t)g * a.N + n0, here ? a.N - n0 : 0);
+        const int have = alive && b0 + k * apart < a.B ? a.N - n0 : 0;
+        vh[k].load(h0 + k * hs, have);
+        vb[k].load(bp + k * bs, have);
+        vc[k].load(cp + k * cs, have);
     }
+    const int64_t own = b0 + (int64_t)(l < ITEMS ? l : 0) * apart;      // batch item that this lane prepares
+    const int mine = alive && own < a.B;
+    RawPack<T, 1, false> vx, vd, vz;
+    vx.load(static_cast<const T *>(a.x.p) + own * a.x.sb + m, mine);
+    vd.load(static_cast<const T *>(a.dt.p) + own * a.dt.sb + m, mine);
+    vz.load(static_cast<const T *>(a.z.p) + own * a.z.sb + m, mine && a.z.p);
     const float bias = alive && a.dt_bias ? a.dt_bias[m] : 0.0f, skip = alive && a.D ? a.D[m] : 0.0f;
+    const float x = vx.get(0);
+    float dt = vd.get(0) + bias;
+    if (a.softplus) dt = softplus_f(dt);
+    const float u = dt * x;
+    float y[ITEMS], A2[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) A2[j] = va.get(j) * LOG2E;
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
-        const int64_t b = b0 + k * apart;
-        float d = dt[k].get(0) + bias;
-        if (a.softplus) d = softplus_f(d);
-        const float u = d * x[k].get(0);
-        float y = 0.0f;
+        const int from = (lane & ~(L - 1)) + (ITEMS > 1 ? k : 0);
+        const float d = ITEMS > 1 ? __shfl_sync(0xffffffffu, dt, from) : dt, w = ITEMS > 1 ? __shfl_sync(0xffffffffu, u, from) : u;
+        y[k] = 0.0f;
         Pack<float, 4> h;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            h.v[j] = fmaf(exp2_fast(d * va.get(j) * LOG2E), vh[k].get(j), u * vb[k].get(j));
-            y = fmaf(vc[k].get(j), h.v[j], y);
+            h.v[j] = fmaf(exp2_fast(d * A2[j]), vh[k].get(j), w * vb[k].get(j));
+            y[k] = fmaf(vc[k].get(j), h.v[j], y[k]);
         }
-        const bool here = alive && b < a.B;
-        store_pack<VEC>(a.h + b * a.sh + (int64_t)m * a.N + n0, h, here ? a.N - n0 : 0);
-#pragma unroll
-        for (int s = 1; s < L; s <<= 1) y += __shfl_xor_sync(0xffffffffu, y, s);
-        if (here && l == 0) {
-            y = fmaf(skip, x[k].get(0), y);
-            if (a.z.p) y *= silu_f(z[k].get(0));
-            static_cast<T *>(a.y)[b * a.M + m] = from_f32<T>(y);
-        }
+        store_pack<VEC>(h0 + k * hs, h, alive && b0 + k * apart < a.B ? a.N - n0 : 0);
+    }
+    // the lanes of rank k L/ITEMS end up with batch item k, which the lane l = k holds the inputs of
+    reduce_scatter<ITEMS, L, 1>(y, lane);
+    float sum = y[0];
+    if (ITEMS > 1 && L > ITEMS) sum = __shfl_sync(0xffffffffu, sum, (lane & ~(L - 1)) + (l < ITEMS ? l : 0) * (L / ITEMS));
+    if (mine && l < ITEMS) {
+        float out = fmaf(skip, x, sum);
+        if (a.z.p) out *= silu_f(vz.get(0));
+        static_cast<T *>(a.y)[own * a.M + m] = from_f32<T>(out);
     }
 }
 
@@ -1125,12 +1137,13 @@ cudaError_t backward_dispatch(const SelArgs &a, const SelPlan &p, void *dB, void
 template <typename T, int L, bool VEC>
 cudaError_t step_typed(const SelStepArgs &a, cudaStream_t s)
 {
-    // Four batch items per thread once that leaves two blocks for every SM.
-    const bool many = a.B >= 4 && ceil_div(a.B, 4) * a.M * L >= 2 * 148 * 256;
-    const int64_t apart = many ? ceil_div(a.B, 4) : a.B;
+    // Several batch items per thread once that leaves two blocks for every SM.
+    constexpr int ITEMS = L < 4 ? L : 4;
+    const bool many = ceil_div(a.B, ITEMS) * a.M * L >= 2 * 148 * 256;
+    const int64_t apart = many ? ceil_div(a.B, ITEMS) : a.B;
     const unsigned grid = (unsigned)ceil_div(apart * a.M * L, 256);
-    if (many) sel_step_kernel<T, L, 4, VEC><<<grid, 256, 0, s>>>(a, apart);
-    else sel_step_kernel<T, L, 1, VEC><<<grid, 256, 0, s>>>(a, apart);
+    if (many) sel_step_kernel<T, L, ITEMS, VEC><<<grid, 256, 0, s>>>(a, (unsigned)apart);
+    else sel_step_kernel<T, L, 1, VEC><<<grid, 256, 0, s>>>(a, (unsigned)apart);
     return cudaGetLastError();
 }
 
