@@ -6,6 +6,7 @@ exception is raised; there is no PyTorch or CPU substitute.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from typing import Optional, Tuple
 
@@ -250,6 +251,10 @@ def _stream(dev: torch.device):
     if _raw_stream is not None:
         return _raw_stream(dev.index)
     return torch.cuda.current_stream(dev).cuda_stream
+
+
+def _stream_of(index: int):
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
 
 
 class ParamSpec(tuple):
@@ -578,101 +583,125 @@ def rows_of(t: Optional[torch.Tensor]):
     """View of a (B, T, ...) or (B, ...) tensor whose trailing dimensions are contiguous; None passes through."""
     if t is None:
         return None
-    if t.ndim > 2:
-        return Rows(t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0)
-    return Rows(t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0, 0)
+    s = t.stride()
+    return Rows(t.data_ptr(), s[0], s[1] if len(s) > 2 else 0)
 
 
-def _workspace(nbytes: int, dev: torch.device) -> Tuple[Optional[torch.Tensor], int]:
-    return (torch.empty(nbytes, dtype=torch.uint8, device=dev), nbytes) if nbytes > 0 else (None, 0)
+# Sizes of the operators' scratch and checkpoint memory depend on the shape alone.
+@functools.lru_cache(maxsize=4096)
+def _selective_workspace_bytes(B, T, M, N, G, backward):
+    return int(load().exb_selective_workspace_bytes(B, T, M, N, G, backward))
 
 
-def selective_checkpoint(B: int, T: int, M: int, N: int, dev: torch.device) -> torch.Tensor:
-    return torch.empty(int(load().exb_selective_checkpoint_floats(B, T, M, N)), dtype=torch.float32, device=dev)
+@functools.lru_cache(maxsize=4096)
+def _selective_checkpoint_floats(B, T, M, N):
+    return int(load().exb_selective_checkpoint_floats(B, T, M, N))
+
+
+@functools.lru_cache(maxsize=4096)
+def _causal_conv_workspace_bytes(B, T, M, W):
+    return int(load().exb_causal_conv_workspace_bytes(B, T, M, W))
+
+
+@functools.lru_cache(maxsize=4096)
+def _group_norm_workspace_bytes(R, S, C, G, dtype, backward):
+    return int(load().exb_group_norm_workspace_bytes(R, S, C, G, dtype, backward))
+
+
+def _workspace(nbytes: int, like: torch.Tensor) -> Optional[torch.Tensor]:
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes > 0 else None
+
+
+def _launched(status: int, what: str, like: torch.Tensor) -> None:
+    if status != 0:
+        _check(status, what)
+    if _check_every_call:
+        _after_launch(like.device)
+
+
+def selective_checkpoint(B: int, T: int, M: int, N: int, like: torch.Tensor) -> torch.Tensor:
+    return torch.empty(_selective_checkpoint_floats(B, T, M, N), dtype=torch.float32, device=like.device)
 
 
 def selective_forward(y, h_last, ckpt, x, dt, A, Bm, Cm, D, z, dt_bias, h0, lengths, softplus: bool, B: int, T: int, M: int,
                       N: int, G: int) -> None:
-    lib, dev = load(), x.device
-    ws, nbytes = _workspace(int(lib.exb_selective_workspace_bytes(B, T, M, N, G, 0)), dev)
-    st = lib.exb_selective_forward(ptr(y), ptr(h_last), ptr(ckpt), rows_of(x), rows_of(dt), ptr(A), rows_of(Bm), rows_of(Cm), ptr(D),
-                                   rows_of(z), ptr(dt_bias), ptr(h0), ptr(lengths), int(softplus), ptr(ws), nbytes, DTYPES[x.dtype],
-                                   B, T, M, N, G, dev.index, _stream(dev))
-    _check(st, "exb_selective_forward")
-    _after_launch(dev)
+    nbytes, dev = _selective_workspace_bytes(B, T, M, N, G, 0), x.get_device()
+    ws = _workspace(nbytes, x)
+    st = load().exb_selective_forward(y.data_ptr(), h_last.data_ptr(), ptr(ckpt), rows_of(x), rows_of(dt), A.data_ptr(), rows_of(Bm),
+                                      rows_of(Cm), ptr(D), rows_of(z), ptr(dt_bias), ptr(h0), ptr(lengths), softplus, ptr(ws), nbytes,
+                                      DTYPES[x.dtype], B, T, M, N, G, dev, _stream_of(dev))
+    _launched(st, "exb_selective_forward", x)
 
 
 def selective_backward(dx, ddt, dA, dB, dC, dD, dz, ddt_bias, dh0, dy, dh_last, ckpt, x, dt, A, Bm, Cm, D, z, dt_bias, lengths,
                        softplus: bool, B: int, T: int, M: int, N: int, G: int) -> None:
-    lib, dev = load(), x.device
-    ws, nbytes = _workspace(int(lib.exb_selective_workspace_bytes(B, T, M, N, G, 1)), dev)
-    st = lib.exb_selective_backward(ptr(dx), ptr(ddt), ptr(dA), ptr(dB), ptr(dC), ptr(dD), ptr(dz), ptr(ddt_bias), ptr(dh0),
-                                    rows_of(dy), ptr(dh_last), ptr(ckpt), rows_of(x), rows_of(dt), ptr(A), rows_of(Bm), rows_of(Cm),
-                                    ptr(D), rows_of(z), ptr(dt_bias), ptr(lengths), int(softplus), ptr(ws), nbytes, DTYPES[x.dtype],
-                                    B, T, M, N, G, dev.index, _stream(dev))
-    _check(st, "exb_selective_backward")
-    _after_launch(dev)
+    nbytes, dev = _selective_workspace_bytes(B, T, M, N, G, 1), x.get_device()
+    ws = _workspace(nbytes, x)
+    st = load().exb_selective_backward(dx.data_ptr(), ddt.data_ptr(), dA.data_ptr(), dB.data_ptr(), dC.data_ptr(), ptr(dD), ptr(dz),
+                                       ptr(ddt_bias), ptr(dh0), rows_of(dy), ptr(dh_last), ckpt.data_ptr(), rows_of(x), rows_of(dt),
+                                       A.data_ptr(), rows_of(Bm), rows_of(Cm), ptr(D), rows_of(z), ptr(dt_bias), ptr(lengths),
+                                       softplus, ptr(ws), nbytes, DTYPES[x.dtype], B, T, M, N, G, dev, _stream_of(dev))
+    _launched(st, "exb_selective_backward", x)
 
 
 def selective_step(y, h, x, dt, A, Bm, Cm, D, z, dt_bias, softplus: bool, B: int, M: int, N: int, G: int) -> None:
-    dev = x.device
+    dev = x.get_device()
     st = load().exb_selective_step(y.data_ptr(), h.data_ptr(), h.stride(0), rows_of(x), rows_of(dt), A.data_ptr(), rows_of(Bm),
-                                   rows_of(Cm), ptr(D), rows_of(z), ptr(dt_bias), int(softplus), DTYPES[x.dtype], B, M, N, G,
-                                   dev.index, _stream(dev))
-    _check(st, "exb_selective_step")
-    _after_launch(dev)
+                                   rows_of(Cm), ptr(D), rows_of(z), ptr(dt_bias), softplus, DTYPES[x.dtype], B, M, N, G, dev,
+                                   _stream_of(dev))
+    _launched(st, "exb_selective_step", x)
 
 
 def causal_conv_forward(y, last, x, weight, bias, state, lengths, activation, B: int, T: int, M: int, W: int) -> None:
-    dev = x.device
-    st = load().exb_causal_conv_forward(ptr(y), ptr(last), rows_of(x), ptr(weight), ptr(bias), ptr(state), ptr(lengths),
-                                        ACTIVATIONS[activation], int(weight.dtype == torch.float32), DTYPES[x.dtype], B, T, M, W,
-                                        dev.index, _stream(dev))
-    _check(st, "exb_causal_conv_forward")
-    _after_launch(dev)
+    dev = x.get_device()
+    st = load().exb_causal_conv_forward(y.data_ptr(), ptr(last), rows_of(x), weight.data_ptr(), ptr(bias), ptr(state), ptr(lengths),
+                                        ACTIVATIONS[activation], weight.dtype == torch.float32, DTYPES[x.dtype], B, T, M, W, dev,
+                                        _stream_of(dev))
+    _launched(st, "exb_causal_conv_forward", x)
 
 
 def causal_conv_backward(dx, dweight, dbias, dstate, dy, dlast, x, weight, bias, state, lengths, activation, B: int, T: int, M: int,
                          W: int) -> None:
-    lib, dev = load(), x.device
-    ws, nbytes = _workspace(int(lib.exb_causal_conv_workspace_bytes(B, T, M, W)), dev)
-    st = lib.exb_causal_conv_backward(ptr(dx), ptr(dweight), ptr(dbias), ptr(dstate), rows_of(dy), ptr(dlast), rows_of(x), ptr(weight),
-                                      ptr(bias), ptr(state), ptr(lengths), ACTIVATIONS[activation],
-                                      int(weight.dtype == torch.float32), ptr(ws), nbytes, DTYPES[x.dtype], B, T, M, W, dev.index,
-                                      _stream(dev))
-    _check(st, "exb_causal_conv_backward")
-    _after_launch(dev)
+    nbytes, dev = _causal_conv_workspace_bytes(B, T, M, W), x.get_device()
+    ws = _workspace(nbytes, x)
+    st = load().exb_causal_conv_backward(dx.data_ptr(), dweight.data_ptr(), ptr(dbias), ptr(dstate), rows_of(dy), ptr(dlast), rows_of(x),
+                                         weight.data_ptr(), ptr(bias), ptr(state), ptr(lengths), ACTIVATIONS[activation],
+                                         weight.dtype == torch.float32, ptr(ws), nbytes, DTYPES[x.dtype], B, T, M, W, dev,
+                                         _stream_of(dev))
+    _launched(st, "exb_causal_conv_backward", x)
 
 
 def causal_conv_step(y, state, x, weight, bias, activation, B: int, M: int, W: int) -> None:
-    dev = x.device
+    dev = x.get_device()
     st = load().exb_causal_conv_step(y.data_ptr(), state.data_ptr(), state.stride(0), rows_of(x), weight.data_ptr(), ptr(bias),
-                                     ACTIVATIONS[activation], int(weight.dtype == torch.float32), DTYPES[x.dtype], B, M, W, dev.index,
-                                     _stream(dev))
-    _check(st, "exb_causal_conv_step")
-    _after_launch(dev)
+                                     ACTIVATIONS[activation], weight.dtype == torch.float32, DTYPES[x.dtype], B, M, W, dev,
+                                     _stream_of(dev))
+    _launched(st, "exb_causal_conv_step", x)
+
+
+def _f32_params(weight, bias) -> bool:
+    p = weight if weight is not None else bias
+    return p is None or p.dtype == torch.float32
 
 
 def group_norm_forward(y, mean, rstd, x, weight, bias, eps: float, activation, R: int, S: int, C: int, G: int) -> None:
-    lib, dev = load(), x.device
-    f32 = weight is None or weight.dtype == torch.float32
-    ws, nbytes = _workspace(int(lib.exb_group_norm_workspace_bytes(R, S, C, G, DTYPES[x.dtype], 0)), dev)
-    st = lib.exb_group_norm_forward(ptr(y), ptr(mean), ptr(rstd), rows_of(x), ptr(weight), ptr(bias), float(eps),
-                                    ACTIVATIONS[activation], int(f32), ptr(ws), nbytes, DTYPES[x.dtype], R, S, C, G, dev.index,
-                                    _stream(dev))
-    _check(st, "exb_group_norm_forward")
-    _after_launch(dev)
+    dtype, dev = DTYPES[x.dtype], x.get_device()
+    nbytes = _group_norm_workspace_bytes(R, S, C, G, dtype, 0)
+    ws = _workspace(nbytes, x)
+    st = load().exb_group_norm_forward(y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), rows_of(x), ptr(weight), ptr(bias), eps,
+                                       ACTIVATIONS[activation], _f32_params(weight, bias), ptr(ws), nbytes, dtype, R, S, C, G, dev,
+                                       _stream_of(dev))
+    _launched(st, "exb_group_norm_forward", x)
 
 
 def group_norm_backward(dx, dweight, dbias, dy, x, mean, rstd, weight, bias, activation, R: int, S: int, C: int, G: int) -> None:
-    lib, dev = load(), x.device
-    f32 = weight is None or weight.dtype == torch.float32
-    ws, nbytes = _workspace(int(lib.exb_group_norm_workspace_bytes(R, S, C, G, DTYPES[x.dtype], 1)), dev)
-    st = lib.exb_group_norm_backward(ptr(dx), ptr(dweight), ptr(dbias), rows_of(dy), rows_of(x), ptr(mean), ptr(rstd), ptr(weight),
-                                     ptr(bias), ACTIVATIONS[activation], int(f32), ptr(ws), nbytes, DTYPES[x.dtype], R, S, C, G,
-                                     dev.index, _stream(dev))
-    _check(st, "exb_group_norm_backward")
-    _after_launch(dev)
+    dtype, dev = DTYPES[x.dtype], x.get_device()
+    nbytes = _group_norm_workspace_bytes(R, S, C, G, dtype, 1)
+    ws = _workspace(nbytes, x)
+    st = load().exb_group_norm_backward(dx.data_ptr(), ptr(dweight), ptr(dbias), rows_of(dy), rows_of(x), mean.data_ptr(),
+                                        rstd.data_ptr(), ptr(weight), ptr(bias), ACTIVATIONS[activation], _f32_params(weight, bias),
+                                        ptr(ws), nbytes, dtype, R, S, C, G, dev, _stream_of(dev))
+    _launched(st, "exb_group_norm_backward", x)
 
 
 # Tracing aid: NVTX ranges around the calls that launch kernels, named after the entry point, so that a timeline

@@ -37,6 +37,14 @@ def require_like(name: str, t: Optional[torch.Tensor], shape: Tuple[int, ...], d
         raise _lib.ExodusLibraryError(f"tensors on different devices: {device} and {t.device} ('{name}')")
 
 
+def alike(t: Optional[torch.Tensor], shape, dtype: torch.dtype, device: int) -> bool:
+    """Whether ``t`` is absent or what it should be: the quick form of :func:`require_like`, which says what is wrong."""
+    return t is None or (type(t) in _TENSORS and t.shape == shape and t.dtype == dtype and t.get_device() == device)
+
+
+_TENSORS = (torch.Tensor, torch.nn.Parameter)
+
+
 def check_lengths(lengths: Optional[torch.Tensor], batch: int, device: torch.device) -> Optional[torch.Tensor]:
     if lengths is None:
         return None
@@ -49,21 +57,37 @@ def channels_contiguous(t: Optional[torch.Tensor], trailing: int = 1) -> Optiona
     if t is None:
         return None
     step = 1
-    for d in range(t.ndim - 1, t.ndim - 1 - trailing, -1):
-        if t.shape[d] > 1 and t.stride(d) != step:
+    shape, stride = t.shape, t.stride()
+    for d in range(len(shape) - 1, len(shape) - 1 - trailing, -1):
+        if shape[d] > 1 and stride[d] != step:
             return t.contiguous()
-        step *= t.shape[d]
+        step *= shape[d]
     return t
 
 
 def dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return None if t is None else t.contiguous()
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def wants_grad(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether autograd has to record a call on these tensors."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def refuse_grad(what: str, *tensors: Optional[torch.Tensor]) -> None:
     """The in-place single-token forms are not differentiable."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if wants_grad(*tensors):
         raise RuntimeError(f"{what} updates its state in place and is not differentiable: call it under torch.no_grad()")
+
+
+def refuse_second_order(what: str) -> None:
+    """Called in a backward pass, where autograd only records with ``create_graph=True``."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} is differentiable once: its backward pass cannot be recorded (create_graph=True)")
 
 
 def mark_changed(t: torch.Tensor) -> None:

@@ -10,11 +10,26 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib, _seq
 
 __all__ = ["CausalConvTM", "causal_conv", "causal_conv_step"]
+
+
+def _forward(x, weight, bias, state, lengths, activation):
+    """Launches the forward pass: (y, last), and the tensors as the kernels read them."""
+    nb, T, M = x.shape
+    W = weight.shape[1]
+    x = _seq.channels_contiguous(x)
+    weight, bias, state = _seq.dense(weight), _seq.dense(bias), _seq.dense(state)
+    y, last = x.new_empty((nb, T, M)), x.new_empty((nb, W - 1, M))
+    if nb * T * M:
+        _lib.causal_conv_forward(y, last, x, weight, bias, state, lengths, activation, nb, T, M, W)
+    elif state is not None:      # no rows: the state passes through unchanged
+        last.copy_(state)
+    else:
+        last.zero_()
+    return y, last, (x, weight, bias, state)
 
 
 class CausalConvTM(torch.autograd.Function):
@@ -23,38 +38,31 @@ class CausalConvTM(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, state, lengths, activation):
-        nb, T, M = x.shape
-        W = weight.shape[1]
-        x = _seq.channels_contiguous(x)
-        weight, bias, state = (_seq.dense(t) for t in (weight, bias, state))
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        y, last, used = _forward(x, weight, bias, state, lengths, activation)
         ctx.set_materialize_grads(False)
         ctx.activation = activation
-        ctx.save_for_backward(x, weight, bias, state, lengths)
-        if nb * T * M == 0:      # no rows: the state passes through unchanged
-            return y, state.clone() if state is not None else torch.zeros(nb, W - 1, M, dtype=x.dtype, device=x.device)
-        last = torch.empty(nb, W - 1, M, dtype=x.dtype, device=x.device)
-        _lib.causal_conv_forward(y, last, x, weight, bias, state, lengths, activation, nb, T, M, W)
+        ctx.save_for_backward(*used, lengths)
         return y, last
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dlast):
+        _seq.refuse_second_order("causal_conv")
         x, weight, bias, state, lengths = ctx.saved_tensors
         nb, T, M = x.shape
         W = weight.shape[1]
-        empty = nb * T * M == 0
-        new = torch.zeros_like if empty else torch.empty_like
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dweight = new(weight)
-        dbias = new(bias) if bias is not None else None
-        dstate = new(state) if state is not None else None
+        dx = x.new_empty((nb, T, M))
+        dweight = torch.empty_like(weight)
+        dbias = torch.empty_like(bias) if bias is not None else None
+        dstate = torch.empty_like(state) if state is not None else None
         dlast = _seq.dense(dlast)
-        if empty:
+        if nb * T * M == 0:
+            for t in (dweight, dbias, dstate):
+                if t is not None:
+                    t.zero_()
             if dstate is not None and dlast is not None:
                 dstate.copy_(dlast)
         else:
-            dy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if dy is None else _seq.channels_contiguous(dy)
+            dy = x.new_zeros((nb, T, M)) if dy is None else _seq.channels_contiguous(dy)
             _lib.causal_conv_backward(dx, dweight, dbias, dstate, dy, dlast, x, weight, bias, state, lengths, ctx.activation, nb, T, M, W)
         return dx, dweight, dbias, dstate, None, None
 
@@ -72,8 +80,10 @@ def _check(x, weight, bias, activation) -> int:
         raise ValueError(f"filters of 1 to {_lib.CONV_MAX_WIDTH} steps are supported, got {W}")
     if activation not in (None, "silu"):
         raise ValueError(f"'activation' must be None or 'silu', got {activation!r}")
-    _seq.require_like("weight", weight, (M, W), (torch.float32, x.dtype), x.device)
-    _seq.require_like("bias", bias, (M,), (weight.dtype,), x.device)
+    kind, dev = weight.dtype, x.get_device()
+    if dev < 0 or weight.get_device() != dev or (kind != torch.float32 and kind != x.dtype) or not _seq.alike(bias, (M,), kind, dev):
+        _seq.require_like("weight", weight, (M, W), (torch.float32, x.dtype), x.device)
+        _seq.require_like("bias", bias, (M,), (weight.dtype,), x.device)
     return W
 
 
@@ -98,9 +108,13 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     if isinstance(x, torch.Tensor) and x.ndim != 3:
         raise ValueError("'x' must be 3D, (batch, time, channels)")
     W = _check(x, weight, bias, activation)
-    _seq.require_like("state", state, (x.shape[0], W - 1, x.shape[2]), (x.dtype,), x.device)
-    lengths = _seq.check_lengths(lengths, x.shape[0], x.device)
+    if state is not None:
+        _seq.require_like("state", state, (x.shape[0], W - 1, x.shape[2]), (x.dtype,), x.device)
+    if lengths is not None:
+        lengths = _seq.check_lengths(lengths, x.shape[0], x.device)
     _seq.require_cuda("x", x)
+    if not _seq.wants_grad(x, weight, bias, state):
+        return _forward(x, weight, bias, state, lengths, activation)[:2]
     return CausalConvTM.apply(x, weight, bias, state, lengths, activation)
 
 
@@ -115,14 +129,15 @@ def causal_conv_step(state: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
         raise ValueError("'x' must be 2D, (batch, channels)")
     W = _check(x, weight, bias, activation)
     nb, M = x.shape
-    _seq.require_like("state", state, (nb, W - 1, M), (x.dtype,), x.device)
+    if not _seq.alike(state, (nb, W - 1, M), x.dtype, x.get_device()) or state is None:
+        _seq.require_like("state", state, (nb, W - 1, M), (x.dtype,), x.device)
     if nb * M and _seq.channels_contiguous(state, 2) is not state:
         raise ValueError("'state' must be contiguous in its rows and channels: it is updated in place")
     if nb > 1 and state.stride(0) < (W - 1) * M:
         raise ValueError("the batch items of 'state' overlap")
     _seq.require_cuda("x", x)
     _seq.refuse_grad("causal_conv_step", state, x, weight, bias)
-    y = torch.empty(nb, M, dtype=x.dtype, device=x.device)
+    y = x.new_empty((nb, M))
     if nb * M == 0:
         return y
     _lib.causal_conv_step(y, state, _seq.channels_contiguous(x), _seq.dense(weight), _seq.dense(bias), activation, nb, M, W)

@@ -29,10 +29,11 @@ int check_ptr(const char *who, const char *name, const void *p, int64_t es, bool
     return EXB_OK;
 }
 
-exb::View view(const exb_rows *r)
+// A dimension of size one has no stride (whatever the caller's says, it must not keep aligned rows from being seen as such).
+exb::View view(const exb_rows *r, int64_t B, int64_t T)
 {
     exb::View v;
-    if (r) { v.p = r->data; v.sb = r->stride_b; v.st = r->stride_t; }
+    if (r) { v.p = r->data; v.sb = B > 1 ? r->stride_b : 0; v.st = T > 1 ? r->stride_t : 0; }
     return v;
 }
 
@@ -113,7 +114,7 @@ int exb_selective_forward(void *y, float *h_last, float *ckpt, const exb_rows *x
     DeviceGuard guard(device);
     if (!guard.ok) return fail(EXB_ERR_DEVICE, "%s: cannot select device %d", who, device);
     exb::SelArgs a{};
-    a.x = view(x); a.dt = view(dt); a.z = view(z); a.Bm = view(Bm); a.Cm = view(Cm);
+    a.x = view(x, B, T); a.dt = view(dt, B, T); a.z = view(z, B, T); a.Bm = view(Bm, B, T); a.Cm = view(Cm, B, T);
     a.A = A; a.D = D; a.dt_bias = dt_bias; a.h0 = h0; a.lengths = lengths;
     a.B = B; a.T = T; a.M = (int)M; a.N = (int)N; a.G = (int)G; a.softplus = softplus;
     a.y = y; a.h_last = h_last; a.ckpt = ckpt;
@@ -161,7 +162,7 @@ int exb_selective_backward(void *dx, void *ddt, float *dA, void *dB, void *dC, f
     DeviceGuard guard(device);
     if (!guard.ok) return fail(EXB_ERR_DEVICE, "%s: cannot select device %d", who, device);
     exb::SelArgs a{};
-    a.x = view(x); a.dt = view(dt); a.z = view(z); a.Bm = view(Bm); a.Cm = view(Cm); a.dy = view(dy);
+    a.x = view(x, B, T); a.dt = view(dt, B, T); a.z = view(z, B, T); a.Bm = view(Bm, B, T); a.Cm = view(Cm, B, T); a.dy = view(dy, B, T);
     a.A = A; a.D = D; a.dt_bias = dt_bias; a.lengths = lengths; a.dh_last = dh_last;
     a.B = B; a.T = T; a.M = (int)M; a.N = (int)N; a.G = (int)G; a.softplus = softplus;
     a.ckpt = const_cast<float *>(ckpt);
@@ -194,7 +195,7 @@ int exb_selective_step(void *y, float *h, int64_t h_stride, const exb_rows *x, c
     DeviceGuard guard(device);
     if (!guard.ok) return fail(EXB_ERR_DEVICE, "%s: cannot select device %d", who, device);
     exb::SelStepArgs a{};
-    a.x = view(x); a.dt = view(dt); a.z = view(z); a.Bm = view(Bm); a.Cm = view(Cm);
+    a.x = view(x, B, 1); a.dt = view(dt, B, 1); a.z = view(z, B, 1); a.Bm = view(Bm, B, 1); a.Cm = view(Cm, B, 1);
     a.A = A; a.D = D; a.dt_bias = dt_bias; a.h = h; a.sh = h_stride; a.y = y;
     a.B = B; a.M = (int)M; a.N = (int)N; a.G = (int)G; a.softplus = softplus;
     return launched(who, exb::launch_selective_step(a, dtype, (cudaStream_t)stream));
@@ -240,7 +241,7 @@ int exb_causal_conv_forward(void *y, void *last, const exb_rows *x, const void *
     DeviceGuard guard(device);
     if (!guard.ok) return fail(EXB_ERR_DEVICE, "%s: cannot select device %d", who, device);
     exb::ConvArgs a{};
-    a.x = view(x); a.weight = weight; a.bias = bias; a.state = state; a.lengths = lengths; a.y = y; a.last = last;
+    a.x = view(x, B, T); a.weight = weight; a.bias = bias; a.state = state; a.lengths = lengths; a.y = y; a.last = last;
     a.B = B; a.T = T; a.M = (int)M; a.W = (int)W; a.silu = activation == EXB_ACT_SILU; a.params_f32 = params_f32 || dtype == EXB_F32;
     return launched(who, exb::launch_conv_forward(a, dtype, (cudaStream_t)stream));
 }
@@ -273,7 +274,7 @@ int exb_causal_conv_backward(void *dx, void *dweight, void *dbias, void *dstate,
     DeviceGuard guard(device);
     if (!guard.ok) return fail(EXB_ERR_DEVICE, "%s: cannot select device %d", who, device);
     exb::ConvArgs a{};
-    a.x = view(x); a.dy = view(dy); a.weight = weight; a.bias = bias; a.state = state; a.lengths = lengths; a.dlast = dlast;
+    a.x = view(x, B, T); a.dy = view(dy, B, T); a.weight = weight; a.bias = bias; a.state = state; a.lengths = lengths; a.dlast = dlast;
     a.dx = dx; a.dstate = dstate;
     a.B = B; a.T = T; a.M = (int)M; a.W = (int)W; a.silu = activation == EXB_ACT_SILU; a.params_f32 = params_f32 || dtype == EXB_F32;
     return launched(who, exb::launch_conv_backward(a, dtype, dweight, dbias, workspace, (cudaStream_t)stream));
@@ -296,7 +297,7 @@ int exb_causal_conv_step(void *y, void *state, int64_t state_stride, const exb_r
     DeviceGuard guard(device);
     if (!guard.ok) return fail(EXB_ERR_DEVICE, "%s: cannot select device %d", who, device);
     exb::ConvStepArgs a{};
-    a.x = view(x); a.weight = weight; a.bias = bias; a.state = state; a.ss = state_stride; a.y = y;
+    a.x = view(x, B, 1); a.weight = weight; a.bias = bias; a.state = state; a.ss = state_stride; a.y = y;
     a.B = B; a.M = (int)M; a.W = (int)W; a.silu = activation == EXB_ACT_SILU; a.params_f32 = params_f32 || dtype == EXB_F32;
     return launched(who, exb::launch_conv_step(a, dtype, (cudaStream_t)stream));
 }
@@ -345,7 +346,7 @@ int exb_group_norm_forward(void *y, float *mean, float *rstd, const exb_rows *x,
     DeviceGuard guard(device);
     if (!guard.ok) return fail(EXB_ERR_DEVICE, "%s: cannot select device %d", who, device);
     exb::NormArgs a{};
-    a.x = view(x); a.weight = weight; a.bias = bias; a.y = y; a.mean = mean; a.rstd = rstd;
+    a.x = view(x, R, S); a.weight = weight; a.bias = bias; a.y = y; a.mean = mean; a.rstd = rstd;
     a.R = R; a.S = S; a.C = (int)C; a.G = (int)G; a.act = activation; a.params_f32 = params_f32 || dtype == EXB_F32; a.eps = eps;
     return launched(who, exb::launch_norm_forward(a, dtype, workspace, (cudaStream_t)stream));
 }
@@ -375,7 +376,7 @@ int exb_group_norm_backward(void *dx, void *dweight, void *dbias, const exb_rows
     DeviceGuard guard(device);
     if (!guard.ok) return fail(EXB_ERR_DEVICE, "%s: cannot select device %d", who, device);
     exb::NormArgs a{};
-    a.x = view(x); a.dy = view(dy); a.weight = weight; a.bias = bias; a.dx = dx; a.mean = const_cast<float *>(mean); a.rstd = const_cast<float *>(rstd);
+    a.x = view(x, R, S); a.dy = view(dy, R, S); a.weight = weight; a.bias = bias; a.dx = dx; a.mean = const_cast<float *>(mean); a.rstd = const_cast<float *>(rstd);
     a.R = R; a.S = S; a.C = (int)C; a.G = (int)G; a.act = activation; a.params_f32 = params_f32 || dtype == EXB_F32;
     return launched(who, exb::launch_norm_backward(a, dtype, dweight, dbias, workspace, (cudaStream_t)stream));
 }

@@ -398,45 +398,85 @@ __device__ __forceinline__ float positions(const Spot &s, int ty)
     return (float)(each + (ty < n - each * s.rows ? 1 : 0));
 }
 
-// Calls f(pack of x, pack of dy, index) for the positions of a thread, AHEAD of them on their way.
-// peek(pack of x) sees the first of them before.
-struct Nothing {
-    template <typename R> __device__ __forceinline__ void operator()(const R &) const {}
-};
-template <typename T, int V, bool VEC, bool TWO, typename F, typename Peek = Nothing>
-__device__ __forceinline__ void walk(const NormArgs &a, const Spot &s, int p, const F &f, const Peek &peek = Peek())
-{
+// The positions of a thread, walked with AHEAD of them on their way.  Aligned rows come through a ring in shared memory that
+// only this thread writes (asynchronous copies) and reads, so that nothing but the copies themselves is waited for and no
+// registers are held; others are loaded into registers.
+constexpr int AHEAD = 8;
+template <typename T, int V, bool VEC, bool TWO>
+struct Walk {
     using R = RawPack<T, V, VEC>;
-    constexpr int AHEAD = TWO ? 2 : 4;
-    const int left = s.chans - p * V;
-    const T *x = static_cast<const T *>(a.x.p) + s.r * a.x.sb + s.c0 + p * V + (s.p0 + s.ty) * a.x.st;
-    const T *g = TWO ? static_cast<const T *>(a.dy.p) + s.r * a.dy.sb + s.c0 + p * V + (s.p0 + s.ty) * a.dy.st : nullptr;
-    const int64_t dx = s.rows * a.x.st, dg = TWO ? s.rows * a.dy.st : 0;
-    R px[AHEAD], pg[AHEAD];
-    auto fetch = [&](int i, bool there) {
-        px[i].load(x, there ? left : 0);
-        x += dx;
-        if (TWO) {
-            pg[i].load(g, there ? left : 0);
-            g += dg;
-        }
-    };
+    static constexpr int RING = VEC ? NT * AHEAD * 16 * (TWO ? 2 : 1) : 0;      // bytes
+    const T *x, *g;
+    int64_t step_x, step_g;
+    int left, count, issued = 0;
+    uint4 *ring;
+
+    __device__ __forceinline__ Walk(const NormArgs &a, const Spot &s, int p, uint4 *ring_) : ring(ring_ + threadIdx.x)
+    {
+        left = s.chans - p * V;
+        count = s.count;
+        x = static_cast<const T *>(a.x.p) + s.r * a.x.sb + s.c0 + p * V + (s.p0 + s.ty) * a.x.st;
+        g = TWO ? static_cast<const T *>(a.dy.p) + s.r * a.dy.sb + s.c0 + p * V + (s.p0 + s.ty) * a.dy.st : nullptr;
+        step_x = s.rows * a.x.st;
+        step_g = TWO ? s.rows * a.dy.st : 0;
+        if (VEC) {
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) fetch(i, i < s.count);
-    peek(px[0]);
-    int q = 0;
-    for (; q + AHEAD <= s.count; q += AHEAD) {
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            const R cx = px[i], cg = pg[i];
-            fetch(i, q + i + AHEAD < s.count);
-            f(cx, cg, q + i);
+            for (int i = 0; i < AHEAD; ++i) issue();
         }
     }
-#pragma unroll
-    for (int i = 0; i < AHEAD - 1; ++i)
-        if (q + i < s.count) f(px[i], pg[i], q + i);
-}
+    __device__ __forceinline__ void issue()
+    {
+        if (issued < count) {
+            uint4 *to = ring + (issued % AHEAD) * NT;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(x) : "memory");
+            if (TWO) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to + AHEAD * NT)), "l"(g) : "memory");
+            x += step_x;
+            g += step_g;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        ++issued;
+    }
+    __device__ __forceinline__ static void take(R &r, const uint4 *from)
+    {
+        if constexpr (VEC) {
+            const uint4 v = *from;
+            r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w;
+        }
+    }
+    // f(pack of x, pack of dy) for every position; peek(pack of x) sees the first of them before.
+    template <typename F, typename Peek>
+    __device__ __forceinline__ void run(const F &f, const Peek &peek)
+    {
+        R cx, cg;
+        if constexpr (VEC) {
+#pragma unroll 4
+            for (int q = 0; q < count; ++q) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
+                const uint4 *from = ring + (q % AHEAD) * NT;
+                take(cx, from);
+                if (TWO) take(cg, from + AHEAD * NT);
+                if (q == 0) peek(cx);
+                issue();
+                f(cx, cg);
+            }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+        } else {
+            for (int q = 0; q < count; ++q) {
+                cx.load(x, left);
+                if (TWO) cg.load(g, left);
+                if (q == 0) peek(cx);
+                f(cx, cg);
+                x += step_x;
+                g += step_g;
+            }
+        }
+    }
+    template <typename F>
+    __device__ __forceinline__ void run(const F &f)
+    {
+        run(f, [](const R &) {});
+    }
+};
 template <typename T, int V, bool VEC>
 __device__ __forceinline__ float2 pair_of(const RawPack<T, V, VEC> &r, int i)
 {
@@ -448,8 +488,9 @@ __device__ __forceinline__ float2 pair_of(const RawPack<T, V, VEC> &r, int i)
 // A thread takes the moments of its channels about their first value, so that a large common offset costs no digits; where
 // whole packs belong to one group, it joins those of a pack.
 template <typename T, int V, bool VEC, typename Out>
-__device__ __forceinline__ void block_moments(const NormArgs &a, const Spot &s, float2 *s_m, const Out &out)
+__device__ __forceinline__ void block_moments(const NormArgs &a, const Spot &s, float2 *s_m, uint4 *ring, const Out &out)
 {
+    using W = Walk<T, V, VEC, false>;
     constexpr int P = V > 1 ? V / 2 : 1;
     const bool whole = V > 1 && a.per % V == 0;
     const int entries = whole ? s.chans / V : s.chans;      // of a row in s_m
@@ -458,7 +499,7 @@ __device__ __forceinline__ void block_moments(const NormArgs &a, const Spot &s, 
         const int left = s.chans - p * V;
 #pragma unroll
         for (int i = 0; i < P; ++i) k[i] = sum[i] = sq[i] = both(0.0f);
-        walk<T, V, VEC, false>(a, s, p, [&](const RawPack<T, V, VEC> &x, const RawPack<T, V, VEC> &, int) {
+        W(a, s, p, ring).run([&](const RawPack<T, V, VEC> &x, const RawPack<T, V, VEC> &) {
 #pragma unroll
             for (int i = 0; i < P; ++i) {
                 const float2 d = add2(pair_of(x, i), k[i]);
@@ -525,13 +566,22 @@ struct GroupOf {
     }
 };
 
-// y from x with the groups' mean and rstd in s_m.
-template <typename T, int V, bool VEC>
-__device__ __forceinline__ void block_apply(const NormArgs &a, const Spot &s, const float2 *s_m)
+// y from x with the groups' mean and rstd in s_m.  ready() is called when the first positions are on their way: it waits
+// for what s_m holds.
+template <typename T, int V, bool VEC, typename Ready>
+__device__ __forceinline__ void block_apply(const NormArgs &a, const Spot &s, const float2 *s_m, uint4 *ring, const Ready &ready)
 {
     constexpr int P = V > 1 ? V / 2 : 1;
-    for (int p = s.px; p < s.packs; p += s.wide) {
-        const int left = s.chans - p * V;
+    const int passes = (s.chans + V * s.wide - 1) / (V * s.wide);      // the same for all threads: ready() may be a barrier
+    for (int k = 0; k < passes; ++k) {
+        const int p = s.px + k * s.wide;
+        const bool there = p < s.packs;
+        const int left = there ? s.chans - p * V : 0;
+        Spot mine = s;
+        if (!there) mine.count = 0;
+        Walk<T, V, VEC, false> walk(a, mine, there ? p : 0, ring);
+        if (k == 0) ready();
+        if (!there) continue;
         float2 mean[P], scale[P], shift[P];
         float wv[V], bv[V];
         load_params<T, V, VEC>(wv, a.weight, s.c0 + p * V, left, a.params_f32, 1.0f);
@@ -546,7 +596,7 @@ __device__ __forceinline__ void block_apply(const NormArgs &a, const Spot &s, co
         }
         T *out = static_cast<T *>(a.y) + (s.r * a.S + s.p0 + s.ty) * a.C + s.c0 + p * V;
         const int64_t step = (int64_t)s.rows * a.C;
-        walk<T, V, VEC, false>(a, s, p, [&](const RawPack<T, V, VEC> &x, const RawPack<T, V, VEC> &, int) {
+        walk.run([&](const RawPack<T, V, VEC> &x, const RawPack<T, V, VEC> &) {
             Pack<T, V> y;
             float2 v[P];
 #pragma unroll
@@ -604,18 +654,19 @@ struct Channels {
 };
 
 // Per channel, over the block's positions: the sums of d n and of d (d: gradient in front of the activation, n: normed x),
-// in s_c [2][channels] and in the block's row of a.part.  s_m: see map_smem.
+// left in s_m[channel] and in the block's row of a.part.  s_m: see map_smem.
 template <typename T, int V, bool VEC>
-__device__ __forceinline__ void block_gradient_sums(const NormArgs &a, const Spot &s, float2 *s_m, float2 *s_c)
+__device__ __forceinline__ void block_gradient_sums(const NormArgs &a, const Spot &s, float2 *s_m, uint4 *ring)
 {
     constexpr int P = V > 1 ? V / 2 : 1;
     for (int p = s.px; p < s.packs; p += s.wide) {
         const int left = s.chans - p * V;
+        Walk<T, V, VEC, true> walk(a, s, p, ring);
         const Channels<T, V, VEC> h(a, s, p);
         float2 s1[P], s2[P];
 #pragma unroll
         for (int i = 0; i < P; ++i) s1[i] = s2[i] = both(0.0f);
-        walk<T, V, VEC, true>(a, s, p, [&](const RawPack<T, V, VEC> &x, const RawPack<T, V, VEC> &g, int) {
+        walk.run([&](const RawPack<T, V, VEC> &x, const RawPack<T, V, VEC> &g) {
             float2 n[P], d[P];
             h.get(n, d, x, g, a.act);
 #pragma unroll
@@ -638,7 +689,7 @@ __device__ __forceinline__ void block_gradient_sums(const NormArgs &a, const Spo
         for (int k = 0; k < s.rows; ++k) t = add2(t, s_m[k * s.chans + c]);
         out[c] = t.y;
         out[a.C + c] = t.x;
-        s_c[c] = t;
+        s_m[c] = t;      // of this column only this thread has read
     }
     __syncthreads();
 }
@@ -659,13 +710,21 @@ __device__ __forceinline__ void group_sums(const NormArgs &a, const Spot &s, con
     }
 }
 
-// dx with the groups' two sums over their number of values in s_g.
-template <typename T, int V, bool VEC>
-__device__ __forceinline__ void block_gradient(const NormArgs &a, const Spot &s, const float2 *s_g)
+// dx with the groups' two sums over their number of values in s_g; ready() as above.
+template <typename T, int V, bool VEC, typename Ready>
+__device__ __forceinline__ void block_gradient(const NormArgs &a, const Spot &s, const float2 *s_g, uint4 *ring, const Ready &ready)
 {
     constexpr int P = V > 1 ? V / 2 : 1;
-    for (int p = s.px; p < s.packs; p += s.wide) {
-        const int left = s.chans - p * V;
+    const int passes = (s.chans + V * s.wide - 1) / (V * s.wide);
+    for (int k = 0; k < passes; ++k) {
+        const int p = s.px + k * s.wide;
+        const bool there = p < s.packs;
+        const int left = there ? s.chans - p * V : 0;
+        Spot mine = s;
+        if (!there) mine.count = 0;
+        Walk<T, V, VEC, true> walk(a, mine, there ? p : 0, ring);
+        if (k == 0) ready();
+        if (!there) continue;
         const Channels<T, V, VEC> h(a, s, p);
         float2 u[P], v[P];
         GroupOf group(p * V, a.per);
@@ -677,7 +736,7 @@ __device__ __forceinline__ void block_gradient(const NormArgs &a, const Spot &s,
         }
         T *out = static_cast<T *>(a.dx) + (s.r * a.S + s.p0 + s.ty) * a.C + s.c0 + p * V;
         const int64_t step = (int64_t)s.rows * a.C;
-        walk<T, V, VEC, true>(a, s, p, [&](const RawPack<T, V, VEC> &x, const RawPack<T, V, VEC> &g, int) {
+        walk.run([&](const RawPack<T, V, VEC> &x, const RawPack<T, V, VEC> &g) {
             Pack<T, V> o;
             float2 n[P], d[P];
             h.get(n, d, x, g, a.act);
@@ -706,43 +765,48 @@ __device__ __forceinline__ void finish_group(const NormArgs &a, const Spot &s, f
 
 // ---- one cluster per sample (and slab of groups): a.chunks blocks, which is the cluster's size
 
+// Dynamic shared memory of the map kernels: the rings, then a.smem pairs (see map_smem), then what each says.
 template <typename T, int V, bool VEC>
 __global__ void __launch_bounds__(NT, 3) norm_cluster_forward_kernel(const NormArgs a)
 {
-    extern __shared__ float2 s_m[];      // map_smem; behind it [groups] moments of the block
+    extern __shared__ uint4 ring[];
     namespace cg = cooperative_groups;
     const cg::cluster_group cluster = cg::this_cluster();
     const Spot s = place<V>(a);
-    Moments *own = reinterpret_cast<Moments *>(s_m + a.smem);
-    block_moments<T, V, VEC>(a, s, s_m, [&](int g, const Moments &m) { own[g] = m; });
-    cluster.sync();
-    for (int g = threadIdx.x / 32; g < s.groups; g += NT / 32) {
-        const Moments m = join(a.chunks, [&](int r) { return cluster.map_shared_rank(own, r)[g]; });
-        if (threadIdx.x % 32 == 0) finish_group(a, s, s_m, g, m, s.chunk == 0);
-    }
-    cluster.sync();      // nobody reads another block's moments any more; s_m is written
-    block_apply<T, V, VEC>(a, s, s_m);
+    float2 *s_m = reinterpret_cast<float2 *>(reinterpret_cast<char *>(ring) + Walk<T, V, VEC, false>::RING);
+    Moments *own = reinterpret_cast<Moments *>(s_m + a.smem);      // [groups]
+    block_moments<T, V, VEC>(a, s, s_m, ring, [&](int g, const Moments &m) { own[g] = m; });
+    block_apply<T, V, VEC>(a, s, s_m, ring, [&]() {
+        cluster.sync();
+        for (int g = threadIdx.x / 32; g < s.groups; g += NT / 32) {
+            const Moments m = join(a.chunks, [&](int r) { return cluster.map_shared_rank(own, r)[g]; });
+            if (threadIdx.x % 32 == 0) finish_group(a, s, s_m, g, m, s.chunk == 0);
+        }
+        cluster.sync();      // nobody reads another block's moments any more; s_m is written
+    });
 }
 
 template <typename T, int V, bool VEC>
-__global__ void __launch_bounds__(NT, 3) norm_cluster_backward_kernel(const NormArgs a)
+__global__ void __launch_bounds__(NT, 2) norm_cluster_backward_kernel(const NormArgs a)
 {
-    extern __shared__ float2 s_m[];      // map_smem; [channels] sums; [groups] sums of the block
+    extern __shared__ uint4 ring[];
     namespace cg = cooperative_groups;
     const cg::cluster_group cluster = cg::this_cluster();
     const Spot s = place<V>(a);
-    float2 *s_c = s_m + a.smem, *own = s_c + a.slab * a.per;
-    block_gradient_sums<T, V, VEC>(a, s, s_m, s_c);
-    group_sums<T>(a, s, [&](int c) { return s_c[c]; }, [&](int g, float2 t) { own[g] = t; });
-    cluster.sync();
-    const float inv = 1.0f / ((float)a.S * (float)a.per);
-    for (int g = threadIdx.x; g < s.groups; g += NT) {
-        float2 t = both(0.0f);
-        for (int r = 0; r < a.chunks; ++r) t = add2(t, cluster.map_shared_rank(own, r)[g]);
-        s_m[g] = mul2(t, both(inv));
-    }
-    cluster.sync();
-    block_gradient<T, V, VEC>(a, s, s_m);
+    float2 *s_m = reinterpret_cast<float2 *>(reinterpret_cast<char *>(ring) + Walk<T, V, VEC, true>::RING);
+    float2 *own = s_m + a.smem;      // [groups] sums of the block
+    block_gradient_sums<T, V, VEC>(a, s, s_m, ring);
+    block_gradient<T, V, VEC>(a, s, s_m, ring, [&]() {
+        group_sums<T>(a, s, [&](int c) { return s_m[c]; }, [&](int g, float2 t) { own[g] = t; });
+        cluster.sync();
+        const float inv = 1.0f / ((float)a.S * (float)a.per);
+        for (int g = threadIdx.x; g < s.groups; g += NT) {
+            float2 t = both(0.0f);
+            for (int r = 0; r < a.chunks; ++r) t = add2(t, cluster.map_shared_rank(own, r)[g]);
+            s_m[g] = mul2(t, both(inv));
+        }
+        cluster.sync();
+    });
 }
 
 // ---- two kernels
@@ -750,9 +814,10 @@ __global__ void __launch_bounds__(NT, 3) norm_cluster_backward_kernel(const Norm
 template <typename T, int V, bool VEC>
 __global__ void __launch_bounds__(NT, 3) norm_stats_kernel(const NormArgs a)
 {
-    extern __shared__ float2 s_m[];
+    extern __shared__ uint4 ring[];
+    float2 *s_m = reinterpret_cast<float2 *>(reinterpret_cast<char *>(ring) + Walk<T, V, VEC, false>::RING);
     const Spot s = place<V>(a);
-    block_moments<T, V, VEC>(a, s, s_m, [&](int g, const Moments &m) {
+    block_moments<T, V, VEC>(a, s, s_m, ring, [&](int g, const Moments &m) {
         float *out = a.part + ((s.r * a.chunks + s.chunk) * a.G + s.g0 + g) * 2;
         out[0] = m.mean;
         out[1] = m.m2;
@@ -762,45 +827,50 @@ __global__ void __launch_bounds__(NT, 3) norm_stats_kernel(const NormArgs a)
 template <typename T, int V, bool VEC>
 __global__ void __launch_bounds__(NT, 3) norm_apply_kernel(const NormArgs a)
 {
-    extern __shared__ float2 s_m[];      // [groups]
+    extern __shared__ uint4 ring[];
+    float2 *s_m = reinterpret_cast<float2 *>(reinterpret_cast<char *>(ring) + Walk<T, V, VEC, false>::RING);      // [groups]
     const Spot s = place<V>(a);
-    for (int g = threadIdx.x / 32; g < s.groups; g += NT / 32) {
-        const Moments m = join(a.chunks, [&](int i) {
-            const int64_t lo = i * a.chunk, hi = lo + a.chunk < a.S ? lo + a.chunk : a.S;
-            const float *in = a.part + ((s.r * a.chunks + i) * a.G + s.g0 + g) * 2;
-            return Moments{(float)((hi - lo) * a.per), in[0], in[1]};
-        });
-        if (threadIdx.x % 32 == 0) finish_group(a, s, s_m, g, m, s.chunk == 0);
-    }
-    __syncthreads();
-    block_apply<T, V, VEC>(a, s, s_m);
-}
-
-template <typename T, int V, bool VEC>
-__global__ void __launch_bounds__(NT, 3) norm_backward_sums_kernel(const NormArgs a)
-{
-    extern __shared__ float2 s_m[];
-    const Spot s = place<V>(a);
-    block_gradient_sums<T, V, VEC>(a, s, s_m, s_m + a.smem);
-}
-
-template <typename T, int V, bool VEC>
-__global__ void __launch_bounds__(NT, 3) norm_backward_apply_kernel(const NormArgs a)
-{
-    extern __shared__ float2 s_m[];      // [groups]
-    const Spot s = place<V>(a);
-    const float inv = 1.0f / ((float)a.S * (float)a.per);
-    group_sums<T>(a, s, [&](int c) {
-        float2 t = both(0.0f);
-#pragma unroll 4
-        for (int k = 0; k < a.chunks; ++k) {
-            const float *in = a.part + (s.r * a.chunks + k) * 2 * a.C + s.c0 + c;
-            t = add2(t, make_float2(in[a.C], in[0]));
+    block_apply<T, V, VEC>(a, s, s_m, ring, [&]() {
+        for (int g = threadIdx.x / 32; g < s.groups; g += NT / 32) {
+            const Moments m = join(a.chunks, [&](int i) {
+                const int64_t lo = i * a.chunk, hi = lo + a.chunk < a.S ? lo + a.chunk : a.S;
+                const float *in = a.part + ((s.r * a.chunks + i) * a.G + s.g0 + g) * 2;
+                return Moments{(float)((hi - lo) * a.per), in[0], in[1]};
+            });
+            if (threadIdx.x % 32 == 0) finish_group(a, s, s_m, g, m, s.chunk == 0);
         }
-        return t;
-    }, [&](int g, float2 t) { s_m[g] = mul2(t, both(inv)); });
-    __syncthreads();
-    block_gradient<T, V, VEC>(a, s, s_m);
+        __syncthreads();
+    });
+}
+
+template <typename T, int V, bool VEC>
+__global__ void __launch_bounds__(NT, 2) norm_backward_sums_kernel(const NormArgs a)
+{
+    extern __shared__ uint4 ring[];
+    float2 *s_m = reinterpret_cast<float2 *>(reinterpret_cast<char *>(ring) + Walk<T, V, VEC, true>::RING);
+    const Spot s = place<V>(a);
+    block_gradient_sums<T, V, VEC>(a, s, s_m, ring);
+}
+
+template <typename T, int V, bool VEC>
+__global__ void __launch_bounds__(NT, 2) norm_backward_apply_kernel(const NormArgs a)
+{
+    extern __shared__ uint4 ring[];
+    float2 *s_m = reinterpret_cast<float2 *>(reinterpret_cast<char *>(ring) + Walk<T, V, VEC, true>::RING);      // [groups]
+    const Spot s = place<V>(a);
+    block_gradient<T, V, VEC>(a, s, s_m, ring, [&]() {
+        const float inv = 1.0f / ((float)a.S * (float)a.per);
+        group_sums<T>(a, s, [&](int c) {
+            float2 t = both(0.0f);
+#pragma unroll 4
+            for (int k = 0; k < a.chunks; ++k) {
+                const float *in = a.part + (s.r * a.chunks + k) * 2 * a.C + s.c0 + c;
+                t = add2(t, make_float2(in[a.C], in[0]));
+            }
+            return t;
+        }, [&](int g, float2 t) { s_m[g] = mul2(t, both(inv)); });
+        __syncthreads();
+    });
 }
 
 // ---------------------------------------------------------------------------------------------- launchers
@@ -943,7 +1013,7 @@ struct TokenBackward {
     }
 };
 
-// Pairs of shared memory in front of what a map kernel keeps besides: one per thread row and channel (one per group at least).
+// Pairs of shared memory that a map kernel works in: one per thread row and channel (one per group at least).
 template <int V>
 int map_smem(const NormArgs &a)
 {
@@ -980,28 +1050,31 @@ cudaError_t launch_clusters(K kernel, const NormArgs &a, unsigned grid, int smem
 template <typename T, int V, bool VEC>
 cudaError_t maps_forward(NormArgs a, bool cluster, cudaStream_t s)
 {
+    constexpr int RING = Walk<T, V, VEC, false>::RING;
     const unsigned grid = (unsigned)(a.R * a.chunks * a.slabs);
     a.smem = map_smem<V>(a);
-    int smem = a.smem * (int)sizeof(float2);
+    const int smem = RING + a.smem * (int)sizeof(float2), apply = RING + a.slab * (int)sizeof(float2);
     if (cluster) return launch_clusters(norm_cluster_forward_kernel<T, V, VEC>, a, grid, smem + a.slab * (int)sizeof(Moments), s);
     cudaError_t e = allow_smem(norm_stats_kernel<T, V, VEC>, smem);
+    if (e == cudaSuccess) e = allow_smem(norm_apply_kernel<T, V, VEC>, apply);
     if (e != cudaSuccess) return e;
     norm_stats_kernel<T, V, VEC><<<grid, NT, smem, s>>>(a);
-    norm_apply_kernel<T, V, VEC><<<grid, NT, a.slab * sizeof(float2), s>>>(a);
+    norm_apply_kernel<T, V, VEC><<<grid, NT, apply, s>>>(a);
     return cudaGetLastError();
 }
 template <typename T, int V, bool VEC>
 cudaError_t maps_backward(NormArgs a, bool cluster, cudaStream_t s)
 {
+    constexpr int RING = Walk<T, V, VEC, true>::RING;
     const unsigned grid = (unsigned)(a.R * a.chunks * a.slabs);
     a.smem = map_smem<V>(a);
-    const int chans = a.slab * (a.C / a.G);
-    const int smem = (a.smem + chans) * (int)sizeof(float2);
+    const int smem = RING + a.smem * (int)sizeof(float2), apply = RING + a.slab * (int)sizeof(float2);
     if (cluster) return launch_clusters(norm_cluster_backward_kernel<T, V, VEC>, a, grid, smem + a.slab * (int)sizeof(float2), s);
     cudaError_t e = allow_smem(norm_backward_sums_kernel<T, V, VEC>, smem);
+    if (e == cudaSuccess) e = allow_smem(norm_backward_apply_kernel<T, V, VEC>, apply);
     if (e != cudaSuccess) return e;
     norm_backward_sums_kernel<T, V, VEC><<<grid, NT, smem, s>>>(a);
-    norm_backward_apply_kernel<T, V, VEC><<<grid, NT, a.slab * sizeof(float2), s>>>(a);
+    norm_backward_apply_kernel<T, V, VEC><<<grid, NT, apply, s>>>(a);
     return cudaGetLastError();
 }
 

@@ -10,11 +10,21 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib, _seq
 
 __all__ = ["GroupNormCL", "group_norm"]
+
+
+def _forward(x, num_groups, weight, bias, eps, activation):
+    """Launches the forward pass: y, and what the backward pass reads."""
+    R, S, C = x.shape
+    x, weight, bias = _seq.channels_contiguous(x), _seq.dense(weight), _seq.dense(bias)
+    y = x.new_empty((R, S, C))
+    mean, rstd = (torch.empty((R, num_groups), dtype=torch.float32, device=x.device) for _ in range(2))
+    if R * S * C:
+        _lib.group_norm_forward(y, mean, rstd, x, weight, bias, eps, activation, R, S, C, num_groups)
+    return y, (x, weight, bias, mean, rstd)
 
 
 class GroupNormCL(torch.autograd.Function):
@@ -23,31 +33,26 @@ class GroupNormCL(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, num_groups, weight, bias, eps, activation):
-        R, S, C = x.shape
-        x = _seq.channels_contiguous(x)
-        weight, bias = _seq.dense(weight), _seq.dense(bias)
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        mean = torch.empty(R, num_groups, dtype=torch.float32, device=x.device)
-        rstd = torch.empty_like(mean)
-        if R * S * C:
-            _lib.group_norm_forward(y, mean, rstd, x, weight, bias, eps, activation, R, S, C, num_groups)
+        y, used = _forward(x, num_groups, weight, bias, eps, activation)
         ctx.num_groups, ctx.activation = num_groups, activation
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        ctx.save_for_backward(*used)
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        _seq.refuse_second_order("group_norm")
         x, weight, bias, mean, rstd = ctx.saved_tensors
         R, S, C = x.shape
-        empty = R * S * C == 0
-        new = torch.zeros_like if empty else torch.empty_like
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dweight = new(weight) if weight is not None else None
-        dbias = new(bias) if bias is not None else None
-        if not empty:
+        dx = x.new_empty((R, S, C))
+        dweight = torch.empty_like(weight) if weight is not None else None
+        dbias = torch.empty_like(bias) if bias is not None else None
+        if R * S * C:
             _lib.group_norm_backward(dx, dweight, dbias, _seq.channels_contiguous(dy), x, mean, rstd, weight, bias, ctx.activation, R, S,
                                      C, ctx.num_groups)
+        else:
+            for t in (dweight, dbias):
+                if t is not None:
+                    t.zero_()
         return dx, None, dweight, dbias, None, None
 
 
@@ -85,5 +90,9 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
     positions = 1
     for n in x.shape[1:-1]:
         positions *= n
-    y = GroupNormCL.apply(x.reshape(x.shape[0], positions, C), num_groups, weight, bias, float(eps), activation)
-    return y.reshape(x.shape)
+    flat = x if x.ndim == 3 else x.reshape(x.shape[0], positions, C)
+    if _seq.wants_grad(x, weight, bias):
+        y = GroupNormCL.apply(flat, num_groups, weight, bias, float(eps), activation)
+    else:
+        y = _forward(flat, num_groups, weight, bias, float(eps), activation)[0]
+    return y if x.ndim == 3 else y.reshape(x.shape)

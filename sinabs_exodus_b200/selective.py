@@ -16,11 +16,31 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib, _seq
 
 __all__ = ["SelectiveScanTM", "selective_scan", "selective_step"]
+
+
+def _forward(x, dt, A, B, C, D, z, dt_bias, h0, lengths, dt_softplus, keep):
+    """Launches the forward pass: (y, h_last, checkpoints or None), and the tensors as the kernels read them."""
+    nb, T, M = x.shape
+    G, N = B.shape[2:]
+    x, dt, z = _seq.channels_contiguous(x), _seq.channels_contiguous(dt), _seq.channels_contiguous(z)
+    B, C = _seq.channels_contiguous(B, 2), _seq.channels_contiguous(C, 2)
+    A, D, dt_bias, h0 = _seq.dense(A), _seq.dense(D), _seq.dense(dt_bias), _seq.dense(h0)
+    y = x.new_empty((nb, T, M))
+    h_last = A.new_empty((nb, M, N))
+    ckpt = None
+    if nb * T * M:
+        if keep:
+            ckpt = _lib.selective_checkpoint(nb, T, M, N, x)
+        _lib.selective_forward(y, h_last, ckpt, x, dt, A, B, C, D, z, dt_bias, h0, lengths, dt_softplus, nb, T, M, N, G)
+    elif h0 is not None:      # nothing to integrate: the state passes through unchanged
+        h_last.copy_(h0)
+    else:
+        h_last.zero_()
+    return y, h_last, ckpt, (x, dt, A, B, C, D, z, dt_bias)
 
 
 class SelectiveScanTM(torch.autograd.Function):
@@ -29,47 +49,35 @@ class SelectiveScanTM(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, dt, A, B, C, D, z, dt_bias, h0, lengths, dt_softplus):
-        nb, T, M = x.shape
-        G, N = B.shape[2], B.shape[3]
-        x, dt, z = (_seq.channels_contiguous(t) for t in (x, dt, z))
-        B, C = (_seq.channels_contiguous(t, 2) for t in (B, C))
-        A, D, dt_bias, h0 = (_seq.dense(t) for t in (A, D, dt_bias, h0))
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        y, h_last, ckpt, used = _forward(x, dt, A, B, C, D, z, dt_bias, h0, lengths, dt_softplus, True)
         ctx.set_materialize_grads(False)
-        ctx.sizes = (nb, T, M, N, G)
         ctx.softplus = dt_softplus
         ctx.had_h0 = h0 is not None
-        if nb * T * M == 0:      # nothing to integrate: the state passes through unchanged
-            h_last = h0.clone() if h0 is not None else torch.zeros(nb, M, N, dtype=torch.float32, device=x.device)
-            ctx.save_for_backward(x, dt, A, B, C, D, z, dt_bias, lengths, None)
-            return y, h_last
-        h_last = torch.empty(nb, M, N, dtype=torch.float32, device=x.device)
-        ckpt = _lib.selective_checkpoint(nb, T, M, N, x.device) if any(ctx.needs_input_grad) else None
-        _lib.selective_forward(y, h_last, ckpt, x, dt, A, B, C, D, z, dt_bias, h0, lengths, dt_softplus, nb, T, M, N, G)
-        ctx.save_for_backward(x, dt, A, B, C, D, z, dt_bias, lengths, ckpt)
+        ctx.save_for_backward(*used, lengths, ckpt)
         return y, h_last
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dh_last):
+        _seq.refuse_second_order("selective_scan")
         x, dt, A, B, C, D, z, dt_bias, lengths, ckpt = ctx.saved_tensors
-        nb, T, M, N, G = ctx.sizes
-        dev = x.device
-        new = torch.zeros if ckpt is None else torch.empty
-        f32 = dict(dtype=torch.float32, device=dev)
-        dx, ddt = (new(nb, T, M, dtype=x.dtype, device=dev) for _ in range(2))
-        dz = new(nb, T, M, dtype=x.dtype, device=dev) if z is not None else None
-        dB, dC = (new(nb, T, G, N, dtype=x.dtype, device=dev) for _ in range(2))
-        dA = new(M, N, **f32)
-        dD = new(M, **f32) if D is not None else None
-        ddt_bias = new(M, **f32) if dt_bias is not None else None
-        dh0 = new(nb, M, N, **f32) if ctx.had_h0 else None
+        nb, T, M = x.shape
+        G, N = B.shape[2:]
+        dx, ddt = x.new_empty((nb, T, M)), x.new_empty((nb, T, M))
+        dz = x.new_empty((nb, T, M)) if z is not None else None
+        dB, dC = x.new_empty((nb, T, G, N)), x.new_empty((nb, T, G, N))
+        dA = A.new_empty((M, N))
+        dD = A.new_empty((M,)) if D is not None else None
+        ddt_bias = A.new_empty((M,)) if dt_bias is not None else None
+        dh0 = A.new_empty((nb, M, N)) if ctx.had_h0 else None
         dh_last = _seq.dense(dh_last)
-        if ckpt is None:
+        if ckpt is None:      # an empty problem
+            for t in (dx, ddt, dz, dB, dC, dA, dD, ddt_bias, dh0):
+                if t is not None:
+                    t.zero_()
             if dh0 is not None and dh_last is not None:
                 dh0.copy_(dh_last)
         else:
-            dy = torch.zeros(nb, T, M, dtype=x.dtype, device=dev) if dy is None else _seq.channels_contiguous(dy)
+            dy = x.new_zeros((nb, T, M)) if dy is None else _seq.channels_contiguous(dy)
             _lib.selective_backward(dx, ddt, dA, dB, dC, dD, dz, ddt_bias, dh0, dy, dh_last, ckpt, x, dt, A, B, C, D, z, dt_bias,
                                     lengths, ctx.softplus, nb, T, M, N, G)
         return dx, ddt, dA, dB, dC, dD, dz, ddt_bias, dh0, None, None
@@ -81,7 +89,7 @@ def _grouped(name: str, t: torch.Tensor, lead: Tuple[int, ...]) -> torch.Tensor:
         raise TypeError(f"'{name}' must be a tensor, got {type(t).__name__}")
     if t.ndim == len(lead) + 1:
         t = t.unsqueeze(-2)
-    if t.ndim != len(lead) + 2 or tuple(t.shape[:-2]) != lead:
+    if t.ndim != len(lead) + 2 or t.shape[:-2] != lead:
         raise ValueError(f"'{name}' must have shape {lead + ('states',)} or {lead + ('groups', 'states')}, got {tuple(t.shape)}")
     return t
 
@@ -96,7 +104,12 @@ def _check(x, dt, A, B, C, D, z, dt_bias):
         raise ValueError(f"1 to {_lib.SELECTIVE_MAX_STATES} states per channel are supported, got {N}")
     if G < 1 or M % G:
         raise ValueError(f"the {G} groups of 'B' must divide the {M} channels")
-    same, f32 = (x.dtype,), (torch.float32,)
+    kind, dev, f = x.dtype, x.get_device(), torch.float32
+    if (_seq.alike(dt, x.shape, kind, dev) and _seq.alike(z, x.shape, kind, dev) and _seq.alike(B, lead + (G, N), kind, dev)
+            and _seq.alike(C, lead + (G, N), kind, dev) and _seq.alike(A, (M, N), f, dev) and _seq.alike(D, (M,), f, dev)
+            and _seq.alike(dt_bias, (M,), f, dev) and dev >= 0):
+        return B, C
+    same, f32 = (kind,), (f,)
     _seq.require_like("dt", dt, x.shape, same, x.device)
     _seq.require_like("z", z, x.shape, same, x.device)
     _seq.require_like("B", B, lead + (G, N), same, x.device)
@@ -133,10 +146,14 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     if isinstance(x, torch.Tensor) and x.ndim != 3:
         raise ValueError("'x' must be 3D, (batch, time, channels)")
     B, C = _check(x, dt, A, B, C, D, z, dt_bias)
-    _seq.require_like("h0", h0, (x.shape[0], x.shape[2], B.shape[3]), (torch.float32,), x.device)
-    lengths = _seq.check_lengths(lengths, x.shape[0], x.device)
+    if h0 is not None:
+        _seq.require_like("h0", h0, (x.shape[0], x.shape[2], B.shape[3]), (torch.float32,), x.device)
+    if lengths is not None:
+        lengths = _seq.check_lengths(lengths, x.shape[0], x.device)
     _seq.require_cuda("x", x)
-    return SelectiveScanTM.apply(x, dt, A, B, C, D, z, dt_bias, h0, lengths, bool(dt_softplus))
+    if _seq.wants_grad(x, dt, A, B, C, D, z, dt_bias, h0):
+        return SelectiveScanTM.apply(x, dt, A, B, C, D, z, dt_bias, h0, lengths, bool(dt_softplus))
+    return _forward(x, dt, A, B, C, D, z, dt_bias, h0, lengths, bool(dt_softplus), False)[:2]
 
 
 def selective_step(h: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
@@ -152,14 +169,15 @@ def selective_step(h: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, A: torch.
     B, C = _check(x, dt, A, B, C, D, z, dt_bias)
     nb, M = x.shape
     G, N = B.shape[1], B.shape[2]
-    _seq.require_like("h", h, (nb, M, N), (torch.float32,), x.device)
+    if not _seq.alike(h, (nb, M, N), torch.float32, x.get_device()) or h is None:
+        _seq.require_like("h", h, (nb, M, N), (torch.float32,), x.device)
     if nb * M and _seq.channels_contiguous(h, 2) is not h:
         raise ValueError("'h' must be contiguous in its channels and states: it is updated in place")
     if nb > 1 and h.stride(0) < M * N:
         raise ValueError("the batch items of 'h' overlap")
     _seq.require_cuda("x", x)
     _seq.refuse_grad("selective_step", h, x, dt, A, B, C, D, z, dt_bias)
-    y = torch.empty(nb, M, dtype=x.dtype, device=x.device)
+    y = x.new_empty((nb, M))
     if nb * M == 0:
         return y
     _lib.selective_step(y, h, _seq.channels_contiguous(x), _seq.channels_contiguous(dt), _seq.dense(A), _seq.channels_contiguous(B, 2),
