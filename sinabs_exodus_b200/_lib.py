@@ -579,12 +579,24 @@ CONV_MAX_WIDTH = 8
 NORM_MAX_GROUP = 16384
 
 
-def rows_of(t: Optional[torch.Tensor]):
-    """View of a (B, T, ...) or (B, ...) tensor whose trailing dimensions are contiguous; None passes through."""
+def rows_of(t: Optional[torch.Tensor], trailing: int = 1):
+    """View of a (B, T, ...) or (B, ...) tensor whose ``trailing`` last dimensions are contiguous, of a copy where they are
+    not (which the view keeps alive); None passes through."""
     if t is None:
         return None
     s = t.stride()
-    return Rows(t.data_ptr(), s[0], s[1] if len(s) > 2 else 0)
+    if s[-1] == 1 and (trailing == 1 or s[-2] == t.shape[-1]):
+        return Rows(t.data_ptr(), s[0], s[1] if len(s) > trailing + 1 else 0)
+    step = 1
+    for d in range(len(s) - 1, len(s) - 1 - trailing, -1):
+        if t.shape[d] > 1 and s[d] != step:
+            t = t.contiguous()
+            s = t.stride()
+            break
+        step *= t.shape[d]
+    r = Rows(t.data_ptr(), s[0], s[1] if len(s) > trailing + 1 else 0)
+    r.keep = t
+    return r
 
 
 # Sizes of the operators' scratch and checkpoint memory depend on the shape alone.
@@ -627,8 +639,8 @@ def selective_forward(y, h_last, ckpt, x, dt, A, Bm, Cm, D, z, dt_bias, h0, leng
                       N: int, G: int) -> None:
     nbytes, dev = _selective_workspace_bytes(B, T, M, N, G, 0), x.get_device()
     ws = _workspace(nbytes, x)
-    st = load().exb_selective_forward(y.data_ptr(), h_last.data_ptr(), ptr(ckpt), rows_of(x), rows_of(dt), A.data_ptr(), rows_of(Bm),
-                                      rows_of(Cm), ptr(D), rows_of(z), ptr(dt_bias), ptr(h0), ptr(lengths), softplus, ptr(ws), nbytes,
+    st = load().exb_selective_forward(y.data_ptr(), h_last.data_ptr(), ptr(ckpt), rows_of(x), rows_of(dt), A.data_ptr(), rows_of(Bm, 2),
+                                      rows_of(Cm, 2), ptr(D), rows_of(z), ptr(dt_bias), ptr(h0), ptr(lengths), softplus, ptr(ws), nbytes,
                                       DTYPES[x.dtype], B, T, M, N, G, dev, _stream_of(dev))
     _launched(st, "exb_selective_forward", x)
 
@@ -639,15 +651,15 @@ def selective_backward(dx, ddt, dA, dB, dC, dD, dz, ddt_bias, dh0, dy, dh_last, 
     ws = _workspace(nbytes, x)
     st = load().exb_selective_backward(dx.data_ptr(), ddt.data_ptr(), dA.data_ptr(), dB.data_ptr(), dC.data_ptr(), ptr(dD), ptr(dz),
                                        ptr(ddt_bias), ptr(dh0), rows_of(dy), ptr(dh_last), ckpt.data_ptr(), rows_of(x), rows_of(dt),
-                                       A.data_ptr(), rows_of(Bm), rows_of(Cm), ptr(D), rows_of(z), ptr(dt_bias), ptr(lengths),
+                                       A.data_ptr(), rows_of(Bm, 2), rows_of(Cm, 2), ptr(D), rows_of(z), ptr(dt_bias), ptr(lengths),
                                        softplus, ptr(ws), nbytes, DTYPES[x.dtype], B, T, M, N, G, dev, _stream_of(dev))
     _launched(st, "exb_selective_backward", x)
 
 
 def selective_step(y, h, x, dt, A, Bm, Cm, D, z, dt_bias, softplus: bool, B: int, M: int, N: int, G: int) -> None:
     dev = x.get_device()
-    st = load().exb_selective_step(y.data_ptr(), h.data_ptr(), h.stride(0), rows_of(x), rows_of(dt), A.data_ptr(), rows_of(Bm),
-                                   rows_of(Cm), ptr(D), rows_of(z), ptr(dt_bias), softplus, DTYPES[x.dtype], B, M, N, G, dev,
+    st = load().exb_selective_step(y.data_ptr(), h.data_ptr(), h.stride(0), rows_of(x), rows_of(dt), A.data_ptr(), rows_of(Bm, 2),
+                                   rows_of(Cm, 2), ptr(D), rows_of(z), ptr(dt_bias), softplus, DTYPES[x.dtype], B, M, N, G, dev,
                                    _stream_of(dev))
     _launched(st, "exb_selective_step", x)
 

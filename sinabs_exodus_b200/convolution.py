@@ -20,7 +20,6 @@ def _forward(x, weight, bias, state, lengths, activation):
     """Launches the forward pass: (y, last), and the tensors as the kernels read them."""
     nb, T, M = x.shape
     W = weight.shape[1]
-    x = _seq.channels_contiguous(x)
     weight, bias, state = _seq.dense(weight), _seq.dense(bias), _seq.dense(state)
     y, last = x.new_empty((nb, T, M)), x.new_empty((nb, W - 1, M))
     if nb * T * M:
@@ -62,7 +61,8 @@ class CausalConvTM(torch.autograd.Function):
             if dstate is not None and dlast is not None:
                 dstate.copy_(dlast)
         else:
-            dy = x.new_zeros((nb, T, M)) if dy is None else _seq.channels_contiguous(dy)
+            if dy is None:
+                dy = x.new_zeros((nb, T, M))
             _lib.causal_conv_backward(dx, dweight, dbias, dstate, dy, dlast, x, weight, bias, state, lengths, ctx.activation, nb, T, M, W)
         return dx, dweight, dbias, dstate, None, None
 
@@ -131,15 +131,16 @@ def causal_conv_step(state: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
     nb, M = x.shape
     if not _seq.alike(state, (nb, W - 1, M), x.dtype, x.get_device()) or state is None:
         _seq.require_like("state", state, (nb, W - 1, M), (x.dtype,), x.device)
-    if nb * M and _seq.channels_contiguous(state, 2) is not state:
-        raise ValueError("'state' must be contiguous in its rows and channels: it is updated in place")
-    if nb > 1 and state.stride(0) < (W - 1) * M:
-        raise ValueError("the batch items of 'state' overlap")
+    if not state.is_contiguous():
+        if nb * M and _seq.channels_contiguous(state, 2) is not state:
+            raise ValueError("'state' must be contiguous in its rows and channels: it is updated in place")
+        if nb > 1 and state.stride(0) < (W - 1) * M:
+            raise ValueError("the batch items of 'state' overlap")
     _seq.require_cuda("x", x)
     _seq.refuse_grad("causal_conv_step", state, x, weight, bias)
     y = x.new_empty((nb, M))
     if nb * M == 0:
         return y
-    _lib.causal_conv_step(y, state, _seq.channels_contiguous(x), _seq.dense(weight), _seq.dense(bias), activation, nb, M, W)
+    _lib.causal_conv_step(y, state, x, _seq.dense(weight), _seq.dense(bias), activation, nb, M, W)
     _seq.mark_changed(state)
     return y

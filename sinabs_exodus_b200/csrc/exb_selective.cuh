@@ -33,6 +33,15 @@ struct SelArgs {
     float *seg_dt;                       // [B][segments][M]
 };
 
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Whether rows can be read four elements at a time.
+template <typename T>
+bool pack_aligned(const View &v)
+{
+    return !v.p || (reinterpret_cast<uintptr_t>(v.p) % (4 * sizeof(T)) == 0 && v.sb % 4 == 0 && v.st % 4 == 0);
+}
+
 // Lanes per channel: four states in each.
 inline int sel_lanes(int N)
 {
@@ -45,11 +54,15 @@ inline int sel_lanes(int N)
 inline int sel_padded(int N) { const int l = sel_lanes(N); return 4 * (l < 2 ? 2 : l); }
 
 struct SelPlan {
-    int L, NP, CC, tiles, segments;
+    int L, S, NP, CC, tiles, segments;      // lanes of a channel, states of a lane, their product; channels of a block
     int64_t seg, chunks;
     int64_t off_h, off_dt, off_bc, off_a, off_d, bytes;      // offsets into the workspace
 };
 SelPlan sel_plan(int64_t B, int64_t T, int M, int N, int G, bool backward);
+
+// One translation unit per element type (exb_selective_f32.cu and so on): the kernels come in many shapes.
+template <typename T> cudaError_t selective_forward_typed(const SelArgs &a, const SelPlan &p, cudaStream_t s);
+template <typename T> cudaError_t selective_backward_typed(const SelArgs &a, const SelPlan &p, void *dB, void *dC, cudaStream_t s);
 
 cudaError_t launch_selective_forward(SelArgs a, int dtype, void *ws, cudaStream_t stream);
 cudaError_t launch_selective_backward(SelArgs a, int dtype, void *dB, void *dC, float *dA, float *dD, float *dbias, void *ws,

@@ -1,0 +1,9 @@
+// The selective scan on float16 tensors.
+#include "exb_selective_kernels.cuh"
+
+namespace exb {
+
+template cudaError_t selective_forward_typed<__half>(const SelArgs &, const SelPlan &, cudaStream_t);
+template cudaError_t selective_backward_typed<__half>(const SelArgs &, const SelPlan &, void *, void *, cudaStream_t);
+
+}  // namespace exb

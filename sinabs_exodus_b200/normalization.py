@@ -19,7 +19,7 @@ __all__ = ["GroupNormCL", "group_norm"]
 def _forward(x, num_groups, weight, bias, eps, activation):
     """Launches the forward pass: y, and what the backward pass reads."""
     R, S, C = x.shape
-    x, weight, bias = _seq.channels_contiguous(x), _seq.dense(weight), _seq.dense(bias)
+    weight, bias = _seq.dense(weight), _seq.dense(bias)
     y = x.new_empty((R, S, C))
     mean, rstd = (torch.empty((R, num_groups), dtype=torch.float32, device=x.device) for _ in range(2))
     if R * S * C:
@@ -47,7 +47,7 @@ class GroupNormCL(torch.autograd.Function):
         dweight = torch.empty_like(weight) if weight is not None else None
         dbias = torch.empty_like(bias) if bias is not None else None
         if R * S * C:
-            _lib.group_norm_backward(dx, dweight, dbias, _seq.channels_contiguous(dy), x, mean, rstd, weight, bias, ctx.activation, R, S,
+            _lib.group_norm_backward(dx, dweight, dbias, dy, x, mean, rstd, weight, bias, ctx.activation, R, S,
                                      C, ctx.num_groups)
         else:
             for t in (dweight, dbias):

@@ -26,8 +26,6 @@ def _forward(x, dt, A, B, C, D, z, dt_bias, h0, lengths, dt_softplus, keep):
     """Launches the forward pass: (y, h_last, checkpoints or None), and the tensors as the kernels read them."""
     nb, T, M = x.shape
     G, N = B.shape[2:]
-    x, dt, z = _seq.channels_contiguous(x), _seq.channels_contiguous(dt), _seq.channels_contiguous(z)
-    B, C = _seq.channels_contiguous(B, 2), _seq.channels_contiguous(C, 2)
     A, D, dt_bias, h0 = _seq.dense(A), _seq.dense(D), _seq.dense(dt_bias), _seq.dense(h0)
     y = x.new_empty((nb, T, M))
     h_last = A.new_empty((nb, M, N))
@@ -77,7 +75,8 @@ class SelectiveScanTM(torch.autograd.Function):
             if dh0 is not None and dh_last is not None:
                 dh0.copy_(dh_last)
         else:
-            dy = x.new_zeros((nb, T, M)) if dy is None else _seq.channels_contiguous(dy)
+            if dy is None:
+                dy = x.new_zeros((nb, T, M))
             _lib.selective_backward(dx, ddt, dA, dB, dC, dD, dz, ddt_bias, dh0, dy, dh_last, ckpt, x, dt, A, B, C, D, z, dt_bias,
                                     lengths, ctx.softplus, nb, T, M, N, G)
         return dx, ddt, dA, dB, dC, dD, dz, ddt_bias, dh0, None, None
@@ -171,17 +170,16 @@ def selective_step(h: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, A: torch.
     G, N = B.shape[1], B.shape[2]
     if not _seq.alike(h, (nb, M, N), torch.float32, x.get_device()) or h is None:
         _seq.require_like("h", h, (nb, M, N), (torch.float32,), x.device)
-    if nb * M and _seq.channels_contiguous(h, 2) is not h:
-        raise ValueError("'h' must be contiguous in its channels and states: it is updated in place")
-    if nb > 1 and h.stride(0) < M * N:
-        raise ValueError("the batch items of 'h' overlap")
+    if not h.is_contiguous():
+        if nb * M and _seq.channels_contiguous(h, 2) is not h:
+            raise ValueError("'h' must be contiguous in its channels and states: it is updated in place")
+        if nb > 1 and h.stride(0) < M * N:
+            raise ValueError("the batch items of 'h' overlap")
     _seq.require_cuda("x", x)
     _seq.refuse_grad("selective_step", h, x, dt, A, B, C, D, z, dt_bias)
     y = x.new_empty((nb, M))
     if nb * M == 0:
         return y
-    _lib.selective_step(y, h, _seq.channels_contiguous(x), _seq.channels_contiguous(dt), _seq.dense(A), _seq.channels_contiguous(B, 2),
-                        _seq.channels_contiguous(C, 2), _seq.dense(D), _seq.channels_contiguous(z), _seq.dense(dt_bias),
-                        bool(dt_softplus), nb, M, N, G)
+    _lib.selective_step(y, h, x, dt, _seq.dense(A), B, C, _seq.dense(D), z, _seq.dense(dt_bias), bool(dt_softplus), nb, M, N, G)
     _seq.mark_changed(h)
     return y
