@@ -132,12 +132,55 @@ __global__ void __launch_bounds__(TX * TY) conv_forward_kernel(const ConvArgs a)
     }
 }
 
+// Rows of x and dy on their way to one thread: STEP rows at a time, DEPTH times ahead, through a ring in shared memory that
+// only this thread writes (asynchronous copies, which fill in zeros for rows that do not exist) and reads.  In registers they
+// would cost the occupancy that the backward pass needs.  Rows that are not aligned are loaded when they are needed.
+template <typename T, int V, bool VEC>
+struct Rows {
+    static constexpr int DEPTH = 3, BYTES = V * (int)sizeof(T);
+    static constexpr int RING = VEC ? DEPTH * STEP * 2 * TX * TY * BYTES : 0;
+    char *ring;
+    int slot = 0;      // group that is taken next
+
+    __device__ __forceinline__ explicit Rows(char *base) : ring(base + (threadIdx.y * TX + threadIdx.x) * BYTES) {}
+    __device__ __forceinline__ char *at(int group, int j, int which) const { return ring + ((group * STEP + j) * 2 + which) * (TX * TY * BYTES); }
+    __device__ __forceinline__ static void copy(char *to, const T *from, bool there)
+    {
+        const unsigned dst = (unsigned)__cvta_generic_to_shared(to), bytes = there ? BYTES : 0;
+        if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");
+        else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");
+    }
+    // Rows t .. t + STEP of both tensors on their way into group `group` (rows that do not exist: any valid address).
+    template <typename There>
+    __device__ __forceinline__ void issue(int group, const T *x, int64_t step_x, const T *g, int64_t step_g, int64_t t, const There &there) const
+    {
+#pragma unroll
+        for (int j = 0; j < STEP; ++j) {
+            const bool h = there(t + j);
+            copy(at(group, j, 0), h ? x + (t + j) * step_x : x, h);
+            copy(at(group, j, 1), h ? g + (t + j) * step_g : g, h);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    __device__ __forceinline__ static void take(RawPack<T, V, VEC> &r, const char *from)
+    {
+        if constexpr (BYTES == 16) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(from);
+            r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w;
+        } else {
+            const uint2 v = *reinterpret_cast<const uint2 *>(from);
+            r.w[0] = v.x; r.w[1] = v.y;
+        }
+    }
+};
+
 // A thread forms the gradient in front of the activation, d, for its run and for the W - 1 steps behind it (which the rows
 // of its run feed), and from those dx; filter and bias gradients only take the run's own steps.
 template <typename T, int V, int W, bool VEC>
-__global__ void __launch_bounds__(TX * TY) conv_backward_kernel(const ConvArgs a)
+__global__ void __launch_bounds__(TX * TY, W <= 4 ? 3 : 1) conv_backward_kernel(const ConvArgs a)
 {
-    extern __shared__ float s_part[];      // [TY][W + 1][TX * V]
+    extern __shared__ uint4 s_raw[];      // the rings, and at the end the sums [TY][W + 1][TX * V]
+    float *s_part = reinterpret_cast<float *>(s_raw);
     const Spot s = place<V>(a);
     float2 dw[W + 1][V / 2];
 #pragma unroll
@@ -146,16 +189,16 @@ __global__ void __launch_bounds__(TX * TY) conv_backward_kernel(const ConvArgs a
         for (int k = 0; k <= W; ++k) dw[k][i] = both(0.0f);
     if (s.left > 0 && s.t0 < a.T) {
         const Filter<T, V, W> f(a, s);
-        RawPack<T, V, VEC> next_x[STEP], next_g[STEP];
+        using Ring = Rows<T, V, VEC>;
+        Ring ring(reinterpret_cast<char *>(s_raw));
         float2 row[STEP + W - 1][V / 2], d[STEP + W - 1][V / 2];      // entry j: step t - (W - 1) + j
         const int64_t end = s.t1 + W - 1;      // rows t - (W - 1) in [t0 (or the state's), t1) come out
-        auto fetch = [&](int64_t t) {
+        const T *x = static_cast<const T *>(a.x.p) + s.b * a.x.sb + s.m, *dy = static_cast<const T *>(a.dy.p) + s.b * a.dy.sb + s.m;
+        auto there = [&](int64_t t) { return t < s.len && t < end; };
+        if constexpr (VEC) {
 #pragma unroll
-            for (int j = 0; j < STEP; ++j) {
-                load_row<T, V, W, VEC>(next_x[j], a, s, t + j);
-                next_g[j].load(static_cast<const T *>(a.dy.p) + s.b * a.dy.sb + (t + j) * a.dy.st + s.m, (t + j < s.len && t + j < end) ? s.left : 0);
-            }
-        };
+            for (int q = 0; q < Ring::DEPTH; ++q) ring.issue(q, x, a.x.st, dy, a.dy.st, s.t0 + q * STEP, there);
+        }
 #pragma unroll
         for (int k = 0; k < W - 1; ++k) {
             RawPack<T, V, VEC> r;
@@ -166,19 +209,31 @@ __global__ void __launch_bounds__(TX * TY) conv_backward_kernel(const ConvArgs a
                 d[k][i] = both(0.0f);
             }
         }
-        fetch(s.t0);
         T *out = static_cast<T *>(a.dx) + (s.b * a.T + s.t0 - (W - 1)) * a.M + s.m;
         T *out_state = (s.t0 == 0 && a.dstate) ? static_cast<T *>(a.dstate) + s.b * (W - 1) * a.M + s.m : nullptr;
         for (int64_t t = s.t0; t < end; t += STEP) {
             float2 up[STEP][V / 2];
+            if constexpr (VEC) asm volatile("cp.async.wait_group %0;" ::"n"(Ring::DEPTH - 1) : "memory");
 #pragma unroll
-            for (int j = 0; j < STEP; ++j)
+            for (int j = 0; j < STEP; ++j) {
+                RawPack<T, V, VEC> rx, rg;
+                if constexpr (VEC) {
+                    Ring::take(rx, ring.at(ring.slot, j, 0));
+                    Ring::take(rg, ring.at(ring.slot, j, 1));
+                } else {
+                    rx.load(x + (t + j) * a.x.st, there(t + j) ? s.left : 0);
+                    rg.load(dy + (t + j) * a.dy.st, there(t + j) ? s.left : 0);
+                }
 #pragma unroll
                 for (int i = 0; i < V / 2; ++i) {
-                    row[W - 1 + j][i] = next_x[j].pair(i);
-                    up[j][i] = next_g[j].pair(i);
+                    row[W - 1 + j][i] = rx.pair(i);
+                    up[j][i] = rg.pair(i);
                 }
-            if (t + STEP < end) fetch(t + STEP);
+            }
+            if constexpr (VEC) {
+                ring.issue(ring.slot, x, a.x.st, dy, a.dy.st, t + Ring::DEPTH * STEP, there);
+                ring.slot = ring.slot == Ring::DEPTH - 1 ? 0 : ring.slot + 1;
+            }
 #pragma unroll
             for (int j = 0; j < STEP; ++j) {
                 const int64_t now = t + j, r = now - (W - 1);
@@ -225,6 +280,8 @@ __global__ void __launch_bounds__(TX * TY) conv_backward_kernel(const ConvArgs a
                 }
         }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();      // nobody's rows are on their way any more
 #pragma unroll
     for (int k = 0; k <= W; ++k)
 #pragma unroll
@@ -329,8 +386,11 @@ cudaError_t backward_typed(ConvArgs a, void *dweight, void *dbias, cudaStream_t 
 {
     a.run = run_of(a.B, a.T, a.M, 64);
     const int64_t rows = a.B * ceil_div(a.T, a.run * TY);
-    constexpr int smem = TY * (W + 1) * TX * N * (int)sizeof(float);
-    static_assert(smem <= 48 * 1024, "");
+    constexpr int sums = TY * (W + 1) * TX * N * (int)sizeof(float), ring = Rows<T, N, VEC>::RING, smem = sums > ring ? sums : ring;
+    if (smem > 48 * 1024) {
+        cudaError_t e = cudaFuncSetAttribute(conv_backward_kernel<T, N, W, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+    }
     conv_backward_kernel<T, N, W, VEC><<<(unsigned)(ceil_div(a.M, TX * N) * rows), dim3(TX, TY), smem, s>>>(a);
     const int64_t cols = (int64_t)(W + 1) * a.M;
     if (a.params_f32) launch_column_sum(PutParams<float>{(float *)dweight, (float *)dbias, a.M, W}, a.part, rows, cols, s);
