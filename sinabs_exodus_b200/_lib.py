@@ -696,22 +696,23 @@ def _f32_params(weight, bias) -> bool:
     return p is None or p.dtype == torch.float32
 
 
-def group_norm_forward(y, mean, rstd, x, weight, bias, eps: float, activation, R: int, S: int, C: int, G: int) -> None:
+def group_norm_forward(y, stats, x, weight, bias, eps: float, activation, R: int, S: int, C: int, G: int) -> None:
+    """``stats``: (2, R, G) float32, the groups' means and the reciprocals of their deviations."""
     dtype, dev = DTYPES[x.dtype], x.get_device()
     nbytes = _group_norm_workspace_bytes(R, S, C, G, dtype, 0)
     ws = _workspace(nbytes, x)
-    st = load().exb_group_norm_forward(y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), rows_of(x), ptr(weight), ptr(bias), eps,
+    st = load().exb_group_norm_forward(y.data_ptr(), stats.data_ptr(), stats.data_ptr() + 4 * R * G, rows_of(x), ptr(weight), ptr(bias), eps,
                                        ACTIVATIONS[activation], _f32_params(weight, bias), ptr(ws), nbytes, dtype, R, S, C, G, dev,
                                        _stream_of(dev))
     _launched(st, "exb_group_norm_forward", x)
 
 
-def group_norm_backward(dx, dweight, dbias, dy, x, mean, rstd, weight, bias, activation, R: int, S: int, C: int, G: int) -> None:
+def group_norm_backward(dx, dweight, dbias, dy, x, stats, weight, bias, activation, R: int, S: int, C: int, G: int) -> None:
     dtype, dev = DTYPES[x.dtype], x.get_device()
     nbytes = _group_norm_workspace_bytes(R, S, C, G, dtype, 1)
     ws = _workspace(nbytes, x)
-    st = load().exb_group_norm_backward(dx.data_ptr(), ptr(dweight), ptr(dbias), rows_of(dy), rows_of(x), mean.data_ptr(),
-                                        rstd.data_ptr(), ptr(weight), ptr(bias), ACTIVATIONS[activation], _f32_params(weight, bias),
+    st = load().exb_group_norm_backward(dx.data_ptr(), ptr(dweight), ptr(dbias), rows_of(dy), rows_of(x), stats.data_ptr(),
+                                        stats.data_ptr() + 4 * R * G, ptr(weight), ptr(bias), ACTIVATIONS[activation], _f32_params(weight, bias),
                                         ptr(ws), nbytes, dtype, R, S, C, G, dev, _stream_of(dev))
     _launched(st, "exb_group_norm_backward", x)
 

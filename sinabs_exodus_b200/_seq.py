@@ -45,11 +45,12 @@ def alike(t: Optional[torch.Tensor], shape, dtype: torch.dtype, device: int) -> 
 _TENSORS = (torch.Tensor, torch.nn.Parameter)
 
 
-def check_lengths(lengths: Optional[torch.Tensor], batch: int, device: torch.device) -> Optional[torch.Tensor]:
-    if lengths is None:
-        return None
+def check_lengths(lengths: torch.Tensor, batch: int, steps: int, device: torch.device) -> torch.Tensor:
+    """``lengths`` as the kernels take them; 64-bit values are clamped before they lose their upper half."""
     require_like("lengths", lengths, (batch,), (torch.int32, torch.int64), device)
-    return lengths.to(torch.int32).contiguous()
+    if lengths.dtype == torch.int64:
+        lengths = lengths.clamp(0, steps).to(torch.int32)
+    return lengths.contiguous()
 
 
 def channels_contiguous(t: Optional[torch.Tensor], trailing: int = 1) -> Optional[torch.Tensor]:

@@ -111,7 +111,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     if state is not None:
         _seq.require_like("state", state, (x.shape[0], W - 1, x.shape[2]), (x.dtype,), x.device)
     if lengths is not None:
-        lengths = _seq.check_lengths(lengths, x.shape[0], x.device)
+        lengths = _seq.check_lengths(lengths, x.shape[0], x.shape[1], x.device)
     _seq.require_cuda("x", x)
     if not _seq.wants_grad(x, weight, bias, state):
         return _forward(x, weight, bias, state, lengths, activation)[:2]

@@ -1051,7 +1051,9 @@ template <typename T, int V, bool VEC>
 cudaError_t maps_forward(NormArgs a, bool cluster, cudaStream_t s)
 {
     constexpr int RING = Walk<T, V, VEC, false>::RING;
-    const unsigned grid = (unsigned)(a.R * a.chunks * a.slabs);
+    const int64_t blocks = a.R * a.chunks * a.slabs;
+    if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+    const unsigned grid = (unsigned)blocks;
     a.smem = map_smem<V>(a);
     const int smem = RING + a.smem * (int)sizeof(float2), apply = RING + a.slab * (int)sizeof(float2);
     if (cluster) return launch_clusters(norm_cluster_forward_kernel<T, V, VEC>, a, grid, smem + a.slab * (int)sizeof(Moments), s);
@@ -1066,7 +1068,9 @@ template <typename T, int V, bool VEC>
 cudaError_t maps_backward(NormArgs a, bool cluster, cudaStream_t s)
 {
     constexpr int RING = Walk<T, V, VEC, true>::RING;
-    const unsigned grid = (unsigned)(a.R * a.chunks * a.slabs);
+    const int64_t blocks = a.R * a.chunks * a.slabs;
+    if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+    const unsigned grid = (unsigned)blocks;
     a.smem = map_smem<V>(a);
     const int smem = RING + a.smem * (int)sizeof(float2), apply = RING + a.slab * (int)sizeof(float2);
     if (cluster) return launch_clusters(norm_cluster_backward_kernel<T, V, VEC>, a, grid, smem + a.slab * (int)sizeof(float2), s);

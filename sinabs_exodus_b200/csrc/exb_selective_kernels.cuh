@@ -947,7 +947,9 @@ __global__ void __launch_bounds__(Geo<L, S>::NT + Geo<L, S>::NH, Geo<L, S>::BLOC
             }
             {      // backward
                 float sb[GS], sa[GS];
-                States<S> vb[SC];
+                States<S> vb[SC], dA_c[2];      // sums of few steps first: thousands of terms one by one would lose digits
+                dA_c[0].fill(0.0f);
+                dA_c[1].fill(0.0f);
 #pragma unroll
                 for (int i = KH - 1; i >= 0; --i) {
                     const int t = half * KH + i;
@@ -968,7 +970,7 @@ __global__ void __launch_bounds__(Geo<L, S>::NT + Geo<L, S>::NH, Geo<L, S>::BLOC
                             g[k].q[q] = mul2(g[k].q[q], av[i][k].q[q]);
                             const float2 u = mul2(g[k].q[q], before[i][k].q[q]);
                             ra = q ? fma2(u, A2[k].q[q], ra) : mul2(u, A2[k].q[q]);
-                            dA[k].q[q] = fma2(u, both(d.x), dA[k].q[q]);
+                            dA_c[k].q[q] = fma2(u, both(d.x), dA_c[k].q[q]);
                         }
                         tb[k] = rb.x + rb.y;
                         ta[k] = ra.x + ra.y;
@@ -981,6 +983,10 @@ __global__ void __launch_bounds__(Geo<L, S>::NT + Geo<L, S>::NH, Geo<L, S>::BLOC
                     }
                     if (i % SC == 0) across(vb, t, 0);
                 }
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int q = 0; q < S / 2; ++q) dA[k].q[q] = add2(dA[k].q[q], dA_c[k].q[q]);
             }
         }
     }

@@ -21,10 +21,10 @@ def _forward(x, num_groups, weight, bias, eps, activation):
     R, S, C = x.shape
     weight, bias = _seq.dense(weight), _seq.dense(bias)
     y = x.new_empty((R, S, C))
-    mean, rstd = (torch.empty((R, num_groups), dtype=torch.float32, device=x.device) for _ in range(2))
+    stats = torch.empty((2, R, num_groups), dtype=torch.float32, device=x.device)      # mean, 1 / deviation
     if R * S * C:
-        _lib.group_norm_forward(y, mean, rstd, x, weight, bias, eps, activation, R, S, C, num_groups)
-    return y, (x, weight, bias, mean, rstd)
+        _lib.group_norm_forward(y, stats, x, weight, bias, eps, activation, R, S, C, num_groups)
+    return y, (x, weight, bias, stats)
 
 
 class GroupNormCL(torch.autograd.Function):
@@ -41,13 +41,13 @@ class GroupNormCL(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         _seq.refuse_second_order("group_norm")
-        x, weight, bias, mean, rstd = ctx.saved_tensors
+        x, weight, bias, stats = ctx.saved_tensors
         R, S, C = x.shape
         dx = x.new_empty((R, S, C))
         dweight = torch.empty_like(weight) if weight is not None else None
         dbias = torch.empty_like(bias) if bias is not None else None
         if R * S * C:
-            _lib.group_norm_backward(dx, dweight, dbias, dy, x, mean, rstd, weight, bias, ctx.activation, R, S,
+            _lib.group_norm_backward(dx, dweight, dbias, dy, x, stats, weight, bias, ctx.activation, R, S,
                                      C, ctx.num_groups)
         else:
             for t in (dweight, dbias):
@@ -82,8 +82,10 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
         raise ValueError(f"'activation' must be None, 'silu' or 'relu', got {activation!r}")
     if not eps >= 0.0:
         raise ValueError(f"'eps' must not be negative, got {eps}")
-    _seq.require_like("weight", weight, (C,), (torch.float32, x.dtype), x.device)
-    _seq.require_like("bias", bias, (C,), (torch.float32, x.dtype), x.device)
+    kind, dev = (weight if weight is not None else x if bias is None else bias).dtype, x.get_device()
+    if dev < 0 or (kind != torch.float32 and kind != x.dtype) or not (_seq.alike(weight, (C,), kind, dev) and _seq.alike(bias, (C,), kind, dev)):
+        _seq.require_like("weight", weight, (C,), (torch.float32, x.dtype), x.device)
+        _seq.require_like("bias", bias, (C,), (torch.float32, x.dtype), x.device)
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError(f"'weight' and 'bias' must have one type, got {weight.dtype} and {bias.dtype}")
     _seq.require_cuda("x", x)

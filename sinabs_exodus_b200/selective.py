@@ -148,7 +148,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     if h0 is not None:
         _seq.require_like("h0", h0, (x.shape[0], x.shape[2], B.shape[3]), (torch.float32,), x.device)
     if lengths is not None:
-        lengths = _seq.check_lengths(lengths, x.shape[0], x.device)
+        lengths = _seq.check_lengths(lengths, x.shape[0], x.shape[1], x.device)
     _seq.require_cuda("x", x)
     if _seq.wants_grad(x, dt, A, B, C, D, z, dt_bias, h0):
         return SelectiveScanTM.apply(x, dt, A, B, C, D, z, dt_bias, h0, lengths, bool(dt_softplus))

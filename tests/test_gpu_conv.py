@@ -182,3 +182,29 @@ def test_step_refuses_gradients():
     p, _, _ = problem(9, 2, 1, 8, 4, F32)
     with pytest.raises(RuntimeError, match="not differentiable"):
         ex.causal_conv_step(p["state"], p["x"][:, 0], p["weight"].requires_grad_(True))
+
+
+def test_step_of_many():
+    """Several batch items per thread."""
+    import sinabs_exodus_b200 as ex
+    for nb, M in ((515, 1024), (33, 4098)):
+        p, _, _ = problem(10, nb, 1, M, 4, BF16)
+        want, want_state = ex.causal_conv(**p)
+        state = p["state"].clone()
+        y = ex.causal_conv_step(state, p["x"][:, 0], p["weight"], p["bias"], activation="silu")
+        assert torch.equal(state, want_state)
+        torch.testing.assert_close(y, want[:, 0], rtol=4 * ref.HALF_STEP[BF16], atol=2e-3)
+
+
+def test_long_runs():
+    """Rows enough that a thread walks its longest run, several times round the ring of rows on their way."""
+    p, dy, dl = problem(11, 2, 5000, 136, 4, F32, lengths=[5000, 4103])
+    check(run(p, dy, dl), p, dy, dl)
+
+
+def test_second_derivatives_are_refused():
+    import sinabs_exodus_b200 as ex
+    p, dy, _ = problem(12, 1, 6, 8, 4, F32)
+    p["x"].requires_grad_(True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(ex.causal_conv(**p)[0], p["x"], dy, create_graph=True)

@@ -192,3 +192,29 @@ def test_layer():
     out = net(torch.randn(6, 2, 5, 7, device=DEV).to(memory_format=torch.channels_last))
     out.sum().backward()
     assert out.shape == (6, 16, 5, 7) and torch.isfinite(layer.weight.grad).all() and net[0].weight.grad.abs().sum() > 0
+
+
+# samples enough that clusters of blocks take one each: of 8, 2, 1 blocks; rows that do not fill a pack; several slabs
+CLUSTERS = [(40, 2100, 64, 8), (150, 1100, 44, 4), (300, 70, 32, 4), (40, 1300, 160, 32), (60, 600, 2048, 8), (310, 3, 24, 2)]
+
+
+@pytest.mark.parametrize("size", CLUSTERS)
+@pytest.mark.parametrize("kind,act", [(F32, "silu"), (BF16, "silu"), (F16, None)])
+def test_clusters(size, kind, act):
+    R, S, C, G = size
+    x, w, b, dy = problem(7, R, S, C, kind)
+    check(run(x, G, w, b, dy, act), x, G, w, b, dy, act, offset=7.0)
+
+
+def test_largest_groups():
+    """Groups as wide as they may be, where the sums over channels fill a block's shared memory."""
+    for S, C, G in ((1, 16384, 1), (5, 16384, 1), (3, 32766, 2)):
+        x, w, b, dy = problem(8, 2, S, C, BF16)
+        check(run(x, G, w, b, dy, "silu"), x, G, w, b, dy, "silu", offset=6.0)
+
+
+def test_second_derivatives_are_refused():
+    import sinabs_exodus_b200 as ex
+    x = torch.randn(2, 5, 8, device=DEV, requires_grad=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(ex.group_norm(x, 2).sum(), x, create_graph=True)

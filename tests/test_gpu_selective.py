@@ -279,3 +279,121 @@ def test_step_refuses_gradients():
         ex.selective_step(p["h0"], A=p["A"], **args)
     with torch.no_grad():
         ex.selective_step(p["h0"], A=p["A"], **args)
+
+
+# The kernels come in two forms, for problems with one block of channels per SM and for larger ones; the sizes above are
+# all of the first.  Many batch items and channels, whole and split over time, every number of lanes.
+LARGE = [(20, 24, 512, 16, 1), (20, 11, 1000, 8, 1), (5, 19, 1024, 32, 2), (4, 24, 640, 64, 1), (3, 9, 408, 128, 1), (5, 560, 256, 16, 1),
+         (4, 600, 258, 7, 1)]
+
+
+@pytest.mark.parametrize("size", LARGE)
+@pytest.mark.parametrize("kind", [F32, BF16])
+def test_many_blocks(size, kind):
+    p, dy, dh = problem(20, *size, kind)
+    check(run(p, dy, dh), p, dy, dh)
+
+
+def test_many_blocks_padded():
+    T = 560
+    p, dy, dh = problem(21, 5, T, 256, 16, 1, F32, lengths=[0, 1, T, 333, 48])
+    for b, n in enumerate(p["lengths"].tolist()):
+        p["x"][b, n:] = p["B"][b, n:] = p["z"][b, n:] = float("nan")
+        dy[b, n:] = float("inf")
+    got = run(p, dy, dh)
+    for k in ("y", "dx", "ddt", "dB", "dC", "dz"):
+        for b, n in enumerate(p["lengths"].tolist()):
+            assert (got[k][b, n:] == 0).all(), k
+    check(got, p, dy, dh)
+
+
+def test_lengths_of_64_bits():
+    import sinabs_exodus_b200 as ex
+    p, _, _ = problem(22, 2, 12, 8, 4, 1, F32)
+    a = ex.selective_scan(**dict(p, lengths=torch.tensor([2 ** 40, 5], device=DEV)))
+    b = ex.selective_scan(**dict(p, lengths=torch.tensor([12, 5], device=DEV, dtype=torch.int32)))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_second_derivatives_are_refused():
+    import sinabs_exodus_b200 as ex
+    p, dy, _ = problem(23, 1, 6, 8, 4, 1, F32)
+    p["x"].requires_grad_(True)
+    y, _ = ex.selective_scan(**p)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(y, p["x"], dy, create_graph=True)
+
+
+def test_upstream_gradient_of_a_sum():
+    """An expanded upstream gradient, as sum() sends it; and one for the state alone."""
+    import sinabs_exodus_b200 as ex
+    p, _, dh = problem(24, 2, 20, 24, 8, 1, F32)
+    a = run(p, torch.ones(2, 20, 24, device=DEV))
+    x = p["x"].clone().requires_grad_(True)
+    ex.selective_scan(**dict(p, x=x))[0].sum().backward()
+    assert torch.equal(x.grad, a["dx"])
+    x.grad = None
+    ex.selective_scan(**dict(p, x=x))[1].backward(dh)
+    b = run(p, torch.zeros(2, 20, 24, device=DEV), dh)
+    assert torch.equal(x.grad, b["dx"])
+
+
+def test_two_graphs_and_two_streams_at_once():
+    """Calls that run side by side have scratch memory of their own."""
+    import sinabs_exodus_b200 as ex
+    ps = [problem(25 + i, 1, 900, 64, 16, 1, F32)[0] for i in range(2)]
+    want = [ex.selective_scan(**p) for p in ps]
+    graphs, held = [], []
+    for p in ps:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            held.append(ex.selective_scan(**p))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in ps]
+    for _ in range(3):
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for w, h in zip(want, held):
+        assert torch.equal(w[0], h[0]) and torch.equal(w[1], h[1])
+    outs = []
+    for s, p in zip(streams, ps):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            outs.append([ex.selective_scan(**p) for _ in range(3)][-1])
+    torch.cuda.synchronize()
+    for w, o in zip(want, outs):
+        assert torch.equal(w[0], o[0]) and torch.equal(w[1], o[1])
+
+
+@pytest.mark.parametrize("nb", [4, 7, 130])
+@pytest.mark.parametrize("N", [3, 8, 16, 40])
+def test_step_of_many(nb, N):
+    """Several batch items per thread, a number that does not divide them among it."""
+    import sinabs_exodus_b200 as ex
+    p, _, _ = problem(30, nb, 1, 2048, N, 1, BF16)
+    h = p["h0"].clone()
+    args = {k: p[k][:, 0] for k in ("x", "dt", "B", "C", "z")}
+    y = ex.selective_step(h, A=p["A"], D=p["D"], dt_bias=p["dt_bias"], **args)
+    check({"y": y[:, None], "h": h}, p)
+
+
+def test_step_in_a_graph_and_inference_mode():
+    import sinabs_exodus_b200 as ex
+    p, _, _ = problem(31, 3, 1, 40, 16, 1, F32)
+    args = {k: p[k][:, 0].contiguous() for k in ("x", "dt", "B", "C", "z")}
+    rest = dict(A=p["A"], D=p["D"], dt_bias=p["dt_bias"])
+    a, b = p["h0"].clone(), p["h0"].clone()
+    for _ in range(4):
+        want = ex.selective_step(a, **args, **rest)
+    ex.selective_step(b.clone(), **args, **rest)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = ex.selective_step(b, **args, **rest)
+    for _ in range(4):
+        g.replay()
+    assert torch.equal(a, b) and torch.equal(want, got)
+    with torch.inference_mode():
+        c = p["h0"].clone()
+        ex.selective_step(c, **args, **rest)
