@@ -74,7 +74,8 @@ struct Filter {
     }
 };
 
-// 8 x 2048 x 4096 bfloat16, W = 4 (268 MB): see the table in the design notes for the measured time.
+// 8 x 2048 x 4096, W = 4, silu, bfloat16 (268 MB read and written): 63 us, 4.3 TB/s; 5 x 1999 x 1023, W = 3, float16, rows that
+// start at odd addresses: 17.8 us, 2.3 TB/s, bound by the single-element accesses.
 template <typename T, int V, int W, bool VEC>
 __global__ void __launch_bounds__(TX * TY) conv_forward_kernel(const ConvArgs a)
 {
@@ -176,6 +177,8 @@ struct Rows {
 
 // A thread forms the gradient in front of the activation, d, for its run and for the W - 1 steps behind it (which the rows
 // of its run feed), and from those dx; filter and bias gradients only take the run's own steps.
+// 8 x 2048 x 4096, W = 4, silu, bfloat16 (403 MB): 144 us, 2.8 TB/s; half of the issue slots are busy with 12 warps on an SM
+// (168 registers: filter, its gradient, and the windows of x and d).  With the rows ahead in registers: 184 us.
 template <typename T, int V, int W, bool VEC>
 __global__ void __launch_bounds__(TX * TY, W <= 4 ? 3 : 1) conv_backward_kernel(const ConvArgs a)
 {
@@ -311,7 +314,8 @@ struct PutParams {
     }
 };
 
-// One step: a thread takes V channels of `items` batch items, with their filters in registers.
+// One step: a thread takes V channels of `items` batch items, with their filters in registers.  512 x 4096, W = 4, bfloat16
+// (34 MB): 6.6 us, 5.1 TB/s.
 template <typename T, int V, int W, bool VEC>
 __global__ void __launch_bounds__(128) conv_step_kernel(const ConvStepArgs a, int items)
 {

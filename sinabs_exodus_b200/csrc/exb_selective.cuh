@@ -55,7 +55,7 @@ inline int sel_padded(int N) { const int l = sel_lanes(N); return 4 * (l < 2 ? 2
 
 struct SelPlan {
     int L, S, NP, CC, tiles, segments;      // lanes of a channel, states of a lane, their product; channels of a block
-    int64_t seg, chunks;
+    int64_t seg;
     int64_t off_h, off_dt, off_bc, off_a, off_d, bytes;      // offsets into the workspace
 };
 SelPlan sel_plan(int64_t B, int64_t T, int M, int N, int G, bool backward);

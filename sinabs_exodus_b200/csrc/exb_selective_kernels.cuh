@@ -1,11 +1,13 @@
-// Selective scan: a leaky integrator whose decay, input weight and readout depend on the input.
+// Selective scan: kernels of the forward pass, of its time split and of the backward pass.  A leaky integrator whose decay,
+// input weight and readout depend on the input:
 //
 //   h_t[d,n] = exp(dt_t[d] A[d,n]) h_{t-1}[d,n] + dt_t[d] x_t[d] B_t[g,n]        g = d / (M / G)
 //   y_t[d]   = (sum_n C_t[g,n] h_t[d,n] + D[d] x_t[d]) * silu(z_t[d])
 //
-// Mapping: L neighbouring lanes hold the N <= 4L states of a channel, four each; a block owns CC channels of one group
-// and one batch item and walks a piece of the time axis.  The block first turns the chunk's x, dt (and z, dy) into
-// what the recurrence needs, one thread per element and not per state, and leaves it in shared memory.
+// What bounds it.  Per step, channel and state an exponential and some seven other operations, for two or three bytes: the
+// exponentials alone (16 per SM and clock, 4.6e12 / s) take three times as long as the bytes at N = 16 in 16 bits, and
+// issuing the rest takes longer still.  So: states in registers, pairs of float32 per instruction, everything that is not
+// per state done once per (step, channel) by warps of their own, sums over lanes without selections.
 #pragma once
 
 #include "exb_selective.cuh"
@@ -298,6 +300,9 @@ constexpr int forward_smem_bytes()
     return (int)sizeof(float) * 2 * (Q::KF * Q::CC * 5 + 2 * Q::KF * Q::NP);
 }
 
+// Measured (N = 16, bfloat16, gated): 1 x 16384 x 1024 in 18 pieces 125 us, half of the issue slots busy, the rest barrier
+// and fixed latencies; 4 x 2048 x 2048 whole, with checkpoints, 169 us on 128 of the 148 SMs (S = 2; with S = 4 one
+// recurrence warp per scheduler, 182 us).  Exponentials: 58 us of either.
 template <typename T, int L, int S, bool VEC>
 __global__ void __launch_bounds__(Geo<L, S>::NT + Geo<L, S>::NH, Geo<L, S>::BLOCKS) sel_forward_kernel(const SelArgs a)
 {
@@ -480,7 +485,7 @@ constexpr int state_smem_bytes()
 }
 
 // What a piece of time hands on when nothing enters it, and its sum of step sizes: the state behind its last step, or
-// (REVERSE) the gradient that goes to the step in front of its first one.
+// (REVERSE) the gradient that goes to the step in front of its first one.  1 x 16384 x 1024 x 16 in 18 pieces: 88 us.
 template <typename T, int L, int S, bool VEC, bool REVERSE>
 __global__ void __launch_bounds__(Geo<L, S>::NT + Geo<L, S>::NH, Geo<L, S>::BLOCKS) sel_state_kernel(const SelArgs a)
 {
@@ -654,7 +659,10 @@ constexpr int backward_smem_bytes()
 // decays a_t in registers, and runs the reverse recurrence  g_t = C_t p_t + a_{t+1} g_{t+1}  (p = dy silu(z)) on them.
 // With four states to a lane it does so by halves of a chunk, the later one first, for which the earlier one is run through
 // once more: a quarter more exponentials, and registers for two blocks on an SM, whose barriers then do not stop all of it.
-// The launch then gives every thread 128 registers, of which the preparing warps hand 40 to those of the recurrence.
+// The launch gives every thread 128 registers, of which the preparing warps hand 40 to those of the recurrence.
+// Measured (N = 16, bfloat16, gated): 4 x 2048 x 2048 whole 424 us, issue slots 63 % busy (about 106 instructions per 128
+// element-steps, of which the sums over lanes take a third); S = 4 in this place 495 us, and split into nine pieces 338 us
+// and 80 us more for what enters them.  Sums over channels through shared memory instead would cost 1 KB per warp and step.
 template <typename T, int L, int S, bool VEC>
 __global__ void __launch_bounds__(Geo<L, S>::NT + Geo<L, S>::NH, Geo<L, S>::BLOCKS) sel_backward_kernel(const SelArgs a)
 {
