@@ -766,8 +766,8 @@ __device__ __forceinline__ void finish_group(const NormArgs &a, const Spot &s, f
 
 // ---- one cluster per sample (and slab of groups): a.chunks blocks, which is the cluster's size
 //
-// 256 x 4096 x 64 in 8 groups, silu, bfloat16: forward 94 us (268 MB past the second reading, which the L2 cache serves),
-// backward 157 us (403 MB); about half of the issue slots busy, the rest the cluster's barriers and the memory latency at
+// 256 x 4096 x 64 in 8 groups, silu, bfloat16: forward 91 us (268 MB past the second reading, which the L2 cache serves),
+// backward 155 us (403 MB); about half of the issue slots busy, the rest the cluster's barriers and the memory latency at
 // both ends of a block's run.  Two kernels: 155 and 279 us.
 
 // Dynamic shared memory of the map kernels: the rings, then a.smem pairs (see map_smem), then what each says.
@@ -787,8 +787,10 @@ __global__ void __launch_bounds__(NT, 3) norm_cluster_forward_kernel(const NormA
             const Moments m = join(a.chunks, [&](int r) { return cluster.map_shared_rank(own, r)[g]; });
             if (threadIdx.x % 32 == 0) finish_group(a, s, s_m, g, m, s.chunk == 0);
         }
-        cluster.sync();      // nobody reads another block's moments any more; s_m is written
+        asm volatile("barrier.cluster.arrive.release;" ::: "memory");      // done with the other blocks' moments (not .aligned: lanes may be apart here)
+        __syncthreads();
     });
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");      // nobody reads this block's any more
 }
 
 template <typename T, int V, bool VEC>
@@ -810,8 +812,10 @@ __global__ void __launch_bounds__(NT, 2) norm_cluster_backward_kernel(const Norm
             for (int r = 0; r < a.chunks; ++r) t = add2(t, cluster.map_shared_rank(own, r)[g]);
             s_m[g] = mul2(t, both(inv));
         }
-        cluster.sync();
+        asm volatile("barrier.cluster.arrive.release;" ::: "memory");      // as above
+        __syncthreads();
     });
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 
 // ---- two kernels

@@ -16,10 +16,9 @@ __global__ void __launch_bounds__(256) sel_step_kernel(const SelStepArgs a, unsi
 {
     const unsigned i = (blockIdx.x * 256u + threadIdx.x) / L;
     const int l = threadIdx.x % L, n0 = 4 * l, lane = threadIdx.x % 32;
-    const unsigned tiles = a.M;
-    const unsigned b0 = i / tiles;
+    const unsigned b0 = i / (unsigned)a.M;
     const bool alive = b0 < apart;
-    const int m = (int)(i - b0 * tiles), g = m / (a.M / a.G);
+    const int m = (int)(i - b0 * (unsigned)a.M), g = m / (a.M / a.G);
     RawPack<float, 4, VEC> vh[ITEMS], va;
     RawPack<T, 4, VEC> vb[ITEMS], vc[ITEMS];
     va.load(a.A + (int64_t)m * a.N + n0, alive ? a.N - n0 : 0);
