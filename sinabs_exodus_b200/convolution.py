@@ -129,7 +129,9 @@ def causal_conv_step(state: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
         raise ValueError("'x' must be 2D, (batch, channels)")
     W = _check(x, weight, bias, activation)
     nb, M = x.shape
-    if not _seq.alike(state, (nb, W - 1, M), x.dtype, x.get_device()) or state is None:
+    if state is None:
+        raise TypeError("'state' must be a tensor, got None")
+    if not _seq.alike(state, (nb, W - 1, M), x.dtype, x.get_device()):
         _seq.require_like("state", state, (nb, W - 1, M), (x.dtype,), x.device)
     if not state.is_contiguous():
         if nb * M and _seq.channels_contiguous(state, 2) is not state:

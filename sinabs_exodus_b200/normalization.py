@@ -7,6 +7,7 @@ a ``channels_last`` feature map, or tokens ``(samples, channels)`` with one posi
 """
 from __future__ import annotations
 
+import math
 from typing import Optional
 
 import torch
@@ -82,17 +83,19 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
         raise ValueError(f"'activation' must be None, 'silu' or 'relu', got {activation!r}")
     if not eps >= 0.0:
         raise ValueError(f"'eps' must not be negative, got {eps}")
-    kind, dev = (weight if weight is not None else x if bias is None else bias).dtype, x.get_device()
+    kind, dev = getattr(weight if weight is not None else x if bias is None else bias, "dtype", None), x.get_device()
     if dev < 0 or (kind != torch.float32 and kind != x.dtype) or not (_seq.alike(weight, (C,), kind, dev) and _seq.alike(bias, (C,), kind, dev)):
         _seq.require_like("weight", weight, (C,), (torch.float32, x.dtype), x.device)
         _seq.require_like("bias", bias, (C,), (torch.float32, x.dtype), x.device)
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError(f"'weight' and 'bias' must have one type, got {weight.dtype} and {bias.dtype}")
     _seq.require_cuda("x", x)
-    positions = 1
-    for n in x.shape[1:-1]:
-        positions *= n
-    flat = x if x.ndim == 3 else x.reshape(x.shape[0], positions, C)
+    if x.ndim == 3:
+        flat = x
+    elif x.ndim == 2:
+        flat = x.unsqueeze(1)
+    else:
+        flat = x.reshape(x.shape[0], math.prod(x.shape[1:-1]), C)
     if _seq.wants_grad(x, weight, bias):
         y = GroupNormCL.apply(flat, num_groups, weight, bias, float(eps), activation)
     else:

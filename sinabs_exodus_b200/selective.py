@@ -89,6 +89,7 @@ def _grouped(name: str, t: torch.Tensor, lead: Tuple[int, ...]) -> torch.Tensor:
     if t.ndim == len(lead) + 1:
         t = t.unsqueeze(-2)
     if t.ndim != len(lead) + 2 or t.shape[:-2] != lead:
+        lead = tuple(lead)
         raise ValueError(f"'{name}' must have shape {lead + ('states',)} or {lead + ('groups', 'states')}, got {tuple(t.shape)}")
     return t
 
@@ -96,23 +97,28 @@ def _grouped(name: str, t: torch.Tensor, lead: Tuple[int, ...]) -> torch.Tensor:
 def _check(x, dt, A, B, C, D, z, dt_bias):
     """Checks what prompts and single tokens share; returns B and C with their group dimension."""
     _seq.require_data("x", x)
-    lead, M = tuple(x.shape[:-1]), x.shape[-1]
+    shape, kind, dev, f = x.shape, x.dtype, x.get_device(), torch.float32
+    lead, M = shape[:-1], shape[-1]
     B, C = _grouped("B", B, lead), _grouped("C", C, lead)
-    G, N = B.shape[-2], B.shape[-1]
+    grouped = B.shape
+    G, N = grouped[-2], grouped[-1]
     if not 1 <= N <= _lib.SELECTIVE_MAX_STATES:
         raise ValueError(f"1 to {_lib.SELECTIVE_MAX_STATES} states per channel are supported, got {N}")
     if G < 1 or M % G:
         raise ValueError(f"the {G} groups of 'B' must divide the {M} channels")
-    kind, dev, f = x.dtype, x.get_device(), torch.float32
-    if (_seq.alike(dt, x.shape, kind, dev) and _seq.alike(z, x.shape, kind, dev) and _seq.alike(B, lead + (G, N), kind, dev)
-            and _seq.alike(C, lead + (G, N), kind, dev) and _seq.alike(A, (M, N), f, dev) and _seq.alike(D, (M,), f, dev)
-            and _seq.alike(dt_bias, (M,), f, dev) and dev >= 0):
+    # the quick form of what follows
+    if (dev >= 0 and dt is not None and A is not None and _seq.alike(dt, shape, kind, dev) and B.dtype == kind and B.get_device() == dev
+            and _seq.alike(C, grouped, kind, dev) and _seq.alike(A, (M, N), f, dev) and _seq.alike(D, (M,), f, dev)
+            and _seq.alike(z, shape, kind, dev) and _seq.alike(dt_bias, (M,), f, dev)):
         return B, C
+    for name, t in (("dt", dt), ("A", A)):
+        if t is None:
+            raise TypeError(f"'{name}' must be a tensor, got None")
     same, f32 = (kind,), (f,)
-    _seq.require_like("dt", dt, x.shape, same, x.device)
-    _seq.require_like("z", z, x.shape, same, x.device)
-    _seq.require_like("B", B, lead + (G, N), same, x.device)
-    _seq.require_like("C", C, lead + (G, N), same, x.device)
+    _seq.require_like("dt", dt, shape, same, x.device)
+    _seq.require_like("z", z, shape, same, x.device)
+    _seq.require_like("B", B, grouped, same, x.device)
+    _seq.require_like("C", C, grouped, same, x.device)
     _seq.require_like("A", A, (M, N), f32, x.device)
     _seq.require_like("D", D, (M,), f32, x.device)
     _seq.require_like("dt_bias", dt_bias, (M,), f32, x.device)
@@ -168,7 +174,9 @@ def selective_step(h: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, A: torch.
     B, C = _check(x, dt, A, B, C, D, z, dt_bias)
     nb, M = x.shape
     G, N = B.shape[1], B.shape[2]
-    if not _seq.alike(h, (nb, M, N), torch.float32, x.get_device()) or h is None:
+    if h is None:
+        raise TypeError("'h' must be a tensor, got None")
+    if not _seq.alike(h, (nb, M, N), torch.float32, x.get_device()):
         _seq.require_like("h", h, (nb, M, N), (torch.float32,), x.device)
     if not h.is_contiguous():
         if nb * M and _seq.channels_contiguous(h, 2) is not h:

@@ -239,3 +239,24 @@ def test_layers_host_side():
         ex.layers.GroupNorm(2, 8)(torch.zeros(2, 9))
     with pytest.raises(ValueError, match="dimensions"):
         ex.layers.GroupNorm(2, 8)(torch.zeros(8))
+
+
+@pytest.mark.parametrize("name", ["dt", "A", "B", "C"])
+def test_what_the_scan_cannot_do_without(name):
+    with pytest.raises(TypeError, match=f"'{name}' must be a tensor"):
+        ex.selective_scan(**{**scan_args(), name: None})
+    a = {k: (v[:, 0] if v.ndim > 2 else v) for k, v in scan_args().items()}
+    with pytest.raises(TypeError, match=f"'{name}' must be a tensor"):
+        ex.selective_step(**{"h": torch.zeros(2, 8, 4), **a, name: None})
+
+
+def test_steps_need_their_state():
+    a = {k: (v[:, 0] if v.ndim > 2 else v) for k, v in scan_args().items()}
+    with pytest.raises(TypeError, match="'h' must be a tensor"):
+        ex.selective_step(None, **a)
+    with pytest.raises(TypeError, match="'state' must be a tensor"):
+        ex.causal_conv_step(None, torch.zeros(2, 8), torch.zeros(8, 4))
+    with pytest.raises(TypeError, match="'weight' must be a tensor"):
+        ex.causal_conv(torch.zeros(2, 5, 8), None)
+    with pytest.raises(TypeError, match="'weight' must be a tensor"):
+        ex.group_norm(torch.zeros(2, 8), 2, [1.0] * 8)
