@@ -4,6 +4,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -79,16 +80,32 @@ def wants_grad(*tensors: Optional[torch.Tensor]) -> bool:
     return False
 
 
+def has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether forward-mode differentiation follows one of these tensors (which says nothing in ``requires_grad``)."""
+    if getattr(forward_ad, "_current_level", 0) < 0:      # no dual_level() around this call: quicker than asking every tensor
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def refuse_tangents(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """The kernels know nothing of tangents: a call would drop them, which stands for a derivative of zero."""
+    if has_tangent(*tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative (torch.autograd.forward_ad)")
+
+
 def refuse_grad(what: str, *tensors: Optional[torch.Tensor]) -> None:
     """The in-place single-token forms are not differentiable."""
     if wants_grad(*tensors):
         raise RuntimeError(f"{what} updates its state in place and is not differentiable: call it under torch.no_grad()")
+    refuse_tangents(what, *tensors)
 
 
-def refuse_second_order(what: str) -> None:
-    """Called in a backward pass, where autograd only records with ``create_graph=True``."""
+def refuse_second_order(what: str, *upstream: Optional[torch.Tensor]) -> None:
+    """Called in a backward pass, where autograd only records with ``create_graph=True``, and where gradients from above
+    have tangents in forward-over-reverse differentiation."""
     if torch.is_grad_enabled():
         raise RuntimeError(f"{what} is differentiable once: its backward pass cannot be recorded (create_graph=True)")
+    refuse_tangents(f"the backward pass of {what}", *upstream)
 
 
 def mark_changed(t: torch.Tensor) -> None:

@@ -45,7 +45,7 @@ class CausalConvTM(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy, dlast):
-        _seq.refuse_second_order("causal_conv")
+        _seq.refuse_second_order("causal_conv", dy, dlast)
         x, weight, bias, state, lengths = ctx.saved_tensors
         nb, T, M = x.shape
         W = weight.shape[1]
@@ -89,7 +89,7 @@ def _check(x, weight, bias, activation) -> int:
 
 def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, state: Optional[torch.Tensor] = None,
                 lengths: Optional[torch.Tensor] = None, activation: Optional[str] = None) -> Tuple[torch.Tensor, torch.Tensor]:
-    """Causal convolution over a whole prompt; differentiable.
+    """Causal convolution over a whole prompt; differentiable, in reverse mode and once.
 
     Parameters
     ----------
@@ -113,6 +113,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     if lengths is not None:
         lengths = _seq.check_lengths(lengths, x.shape[0], x.shape[1], x.device)
     _seq.require_cuda("x", x)
+    _seq.refuse_tangents("causal_conv", x, weight, bias, state)
     if not _seq.wants_grad(x, weight, bias, state):
         return _forward(x, weight, bias, state, lengths, activation)[:2]
     return CausalConvTM.apply(x, weight, bias, state, lengths, activation)

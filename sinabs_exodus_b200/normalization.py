@@ -41,7 +41,7 @@ class GroupNormCL(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        _seq.refuse_second_order("group_norm")
+        _seq.refuse_second_order("group_norm", dy)
         x, weight, bias, stats = ctx.saved_tensors
         R, S, C = x.shape
         dx = x.new_empty((R, S, C))
@@ -59,7 +59,7 @@ class GroupNormCL(torch.autograd.Function):
 
 def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5, activation: Optional[str] = None) -> torch.Tensor:
-    """Group norm of a channels-last tensor; differentiable.
+    """Group norm of a channels-last tensor; differentiable, in reverse mode and once.
 
     Parameters
     ----------
@@ -90,6 +90,7 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError(f"'weight' and 'bias' must have one type, got {weight.dtype} and {bias.dtype}")
     _seq.require_cuda("x", x)
+    _seq.refuse_tangents("group_norm", x, weight, bias)
     if x.ndim == 3:
         flat = x
     elif x.ndim == 2:

@@ -56,7 +56,7 @@ class SelectiveScanTM(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy, dh_last):
-        _seq.refuse_second_order("selective_scan")
+        _seq.refuse_second_order("selective_scan", dy, dh_last)
         x, dt, A, B, C, D, z, dt_bias, lengths, ckpt = ctx.saved_tensors
         nb, T, M = x.shape
         G, N = B.shape[2:]
@@ -129,7 +129,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
                    D: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None, dt_bias: Optional[torch.Tensor] = None,
                    h0: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
                    dt_softplus: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
-    """Selective scan over a whole prompt; differentiable.
+    """Selective scan over a whole prompt; differentiable, in reverse mode and once.
 
     Parameters
     ----------
@@ -156,6 +156,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     if lengths is not None:
         lengths = _seq.check_lengths(lengths, x.shape[0], x.shape[1], x.device)
     _seq.require_cuda("x", x)
+    _seq.refuse_tangents("selective_scan", x, dt, A, B, C, D, z, dt_bias, h0)
     if _seq.wants_grad(x, dt, A, B, C, D, z, dt_bias, h0):
         return SelectiveScanTM.apply(x, dt, A, B, C, D, z, dt_bias, h0, lengths, bool(dt_softplus))
     return _forward(x, dt, A, B, C, D, z, dt_bias, h0, lengths, bool(dt_softplus), False)[:2]
