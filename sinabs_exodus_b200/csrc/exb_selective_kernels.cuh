@@ -266,6 +266,10 @@ __device__ __forceinline__ float2 exponent(float dt, float2 A2) { return fma2(bo
 // State that enters piece `seg` of channel m (S states from n0 on): what the pieces in front of it hand on by
 // themselves, each decayed through those behind it; or (REVERSE) the gradient that enters from behind.  Every block folds
 // that for itself: a launch less, and the loads of several pieces are in flight together.
+// Where states grow (positive rates or negative step sizes), the factor of a whole piece may be beyond float32 although
+// what it applies to is 0, or so small that the product is not: so 0 stays 0, and the factor is applied in two parts (the
+// second is 1 for all others).
+constexpr float ENTER_PART = 120.0f;
 template <bool REVERSE, int NP, int S>
 __device__ __forceinline__ void enter(float (&v)[S], const SelArgs &a, const Where &w, int m, int n0, const States<S> &A2)
 {
@@ -280,7 +284,10 @@ __device__ __forceinline__ void enter(float (&v)[S], const SelArgs &a, const Whe
         const Pack<float, S> own = *reinterpret_cast<const Pack<float, S> *>(a.seg_h + at * NP + n0);
         const float sum = a.seg_dt[at];
 #pragma unroll
-        for (int j = 0; j < S; ++j) v[j] = fmaf(exp2_fast(sum * rate[j]), v[j], own.v[j]);
+        for (int j = 0; j < S; ++j) {
+            const float e = sum * rate[j], part = exp2_fast(min_nan(e, ENTER_PART)) * v[j];
+            v[j] = v[j] == 0.0f ? own.v[j] : fmaf(exp2_fast(fmaxf(e - ENTER_PART, 0.0f)), part, own.v[j]);
+        }
     }
 }
 
