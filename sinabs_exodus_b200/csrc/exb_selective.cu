@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(256) sel_step_kernel(const SelStepArgs a, unsi
         Pack<float, 4> h;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            h.v[j] = fmaf(exp2_fast(d * A2[j]), vh[k].get(j), w * vb[k].get(j));
+            h.v[j] = fmaf(exp2_fast(fmaf(d, A2[j], decay_lift(d * A2[j]))), vh[k].get(j), w * vb[k].get(j));
             y[k] = fmaf(vc[k].get(j), h.v[j], y[k]);
         }
         store_pack<VEC>(h0 + k * hs, h, alive && b0 + k * apart < a.B ? a.N - n0 : 0);

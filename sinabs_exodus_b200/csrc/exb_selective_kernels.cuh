@@ -257,11 +257,15 @@ struct States {
     }
 };
 
-// Exponent of a step's decay.  ex2.approx is good to two units, but on average its result is low: by 2e-8 of its value for
-// exponents from -1 to -0.004, by 6e-9 closer to 0 (a million arguments in each octave).  A decay is applied over and over, so
-// that this, unlike its rounding, adds up: the rate gradients of a training step were off by 1.9e-6 of their norm, 0.9e-6
-// with exact exponentials.  1.4e-8, added before the exponent is rounded, lies in the middle.  The step size 0 still gives 1.
-__device__ __forceinline__ float2 exponent(float dt, float2 A2) { return fma2(both(dt), A2, both(2.0e-8f)); }
+// What to add to the exponents of a chunk's decays (see decay_lift), by those of its first step: one choice for all steps of a
+// chunk costs nothing per step, and a choice that does not fit one of them is off by 2e-8 there.
+template <int S>
+__device__ __forceinline__ void set_lift(States<S> &lift, float dt, const States<S> &A2)
+{
+#pragma unroll
+    for (int q = 0; q < S / 2; ++q) lift.q[q] = make_float2(decay_lift(dt * A2.q[q].x), decay_lift(dt * A2.q[q].y));
+}
+__device__ __forceinline__ float2 exponent(float dt, float2 A2, float2 lift) { return fma2(both(dt), A2, lift); }
 
 // State that enters piece `seg` of channel m (S states from n0 on): what the pieces in front of it hand on by
 // themselves, each decayed through those behind it; or (REVERSE) the gradient that enters from behind.  Every block folds
@@ -285,7 +289,7 @@ __device__ __forceinline__ void enter(float (&v)[S], const SelArgs &a, const Whe
         const float sum = a.seg_dt[at];
 #pragma unroll
         for (int j = 0; j < S; ++j) {
-            const float e = sum * rate[j], part = exp2_fast(min_nan(e, ENTER_PART)) * v[j];
+            const float t = sum * rate[j], e = t + decay_lift(t), part = exp2_fast(min_nan(e, ENTER_PART)) * v[j];
             v[j] = v[j] == 0.0f ? own.v[j] : fmaf(exp2_fast(fmaxf(e - ENTER_PART, 0.0f)), part, own.v[j]);
         }
     }
@@ -442,6 +446,9 @@ __global__ void __launch_bounds__(Geo<L, S>::NT + Geo<L, S>::NH, Geo<L, S>::BLOC
         const float *b = s_b + (j & 1) * K * NP + n0, *cc = s_c + (j & 1) * K * NP + n0;
         float *y = s_y + (j & 1) * K * CC;
         const int steps = blk.steps(j);
+        States<S> lift[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) set_lift(lift[k], in[pair.channel(k)].x, A2[k]);
 #pragma unroll
         for (int t0 = 0; t0 < K; t0 += GS) {
             if (t0 % SEL_CHUNK == 0) {
@@ -465,7 +472,7 @@ __global__ void __launch_bounds__(Geo<L, S>::NT + Geo<L, S>::NH, Geo<L, S>::BLOC
                     float2 s;
 #pragma unroll
                     for (int q = 0; q < S / 2; ++q) {
-                        const float2 e = exponent(d.x, A2[k].q[q]);
+                        const float2 e = exponent(d.x, A2[k].q[q], lift[k].q[q]);
                         h[k].q[q] = fma2(make_float2(exp2_fast(e.x), exp2_fast(e.y)), h[k].q[q], mul2(both(d.y), bb.q[q]));
                         s = q ? fma2(ccv.q[q], h[k].q[q], s) : mul2(ccv.q[q], h[k].q[q]);
                     }
@@ -586,6 +593,9 @@ __global__ void __launch_bounds__(Geo<L, S>::NT + Geo<L, S>::NH, Geo<L, S>::BLOC
         meet<NT + NH>();
         const float2 *in = s_in + (j & 1) * K * CC;
         const float *w = s_w + (j & 1) * K * NP + n0;
+        States<S> lift[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) set_lift(lift[k], in[pair.channel(k)].x, A2[k]);
 #pragma unroll
         for (int i = 0; i < K; ++i) {
             const int t = REVERSE ? K - 1 - i : i;
@@ -597,7 +607,7 @@ __global__ void __launch_bounds__(Geo<L, S>::NT + Geo<L, S>::NH, Geo<L, S>::BLOC
                 dt_sum[k] += d.x;
 #pragma unroll
                 for (int q = 0; q < S / 2; ++q) {
-                    const float2 e = exponent(d.x, A2[k].q[q]), f = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                    const float2 e = exponent(d.x, A2[k].q[q], lift[k].q[q]), f = make_float2(exp2_fast(e.x), exp2_fast(e.y));
                     h[k].q[q] = REVERSE ? mul2(f, fma2(ww.q[q], both(d.y), h[k].q[q])) : fma2(f, h[k].q[q], mul2(both(d.y), ww.q[q]));
                 }
             }
@@ -907,6 +917,9 @@ __global__ void __launch_bounds__(Geo<L, S>::NT + Geo<L, S>::NH, Geo<L, S>::BLOC
                 for (int i = 0; i < X::KEPT; ++i) bc_out[(t * 2 + which) * NP + (i ^ order)] = s[i];
             }
         };
+        States<S> lift[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) set_lift(lift[k], in[pair.channel(k)].x, A2[k]);
 #pragma unroll 1      // unrolled, the halves are interleaved beyond what the registers hold
         for (int half = KB / KH - 1; half >= 0; --half) {
             States<S> h[2], av[KH][2], before[KH][2];      // decays, and the states in front of the steps
@@ -927,7 +940,7 @@ __global__ void __launch_bounds__(Geo<L, S>::NT + Geo<L, S>::NH, Geo<L, S>::BLOC
                         const float2 d = in[t * CC + pair.channel(k)];
 #pragma unroll
                         for (int q = 0; q < S / 2; ++q) {
-                            const float2 e = exponent(d.x, A2[k].q[q]);
+                            const float2 e = exponent(d.x, A2[k].q[q], lift[k].q[q]);
                             h[k].q[q] = fma2(make_float2(exp2_fast(e.x), exp2_fast(e.y)), h[k].q[q], mul2(both(d.y), bb.q[q]));
                         }
                     }
@@ -952,7 +965,7 @@ __global__ void __launch_bounds__(Geo<L, S>::NT + Geo<L, S>::NH, Geo<L, S>::BLOC
                         before[i][k] = h[k];
 #pragma unroll
                         for (int q = 0; q < S / 2; ++q) {
-                            const float2 e = exponent(d.x, A2[k].q[q]);
+                            const float2 e = exponent(d.x, A2[k].q[q], lift[k].q[q]);
                             av[i][k].q[q] = make_float2(exp2_fast(e.x), exp2_fast(e.y));
                             h[k].q[q] = fma2(av[i][k].q[q], h[k].q[q], mul2(both(d.y), bb.q[q]));
                             vc[i % SC].q[q] = k ? fma2(both(pt), h[k].q[q], vc[i % SC].q[q]) : mul2(both(pt), h[k].q[q]);
