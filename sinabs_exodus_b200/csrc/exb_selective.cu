@@ -45,7 +45,7 @@ __global__ void __launch_bounds__(256) sel_step_kernel(const SelStepArgs a, unsi
     const float u = dt * x;
     float y[ITEMS], A2[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) A2[j] = va.get(j) * LOG2E;
+    for (int j = 0; j < 4; ++j) A2[j] = finite_rate(va.get(j)) * LOG2E;
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
         const int from = (lane & ~(L - 1)) + (ITEMS > 1 ? k : 0);

@@ -42,6 +42,10 @@ bool pack_aligned(const View &v)
     return !v.p || (reinterpret_cast<uintptr_t>(v.p) % (4 * sizeof(T)) == 0 && v.sb % 4 == 0 && v.st % 4 == 0);
 }
 
+// Rates are kept finite: an infinite one times the step size 0 (of a row behind the sequence, or the input's own) would not be
+// the 0 it stands for.
+__device__ __forceinline__ float finite_rate(float v) { return min_nan(max_nan(v, -2.0e38f), 2.0e38f); }
+
 // What to add to the exponent e of a decay 2^e, before it is rounded, so that ex2.approx is right on average.  A decay is
 // applied over and over: what its errors have in common adds up over a state's memory of 1 / (dt |A|) steps, what is random
 // about them does not.  By itself it is low by 1.6e-8 to 2.7e-8 of the value for e from -1 to -2^-8 and by 5e-9 to 9e-9 for

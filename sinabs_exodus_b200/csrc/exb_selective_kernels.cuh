@@ -82,13 +82,12 @@ __device__ __forceinline__ void store_states(float *p, const float (&v)[S], int 
     else store_pack<false>(p + n0, f, N - n0);
 }
 
-// Rates, kept finite: an infinite one times the step size 0 of a row behind the sequence would not be the 0 it stands for.
 template <int S>
 __device__ __forceinline__ void load_rates(float (&v)[S], const float *p, int n0, int N)
 {
     load_states(v, p, n0, N);
 #pragma unroll
-    for (int j = 0; j < S; ++j) v[j] = min_nan(max_nan(v[j], -2.0e38f), 2.0e38f);
+    for (int j = 0; j < S; ++j) v[j] = finite_rate(v[j]);
 }
 
 // Two kinds of warps.  The first NT threads of a block run the recurrence; NH more prepare its inputs and take its
