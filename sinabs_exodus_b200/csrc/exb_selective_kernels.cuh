@@ -668,13 +668,18 @@ __device__ __forceinline__ void reorder(float (&v)[S], int order)
 }
 
 constexpr int KB = SEL_CHUNK;
+// Sums over time (gradients of A, D and dt_bias) are kept in registers for so many chunks and then added to their totals in
+// shared memory: one by one, the 2048 terms of a thread that walks 16384 steps alone would drift by some 1e-5 of their sum (equal
+// terms, whose roundings all go the same way), in blocks by less than 1e-6.
+constexpr int SUM_CHUNKS = 32;
 template <int S> constexpr int in_registers = S == 4 ? KB / 2 : KB;      // steps whose decays and states are
 
 template <int L, int S>
 constexpr int backward_smem_bytes()
 {
     using Q = Geo<L, S>;
-    return (int)sizeof(float) * 2 * (KB * Q::CC * 9 + 2 * KB * Across<L, S>::COPIES * Q::NP + Q::WARPS * KB * 2 * Q::NP);
+    return (int)sizeof(float) * 2 * (KB * Q::CC * 9 + 2 * KB * Across<L, S>::COPIES * Q::NP + Q::WARPS * KB * 2 * Q::NP +
+                                     Items<KB, Q::CC, Q::NH>::V * Q::NH + S * Q::NT);
 }
 
 // Walks its piece of time backwards.  It rebuilds the states of a chunk from the chunk's checkpoint, keeping them and the
@@ -700,6 +705,7 @@ __global__ void __launch_bounds__(Geo<L, S>::NT + Geo<L, S>::NH, Geo<L, S>::BLOC
     float *s_y = s_q + 2 * KB * CC, *s_gb = s_y + 2 * KB * CC, *s_ga = s_gb + 2 * KB * CC;      // sums over the states: C h, g B, g a h A log2(e)
     float *s_b = s_ga + 2 * KB * CC, *s_c = s_b + 2 * KB * COPIES * NP;              // [2][KB][COPIES][NP]
     float *s_bc = s_c + 2 * KB * COPIES * NP;             // [2][warp][KB][B, C][NP]
+    float *s_sum = s_bc + 2 * Q::WARPS * KB * 2 * NP;     // totals over time: [2 V][preparing thread], [2 S][recurrence thread]
     const Block<KB, CC> blk(a);
     const bool gated = a.z.p != nullptr;
     const int64_t nchunks = (a.T + SEL_CHUNK - 1) / SEL_CHUNK;
@@ -715,7 +721,7 @@ __global__ void __launch_bounds__(Geo<L, S>::NT + Geo<L, S>::NH, Geo<L, S>::BLOC
         part.channel_values(skip, a.D);
         part.channel_values(bias, a.dt_bias);
 #pragma unroll
-        for (int j = 0; j < V; ++j) dD[j] = dbias[j] = 0.0f;
+        for (int j = 0; j < V; ++j) dD[j] = dbias[j] = s_sum[j * NH + tid] = s_sum[(V + j) * NH + tid] = 0.0f;
         struct Raw {
             RawPack<T, V, VEC> x[ITEMS], dt[ITEMS], z[ITEMS], dy[ITEMS];
             GroupRows<T, KB, CC, NP, NH, COPIES> b, c;
@@ -801,6 +807,14 @@ __global__ void __launch_bounds__(Geo<L, S>::NT + Geo<L, S>::NH, Geo<L, S>::BLOC
                 store_pack<VEC>(static_cast<T *>(a.ddt) + out, od, have);
                 if (gated) store_pack<VEC>(static_cast<T *>(a.dz) + out, oz, have);
             }
+            if (k % SUM_CHUNKS == 0) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    s_sum[j * NH + tid] += dD[j];
+                    s_sum[(V + j) * NH + tid] += dbias[j];
+                    dD[j] = dbias[j] = 0.0f;
+                }
+            }
         };
         fetch(raw[0], blk.count - 1);
         fetch(raw[1], blk.count - 2);
@@ -819,20 +833,13 @@ __global__ void __launch_bounds__(Geo<L, S>::NT + Geo<L, S>::NH, Geo<L, S>::BLOC
         }
         meet<NT + NH>();
         emit(0);
-        // sums of the threads that had the same columns; the recurrence is done with all of the shared memory
-        asm volatile("bar.sync 1, %0;" ::"n"(NH) : "memory");
-        float *s_d = smem;      // [thread][2 V]
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            s_d[tid * 2 * V + j] = dD[j];
-            s_d[tid * 2 * V + V + j] = dbias[j];
-        }
+        // sums of the threads that had the same columns (chunk 0, the last one, has left them all in the totals)
         asm volatile("bar.sync 1, %0;" ::"n"(NH) : "memory");
         for (int i = tid; i < 2 * CC; i += NH) {
             const int ch = i % CC, which = i / CC;
-            float s = 0.0f;
-            for (int q = ch / V; q < NH; q += COLS) s += s_d[q * 2 * V + which * V + ch % V];
-            if (blk.w.ch0 + ch < blk.per) a.part_d[((blk.w.b * a.segments + blk.w.seg) * 2 + which) * a.M + blk.w.g * blk.per + blk.w.ch0 + ch] = s;
+            double s = 0.0;
+            for (int q = ch / V; q < NH; q += COLS) s += s_sum[(which * V + ch % V) * NH + q];
+            if (blk.w.ch0 + ch < blk.per) a.part_d[((blk.w.b * a.segments + blk.w.seg) * 2 + which) * a.M + blk.w.g * blk.per + blk.w.ch0 + ch] = (float)s;
         }
         // rows behind the sequence have no gradient
         const int64_t z_lo = blk.t_end > blk.t_lo ? blk.t_end : blk.t_lo;
@@ -861,6 +868,9 @@ __global__ void __launch_bounds__(Geo<L, S>::NT + Geo<L, S>::NH, Geo<L, S>::BLOC
     const int order = X::order(cw);
     States<S> A2[2], g[2], dA[2];
     States<S> state[2];      // the chunk's checkpoint
+    float *sum_A = s_sum + 2 * Items<KB, CC, NH>::V * NH + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < 2 * S; ++i) sum_A[i * NT] = 0.0f;
     const float *ckpt[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -980,7 +990,7 @@ __global__ void __launch_bounds__(Geo<L, S>::NT + Geo<L, S>::NH, Geo<L, S>::BLOC
             }
             {      // backward
                 float sb[GS], sa[GS];
-                States<S> vb[SC], dA_c[2];      // sums of few steps first: thousands of terms one by one would lose digits
+                States<S> vb[SC], dA_c[2];      // of these steps
                 dA_c[0].fill(0.0f);
                 dA_c[1].fill(0.0f);
 #pragma unroll
@@ -1022,6 +1032,15 @@ __global__ void __launch_bounds__(Geo<L, S>::NT + Geo<L, S>::NH, Geo<L, S>::BLOC
                     for (int q = 0; q < S / 2; ++q) dA[k].q[q] = add2(dA[k].q[q], dA_c[k].q[q]);
             }
         }
+        if (j % SUM_CHUNKS == 0) {
+#pragma unroll
+            for (int i = 0; i < S; ++i) {
+                float2 *d = &dA[i / (S / 2)].q[i % (S / 2)];
+                sum_A[2 * i * NT] += d->x;
+                sum_A[(2 * i + 1) * NT] += d->y;
+                *d = both(0.0f);
+            }
+        }
     }
     meet<NT + NH>();
 #pragma unroll
@@ -1029,7 +1048,8 @@ __global__ void __launch_bounds__(Geo<L, S>::NT + Geo<L, S>::NH, Geo<L, S>::BLOC
         const int c = blk.w.ch0 + pair.channel(k), m = blk.w.g * blk.per + c;
         if (c >= blk.per) continue;
         float v[S], r[S];
-        dA[k].get(v);
+#pragma unroll
+        for (int i = 0; i < S; ++i) v[i] = sum_A[(k * S + i) * NT];
         g[k].get(r);
         reorder(v, order);
         reorder(r, order);
@@ -1047,7 +1067,11 @@ __global__ void sel_sum_bc_kernel(T *dB, T *dC, const float *part, int tiles, in
     const int64_t row = i / (2 * N);
     const int k = (int)(i % (2 * N)), which = k / N, n = k % N;
     float s = 0.0f;
-    for (int q = 0; q < tiles; ++q) s += part[((q * rows + row) * 2 + which) * NP + n];
+    for (int q0 = 0; q0 < tiles; q0 += 32) {      // in blocks, as above
+        float block = 0.0f;
+        for (int q = q0; q < min(q0 + 32, tiles); ++q) block += part[((q * rows + row) * 2 + which) * NP + n];
+        s += block;
+    }
     (which ? dC : dB)[row * N + n] = from_f32<T>(s);
 }
 
