@@ -405,6 +405,9 @@ int exb_leaky_forward_scan_static(float *out, const float *input, const float *v
  * Parameters, states and all sums are float32 unless stated otherwise.  A NULL view, or one whose data is NULL, is an
  * absent tensor.  `lengths` (NULL: T for all) holds B numbers of valid steps, clamped to 0 ... T; rows behind them do
  * not enter anything, whatever they hold: their outputs and gradients are 0 and the state passes them unchanged.
+ * A call with a size of zero (no batch item, no step, no channel) succeeds, launches nothing and WRITES NOTHING: where the
+ * other sizes leave an output with elements, its caller fills it -- h_last and dh0 are then h0 and dh_last (or zeros), last and
+ * dstate are state and dlast (or zeros), gradients of parameters are zeros.
  * Workspaces are scratch: they need not be cleared and hold nothing between calls; calls that may run at the same time
  * need one each. */
 enum { EXB_F32 = 0, EXB_BF16 = 1, EXB_F16 = 2 };

@@ -1,4 +1,7 @@
 """The sequence operators' host side where autograd or a layer's states could go wrong unseen (no GPU needed)."""
+import ctypes
+import os
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -17,6 +20,14 @@ def launched(monkeypatch):
         monkeypatch.setattr(_lib, name, lambda *a, _n=name: calls.append(_n))
     monkeypatch.setattr(_lib, "selective_checkpoint", lambda *a: torch.zeros(1))
     return calls
+
+
+@pytest.fixture(scope="module")
+def library():
+    from sinabs_exodus_b200 import build
+    if not os.path.exists(_lib.LIB_PATH):
+        build.build()
+    return _lib.load()
 
 
 SCAN = dict(x=(2, 5, 8), dt=(2, 5, 8), A=(8, 4), B=(2, 5, 2, 4), C=(2, 5, 2, 4), D=(8,), z=(2, 5, 8), dt_bias=(8,), h0=(2, 8, 4))
@@ -62,3 +73,41 @@ def test_reverse_mode_under_a_dual_level_runs(launched):
         y, _ = ex.selective_scan(**t)
         torch.autograd.grad(y, t["x"], torch.ones_like(y))
     assert launched == ["selective_forward", "selective_backward"]
+
+
+def test_empty_problems_write_nothing(library):
+    """What the header says of sizes of zero: success, and no output is touched (none of these addresses exists)."""
+    lib, p, r, null = library, ctypes.c_void_p(64), ctypes.byref(_lib.Rows(64, 64, 16)), None
+    for B, T, M in ((0, 5, 8), (2, 0, 8), (2, 5, 0)):
+        assert lib.exb_selective_forward(p, p, p, r, r, p, r, r, p, r, p, p, p, 1, p, 0, 0, B, T, M, 4, 1, 0, null) == 0
+        assert lib.exb_selective_backward(p, p, p, p, p, p, p, p, p, r, p, p, r, r, p, r, r, p, r, p, p, 1, p, 0, 0, B, T, M, 4, 1, 0, null) == 0
+        assert lib.exb_causal_conv_forward(p, p, r, p, p, p, p, 0, 1, 0, B, T, M, 4, 0, null) == 0
+        assert lib.exb_causal_conv_backward(p, p, p, p, r, p, r, p, p, p, p, 0, 1, p, 0, 0, B, T, M, 4, 0, null) == 0
+        assert lib.exb_group_norm_forward(p, p, p, r, p, p, 1e-5, 0, 1, p, 0, 0, B, T, M, 1, 0, null) == 0
+        assert lib.exb_group_norm_backward(p, p, p, r, r, p, p, p, p, 0, 1, p, 0, 0, B, T, M, 1, 0, null) == 0
+        if T:
+            assert lib.exb_selective_step(p, p, 32, r, r, p, r, r, p, r, p, 1, 0, B, M, 4, 1, 0, null) == 0
+            assert lib.exb_causal_conv_step(p, p, 24, r, p, p, 0, 1, 0, B, M, 4, 0, null) == 0
+
+
+@pytest.mark.parametrize("nb,T,M", [(0, 5, 8), (2, 0, 8), (2, 5, 0)])
+def test_the_package_fills_the_outputs_of_empty_problems(launched, nb, T, M):
+    G, N, W = 1, 4, 4
+
+    def leaf(*shape):
+        return torch.randn(*shape).requires_grad_(True)
+
+    t = dict(x=leaf(nb, T, M), dt=leaf(nb, T, M), A=leaf(M, N), B=leaf(nb, T, G, N), C=leaf(nb, T, G, N), D=leaf(M), h0=leaf(nb, M, N))
+    y, h = ex.selective_scan(**t)
+    up = torch.randn(nb, M, N)
+    g = dict(zip(t, torch.autograd.grad([y, h], list(t.values()), [torch.randn(nb, T, M), up])))
+    assert torch.equal(h, t["h0"]) and torch.equal(g["h0"], up) and all((g[k] == 0).all() for k in g if k != "h0")
+    t = dict(x=leaf(nb, T, M), weight=leaf(M, W), bias=leaf(M), state=leaf(nb, W - 1, M))
+    y, last = ex.causal_conv(**t)
+    up = torch.randn(nb, W - 1, M)
+    g = dict(zip(t, torch.autograd.grad([y, last], list(t.values()), [torch.randn(nb, T, M), up])))
+    assert torch.equal(last, t["state"]) and torch.equal(g["state"], up) and all((g[k] == 0).all() for k in g if k != "state")
+    t = dict(x=leaf(nb, T, M), weight=leaf(M), bias=leaf(M))
+    g = torch.autograd.grad(ex.group_norm(num_groups=1, **t), list(t.values()), torch.randn(nb, T, M))
+    assert all((v == 0).all() for v in g)
+    assert not launched
