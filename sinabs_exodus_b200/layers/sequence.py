@@ -116,8 +116,10 @@ class SelectiveLeak(nn.Module):
             self.conv_state, self.h = self.conv_state.detach(), self.h.detach()
 
     def _check_states(self, batch: int, like: torch.Tensor) -> None:
-        if self.h is not None and (self.h.shape[0] != batch or self.h.device != like.device or self.conv_state.dtype != like.dtype):
-            raise ValueError(f"the states are those of a batch of {self.h.shape[0]} on {self.h.device} in {self.conv_state.dtype}; "
+        if self.h is not None and (self.h.shape[0] != batch or self.h.device != like.device or self.conv_state.dtype != like.dtype
+                                   or self.h.dtype != torch.float32):
+            raise ValueError(f"the states are those of a batch of {self.h.shape[0]} on {self.h.device}, in {self.conv_state.dtype} "
+                             f"and {self.h.dtype} (here: {batch}, {like.device}, {like.dtype} and {torch.float32}); "
                              "call reset_states() before another one")
 
     def _projections(self, u: torch.Tensor):
@@ -139,9 +141,10 @@ class SelectiveLeak(nn.Module):
         if x.shape[1] == 1 and lengths is None and not torch.is_grad_enabled():
             y = self._token(signal[:, 0], gate[:, 0], weight, conv_bias, rate, skip, bias).unsqueeze(1)
         else:
-            u, self.conv_state = causal_conv(signal, weight, conv_bias, state=self.conv_state, lengths=lengths, activation="silu")
+            u, conv_state = causal_conv(signal, weight, conv_bias, state=self.conv_state, lengths=lengths, activation="silu")
             step, B, C = self._projections(u)
-            y, self.h = selective_scan(u, step, rate, B, C, D=skip, z=gate, dt_bias=bias, h0=self.h, lengths=lengths)
+            y, h = selective_scan(u, step, rate, B, C, D=skip, z=gate, dt_bias=bias, h0=self.h, lengths=lengths)
+            self.conv_state, self.h = conv_state, h      # both or, where a call fails, neither
         if self.norm is not None:
             y = self.norm(y)
         return self.out_proj(y)

@@ -111,3 +111,36 @@ def test_the_package_fills_the_outputs_of_empty_problems(launched, nb, T, M):
     g = torch.autograd.grad(ex.group_norm(num_groups=1, **t), list(t.values()), torch.randn(nb, T, M))
     assert all((v == 0).all() for v in g)
     assert not launched
+
+
+def test_states_of_another_type_are_refused_before_anything_changes(launched):
+    """``half()`` also converts the states that a layer holds; the scan's are float32."""
+    layer = ex.layers.SelectiveLeak(8, num_states=4)
+    x = torch.randn(2, 3, 8)
+    with torch.no_grad():
+        layer(x)
+        layer.half()
+        before = layer.conv_state, layer.h
+        for steps in (3, 1):
+            with pytest.raises(ValueError, match="reset_states"):
+                layer(x[:, :steps].half())
+            assert layer.conv_state is before[0] and layer.h is before[1]
+        layer.reset_states()
+        layer(x.half())
+        assert layer.h.dtype == torch.float32 and layer.conv_state.dtype == torch.float16
+
+
+def test_a_call_that_fails_leaves_both_states(launched, monkeypatch):
+    layer = ex.layers.SelectiveLeak(8, num_states=4)
+    x = torch.randn(2, 3, 8)
+    with torch.no_grad():
+        layer(x)
+        before = layer.conv_state, layer.h
+
+        def out_of_memory(*a):
+            raise torch.cuda.OutOfMemoryError("no room")
+
+        monkeypatch.setattr(_lib, "selective_forward", out_of_memory)
+        with pytest.raises(torch.cuda.OutOfMemoryError):
+            layer(x)
+    assert layer.conv_state is before[0] and layer.h is before[1]
