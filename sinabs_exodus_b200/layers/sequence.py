@@ -41,7 +41,7 @@ class GroupNorm(nn.GroupNorm):
             return group_norm(x.reshape(-1, x.shape[-1]), *args).reshape(x.shape)
         if x.ndim in (4, 5):
             self._check_channels(x.shape[-3], x)
-            maps = x.reshape(-1, *x.shape[-3:]).permute(0, 2, 3, 1)
+            maps = x.reshape(math.prod(x.shape[:-3]), *x.shape[-3:]).permute(0, 2, 3, 1)      # maps may be empty: not -1
             return group_norm(maps, *args).permute(0, 3, 1, 2).reshape(x.shape)
         raise ValueError(f"GroupNorm takes 2 to 5 dimensions, got {tuple(x.shape)}")
 

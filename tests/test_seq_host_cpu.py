@@ -144,3 +144,18 @@ def test_a_call_that_fails_leaves_both_states(launched, monkeypatch):
         with pytest.raises(torch.cuda.OutOfMemoryError):
             layer(x)
     assert layer.conv_state is before[0] and layer.h is before[1]
+
+
+@pytest.mark.parametrize("shape", [(2, 8, 0, 4), (2, 8, 3, 0), (0, 8, 3, 4), (2, 0, 8, 3, 4), (2, 3, 8, 0, 4), (2, 0, 8), (0, 8)])
+@pytest.mark.parametrize("channels_last", [False, True])
+def test_norm_layer_on_empty_maps(launched, shape, channels_last):
+    layer = ex.layers.GroupNorm(2, 8)
+    x = torch.zeros(shape)
+    if channels_last and len(shape) == 4:
+        x = x.to(memory_format=torch.channels_last)
+    x.requires_grad_(True)
+    y = layer(x)
+    assert y.shape == shape and y.dtype == x.dtype
+    y.sum().backward()
+    assert x.grad.shape == shape and (layer.weight.grad == 0).all()
+    assert not launched
