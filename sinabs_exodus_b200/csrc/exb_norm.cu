@@ -451,14 +451,14 @@ struct Walk {
             r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w;
         }
     }
-    // f(pack of x, pack of dy) for every position; peek(pack of x) sees the first of them before.
+    // f(pack of x, pack of dy) for the positions q ... end; peek(pack of x) sees the first of all before.
     template <typename F, typename Peek>
-    __device__ __forceinline__ void run(const F &f, const Peek &peek)
+    __device__ __forceinline__ void some(int q, int end, const F &f, const Peek &peek)
     {
         R cx, cg;
         if constexpr (VEC) {
 #pragma unroll 4
-            for (int q = 0; q < count; ++q) {
+            for (; q < end; ++q) {
                 asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
                 const uint4 *from = ring + (q % AHEAD) * NT;
                 take(cx, from);
@@ -467,9 +467,8 @@ struct Walk {
                 issue();
                 f(cx, cg);
             }
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
         } else {
-            for (int q = 0; q < count; ++q) {
+            for (; q < end; ++q) {
                 cx.load(x, left);
                 if (TWO) cg.load(g, left);
                 if (q == 0) peek(cx);
@@ -479,10 +478,25 @@ struct Walk {
             }
         }
     }
+    // All positions.
     template <typename F>
     __device__ __forceinline__ void run(const F &f)
     {
-        run(f, [](const R &) {});
+        some(0, count, f, [](const R &) {});
+        if (VEC) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+    // All positions; after the first `stop` of them settle(stop) is called, which returns the number to stop at next.
+    template <typename F, typename Peek, typename Settle>
+    __device__ __forceinline__ void run(const F &f, const Peek &peek, int stop, const Settle &settle)
+    {
+        int q = 0;
+        while (stop < count) {
+            some(q, stop, f, peek);
+            q = stop;
+            stop = settle(q);
+        }
+        some(q, count, f, peek);
+        if (VEC) asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
 };
 template <typename T, int V, bool VEC>
@@ -493,8 +507,10 @@ __device__ __forceinline__ float2 pair_of(const RawPack<T, V, VEC> &r, int i)
 }
 
 // Moments of every group over the block's positions, in s_m (see map_smem), passed to out(group of the block, moments).
-// A thread takes the moments of its channels about their first value, so that a large common offset costs no digits; where
-// whole packs belong to one group, it joins those of a pack.
+// A thread takes the moments of its channels about their first value, so that a large common offset costs no digits, and moves
+// them to their mean after 8, 64, 512, ... positions: where the first value lies far off, it would cost the digits of all that
+// follow (a first value of 1e4 among 2048 of deviation 1: 1e-3 of the variance).  Where whole packs belong to one group, it
+// joins those of a pack.
 template <typename T, int V, bool VEC, typename Out>
 __device__ __forceinline__ void block_moments(const NormArgs &a, const Spot &s, float2 *s_m, uint4 *ring, const Out &out)
 {
@@ -520,6 +536,17 @@ __device__ __forceinline__ void block_moments(const NormArgs &a, const Spot &s, 
                 const float2 f = pair_of(x, i);
                 k[i] = make_float2(-f.x, -f.y);
             }
+        }, 8, [&](int n) {
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                const float2 mean = mul2(sum[i], both(1.0f / n)), from = k[i];
+                k[i] = add2(from, make_float2(-mean.x, -mean.y));
+                const float2 moved = add2(from, make_float2(-k[i].x, -k[i].y));      // the mean but for the rounding of k
+                sq[i] = fma2(make_float2(-mean.x, -mean.y), sum[i], sq[i]);
+                sq[i] = make_float2(max_nan(sq[i].x, 0.0f), max_nan(sq[i].y, 0.0f));
+                sum[i] = fma2(both(-(float)n), moved, sum[i]);
+            }
+            return n < 1 << 27 ? 8 * n : 0x7fffffff;
         });
         const float n = (float)s.count, inv = s.count > 0 ? 1.0f / n : 0.0f;
         float mean[V], m2[V];

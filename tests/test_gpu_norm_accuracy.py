@@ -29,3 +29,16 @@ def test_tokens_with_a_very_large_offset(R, C, G):
     n = ref.norm(x.double(), G)
     want = n * w.double() + b.double()
     ref.assert_close(ex.group_norm(x, G, w, b), want, 38 * 2.0 ** -24 * 64 * (1 + n.abs()) * (w.double().abs() + 1) , F32, "y")
+
+
+@pytest.mark.parametrize("R,S", [(40, 8192), (1, 262144)])      # clusters of blocks, and two kernels: 1024 positions per thread
+def test_maps_whose_first_values_lie_far_off(R, S):
+    """Every thread begins on a value of 1e4 and has a thousand of deviation 1 behind it.  About the means of the first 8, 64 and
+    512 of its values, the sums of their squares round like sums of 64 equal terms."""
+    import sinabs_exodus_b200 as ex
+    x, w, b, _ = problem(3, R, S, 1024, F32, mean=0.0, std=1.0)
+    x[:, ::1024] = 1e4
+    y = ex.group_norm(x, 4, w, b)
+    for r in range(0, R, 13):
+        n = ref.norm(x[r:r + 1].double(), 4)
+        ref.assert_close(y[r:r + 1], n * w.double() + b.double(), 120 * 2.0 ** -24 * (1 + n.abs()) * (w.double().abs() + 1), F32, "y")
