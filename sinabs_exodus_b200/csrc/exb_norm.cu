@@ -271,6 +271,11 @@ __global__ void __launch_bounds__(NT, K * V <= 8 ? 4 : 1) norm_token_forward_ker
     }
 }
 
+// Sums over samples and positions are kept in registers for so many of them (rounds: one or two samples each) and then added to
+// their totals in memory: thousands of equal terms (as the gradient of a mean has) one by one would drift by 1e-5 of their
+// sum, because each addition rounds the same way.
+constexpr int SUM_ROUNDS = 64, SUM_POSITIONS = 64;
+
 template <typename T, int V, int L, int K, bool VEC>
 __global__ void __launch_bounds__(NT, K * V <= 8 ? 2 : 1) norm_token_backward_kernel(const NormArgs a, int64_t strides)
 {
@@ -306,7 +311,26 @@ __global__ void __launch_bounds__(NT, K * V <= 8 ? 2 : 1) norm_token_backward_ke
     };
 #pragma unroll
     for (int q = 0; q < ROWS; ++q) fetch(q, q < mine);
+    // adds the sums to the lane group's row of a.part, which only it touches, or starts the row with them
+    auto settle = [&](bool add) {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+#pragma unroll
+                for (int h = 0; h < (V > 1 ? 2 : 1); ++h) {
+                    const int c = u.channel(k) + 2 * i + h;
+                    if (!u.alive || c >= u.per) continue;
+                    float *to = a.part + u.first * 2 * a.C + u.g * u.per + c;
+                    const float w_sum = h ? dw[k][i].y : dw[k][i].x, b_sum = h ? db[k][i].y : db[k][i].x;
+                    to[0] = add ? to[0] + w_sum : w_sum;
+                    to[a.C] = add ? to[a.C] + b_sum : b_sum;
+                }
+                dw[k][i] = db[k][i] = both(0.0f);
+            }
+    };
     for (int j = 0; j < rounds; ++j) {
+        if (j > 0 && j % SUM_ROUNDS == 0) settle(j > SUM_ROUNDS);
         float2 n[ROWS][K][P], e[ROWS][K][P];
         float u1[ROWS], u2[ROWS], rstd[ROWS];
 #pragma unroll
@@ -354,18 +378,7 @@ __global__ void __launch_bounds__(NT, K * V <= 8 ? 2 : 1) norm_token_backward_ke
             out += step_out;
         }
     }
-    if (!u.alive) return;
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int i = 0; i < P; ++i)
-#pragma unroll
-            for (int h = 0; h < (V > 1 ? 2 : 1); ++h) {
-                const int c = u.channel(k) + 2 * i + h;
-                if (c >= u.per) continue;
-                a.part[(u.first * 2 + 0) * a.C + u.g * u.per + c] = h ? dw[k][i].y : dw[k][i].x;
-                a.part[(u.first * 2 + 1) * a.C + u.g * u.per + c] = h ? db[k][i].y : db[k][i].x;
-            }
+    settle(rounds > SUM_ROUNDS);
 }
 
 // ---------------------------------------------------------------------------------------------- maps
@@ -701,6 +714,28 @@ __device__ __forceinline__ void block_gradient_sums(const NormArgs &a, const Spo
         float2 s1[P], s2[P];
 #pragma unroll
         for (int i = 0; i < P; ++i) s1[i] = s2[i] = both(0.0f);
+        float2 *own = s_m + s.ty * s.chans + p * V;
+        auto put = [&]() {
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                if (2 * i < left) own[2 * i] = make_float2(s1[i].x, s2[i].x);
+                if (V > 1 && 2 * i + 1 < left) own[2 * i + 1] = make_float2(s1[i].y, s2[i].y);
+            }
+        };
+        auto settle = [&](int q) {
+            if (q > SUM_POSITIONS) {
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    const float2 x = 2 * i < left ? own[2 * i] : both(0.0f), y = V > 1 && 2 * i + 1 < left ? own[2 * i + 1] : both(0.0f);
+                    s1[i] = add2(s1[i], make_float2(x.x, y.x));
+                    s2[i] = add2(s2[i], make_float2(x.y, y.y));
+                }
+            }
+            put();
+#pragma unroll
+            for (int i = 0; i < P; ++i) s1[i] = s2[i] = both(0.0f);
+            return q + SUM_POSITIONS;
+        };
         walk.run([&](const RawPack<T, V, VEC> &x, const RawPack<T, V, VEC> &g) {
             float2 n[P], d[P];
             h.get(n, d, x, g, a.act);
@@ -709,13 +744,9 @@ __device__ __forceinline__ void block_gradient_sums(const NormArgs &a, const Spo
                 s1[i] = add2(s1[i], d[i]);
                 s2[i] = fma2(d[i], n[i], s2[i]);
             }
-        });
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-            float2 *to = s_m + s.ty * s.chans + p * V + 2 * i;
-            if (2 * i < left) to[0] = make_float2(s1[i].x, s2[i].x);
-            if (V > 1 && 2 * i + 1 < left) to[1] = make_float2(s1[i].y, s2[i].y);
-        }
+        }, [](const RawPack<T, V, VEC> &) {}, SUM_POSITIONS, settle);
+        if (s.count > SUM_POSITIONS) settle(s.count);
+        else put();
     }
     __syncthreads();
     float *out = a.part + (s.r * a.chunks + s.chunk) * 2 * a.C + s.c0;

@@ -5,7 +5,8 @@ import math
 import pytest
 import torch
 
-from tests.test_gpu_selective import DEV, F32
+from tests import _seq_ref as ref
+from tests.test_gpu_selective import DEV
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +36,24 @@ def test_scan(nb, M, N):
     for name, got, want, roundings in (("dA", dA, nb * sum_A, 104 + 20), ("dD", dD, nb * T * x, 104), ("ddt_bias", dbias, nb * sum_dt, 104 + 80)):
         off = float((got.double() / want - 1).abs().max())
         assert off <= roundings * 2.0 ** -24, (name, off)
+
+
+# tokens: 1351 samples for each group of lanes; maps in clusters of blocks and in two kernels: 1024 positions for each thread
+@pytest.mark.parametrize("R,S,C,G,up,roundings", [(50000, 1, 8192, 128, 0.9, 147), (40, 8192, 1024, 4, 0.7, 88), (1, 262144, 1024, 4, 0.7, 88)])
+def test_norm(R, S, C, G, up, roundings):
+    """The upstream gradient of a mean: every term of the bias's gradient is the same.  It passes through sums of 64 positions (128
+    samples) and of their 16 (11) totals, and a few more; the last sums are in float64."""
+    import sinabs_exodus_b200 as ex
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn(R, S, C, generator=g, device=DEV)
+    w, b = torch.ones(C, device=DEV, requires_grad=True), torch.zeros(C, device=DEV, requires_grad=True)
+    dy = torch.full_like(x, up)
+    dw, db = torch.autograd.grad(ex.group_norm(x, G, w, b), [w, b], dy)
+    want = R * S * float(dy.flatten()[0])
+    assert float((db.double() / want - 1).abs().max()) <= roundings * 2.0 ** -24
+    # the weight's: the norm itself, summed; its terms' absolute sum is below the number of terms
+    total = torch.zeros(C, device=DEV, dtype=torch.float64)
+    for r in range(0, R, max(1, (1 << 27) // (S * C))):
+        n = ref.norm(x[r:r + max(1, (1 << 27) // (S * C))].double(), G)
+        total += n.sum((0, 1))
+    assert float((dw.double() - up * total).abs().max()) <= (roundings + 50) * 2.0 ** -24 * R * S * up
