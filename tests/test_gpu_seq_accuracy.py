@@ -2,7 +2,9 @@
 import pytest
 import torch
 
-from tests.test_gpu_selective import DEV, F32, check, problem, run
+from tests import _seq_ref as ref
+from tests._seq_err import scan_bounds
+from tests.test_gpu_selective import DEV, F16, F32, check, problem, run
 
 pytestmark = pytest.mark.gpu
 
@@ -101,3 +103,19 @@ def test_slow_decays_token_by_token(nb, M, N, fed):
     for t in range(STEPS):
         ex.selective_step(h, A=p["A"], dt_softplus=False, **{k: p[k][:, t] for k in ("x", "dt", "B", "C")})
     relative(h, slow_exact(p), not fed)
+
+
+# batch, time, channels, states, groups: split over time and whole, states in every number of lanes, long beyond any memory
+@pytest.mark.parametrize("size", [(1, 1500, 40, 16, 2), (100, 1500, 8, 4, 1), (2, 1100, 24, 64, 1), (1, 2100, 128, 8, 4), (100, 1100, 8, 128, 1),
+                                  (4, 1300, 600, 32, 1)])
+@pytest.mark.parametrize("kind", [F32, F16])
+def test_long_sequences(size, kind):
+    p, dy, dh = problem(5, *size, kind)
+    got = run(p, dy, dh)
+    del p["lengths"]
+    want, _, _, kinds = ref.scan(**p, dy=dy, dh=dh)
+    bound = scan_bounds(**p, dy=dy, dh=dh)
+    for k, v in got.items():
+        if k in ("dB", "dC"):
+            want[k], bound[k] = want[k].view(v.shape), bound[k].view(v.shape)
+        ref.assert_close(v, want[k], bound[k], kinds.get(k, F32), k)
