@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from tests import _seq_ref as ref
-from tests.test_gpu_selective import F32, problem
+from tests.test_gpu_selective import DEV, F32, problem
 
 pytestmark = pytest.mark.gpu
 
@@ -29,3 +29,65 @@ def test_infinite_rates_in_a_step(nb, M, N):
     ref.assert_close(h, want, 30 * 2.0 ** -24 * size, F32, "h")
     ref.assert_close(y, raw * gate, 40 * 2.0 ** -24 * ((size * C.abs()).sum(-1) + (p["D"].double() * x).abs()) * (gate.abs() + 0.1), F32, "y")
     torch.testing.assert_close(h, last, rtol=1e-6, atol=1e-6)
+
+
+def test_backward_twice():
+    """A kept graph gives the same gradients again: nothing that it saved is used up."""
+    import sinabs_exodus_b200 as ex
+    g = torch.Generator(device=DEV).manual_seed(2)
+
+    def leaf(*shape, scale=1.0):
+        return (torch.randn(*shape, generator=g, device=DEV) * scale).requires_grad_(True)
+
+    scan = dict(x=leaf(2, 300, 24), dt=leaf(2, 300, 24), A=(-torch.rand(24, 8, generator=g, device=DEV)).requires_grad_(True), B=leaf(2, 300, 1, 8),
+                C=leaf(2, 300, 1, 8), h0=leaf(2, 24, 8))
+    conv = dict(x=leaf(2, 70, 24), weight=leaf(24, 4), bias=leaf(24), state=leaf(2, 3, 24))
+    norm = dict(x=leaf(3, 50, 24), weight=leaf(24), bias=leaf(24))
+    for y, t in ((ex.selective_scan(**scan)[0], scan), (ex.causal_conv(**conv, activation="silu")[0], conv),
+                 (ex.group_norm(num_groups=4, activation="silu", **norm), norm)):
+        up = torch.randn(y.shape, generator=g, device=DEV)
+        first = torch.autograd.grad(y, list(t.values()), up, retain_graph=True)
+        for a, b in zip(first, torch.autograd.grad(y, list(t.values()), up)):
+            assert torch.equal(a, b)
+
+
+def test_prompts_and_tokens_in_and_out_of_inference_mode():
+    import sinabs_exodus_b200 as ex
+    torch.manual_seed(0)
+    layer = ex.layers.SelectiveLeak(24, num_states=8).to(DEV)
+    x = torch.randn(2, 9, 24, device=DEV)
+    with torch.no_grad():
+        want = torch.cat([layer(x[:, :6])] + [layer(x[:, t:t + 1]) for t in range(6, 9)], 1)
+    for modes in ((torch.no_grad, torch.inference_mode), (torch.inference_mode, torch.no_grad)):
+        layer.reset_states()
+        parts = []
+        with modes[0]():
+            parts.append(layer(x[:, :6]))
+        for t in range(6, 9):
+            with modes[t % 2]():
+                parts.append(layer(x[:, t:t + 1]))
+        assert torch.equal(torch.cat(parts, 1), want)
+
+
+def test_truncated_training_in_a_graph():
+    """``GraphedStep`` with carried states, trained: chunk after chunk, as eager steps with ``zero_grad`` between them."""
+    import sinabs_exodus_b200 as ex
+    torch.manual_seed(0)
+    layer = ex.layers.SelectiveLeak(24, num_states=8, norm_groups=2).to(DEV)
+    x, g = torch.randn(4, 2, 40, 24, device=DEV), torch.randn(4, 2, 40, 24, device=DEV)
+    want = []
+    for c in range(4):
+        layer.zero_grad()
+        y = layer(x[c])
+        y.backward(g[c])
+        want.append((y.detach(), {k: p.grad.clone() for k, p in layer.named_parameters()}))
+    del y
+    layer.reset_states()
+    step = ex.GraphedStep(layer, x[0], g[0], carry_state=True)
+    for name in ("h", "conv_state"):
+        getattr(layer, name).zero_()
+    for c in range(4):
+        out = step(x[c], g[c])
+        torch.testing.assert_close(out, want[c][0], rtol=1e-5, atol=1e-6)
+        for k, p in layer.named_parameters():
+            torch.testing.assert_close(p.grad, want[c][1][k], rtol=1e-4, atol=1e-5)

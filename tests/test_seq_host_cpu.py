@@ -159,3 +159,17 @@ def test_norm_layer_on_empty_maps(launched, shape, channels_last):
     y.sum().backward()
     assert x.grad.shape == shape and (layer.weight.grad == 0).all()
     assert not launched
+
+
+@pytest.mark.parametrize("name", list(CALLS))
+def test_function_transforms_are_refused(monkeypatch, name):
+    """``torch.func`` hands in tensors without memory of their own."""
+    monkeypatch.setattr(_seq, "require_cuda", lambda name, x: None)
+    call, shapes = CALLS[name]
+    t = {k: torch.zeros(*s) for k, s in shapes.items()}
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda x: call(dict(t, x=x)))(torch.zeros(3, *shapes["x"]))
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.grad(lambda x: call(dict(t, x=x)).sum())(t["x"])
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(lambda x: call(dict(t, x=x)), (t["x"],), (t["x"],))
