@@ -831,7 +831,7 @@ __device__ __forceinline__ void finish_group(const NormArgs &a, const Spot &s, f
 
 // ---- one cluster per sample (and slab of groups): a.chunks blocks, which is the cluster's size
 //
-// 256 x 4096 x 64 in 8 groups, silu, bfloat16: forward 91 us (268 MB past the second reading, which the L2 cache serves),
+// 256 x 4096 x 64 in 8 groups, silu, bfloat16: forward 93 us (268 MB past the second reading, which the L2 cache serves),
 // backward 155 us (403 MB); about half of the issue slots busy, the rest the cluster's barriers and the memory latency at
 // both ends of a block's run.  Two kernels: 155 and 279 us.
 

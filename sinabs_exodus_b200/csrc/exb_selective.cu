@@ -9,7 +9,7 @@ namespace {
 
 // A thread takes four states of a channel in ITEMS batch items, `apart` of them between two: the rates are loaded once, and
 // all states are on their way together (the state is what has to move).  The channel's first ITEMS lanes do the work that is
-// not per state for one batch item each.  256 x 4096 x 16, bfloat16: 32 us, 4.4 TB/s of states and inputs (with one batch
+// not per state for one batch item each.  256 x 4096 x 16, bfloat16: 32.7 us, 4.4 TB/s of states and inputs (with one batch
 // item per thread, and all lanes doing that work, 55 us); 1 x 1024 x 16: 2 us, the launch.
 template <typename T, int L, int ITEMS, bool VEC>
 __global__ void __launch_bounds__(256) sel_step_kernel(const SelStepArgs a, unsigned apart)
@@ -146,15 +146,16 @@ SelPlan sel_plan(int64_t B, int64_t T, int M, int N, int G, bool backward)
     p.tiles = (int)ceil_div(M / G, p.CC);
     const int64_t blocks = B * G * p.tiles, unit = 16;
     // Splitting the time axis costs a pass over the states of all pieces (half of the forward pass, a quarter of the
-    // backward one), so it has to bring more than 1.5 times the blocks, for two on each of 148 SMs.  At 128 blocks
-    // (4 x 2048 x 2048 x 16, training) whole and in nine pieces take the same; at 16 (1 x 16384 x 1024 x 16) 9, 18, 27 and
-    // 37 pieces take 282, 221, 236 and 226 us.  A piece is no shorter than 32 steps and than the number of pieces that its
-    // block has to fold.
+    // backward one), so it has to bring more than 1.5 times the blocks, for two on each of 148 SMs.  1 x 4096 steps of 64
+    // channels x 16 states per block, prompt and training, whole against split: 64 blocks 311 and 1206 us against 231 and
+    // 755; 96 blocks 311 and 1209 against 311 and 1005; 112 blocks 310 and 1211 against 392 and 1409.  At 16 blocks
+    // (1 x 16384 x 1024 x 16, prompt) 9, 18, 27 and 37 pieces take 282, 221, 236 and 226 us.  A piece is no shorter than 32
+    // steps and than the number of pieces that its block has to fold.
     int64_t want = blocks >= 96 ? 1 : 296 / blocks;
     while (want > 1 && (T / want < 32 || T / want < want)) --want;
     p.seg = ceil_div(ceil_div(T, want), unit) * unit;
     p.segments = (int)ceil_div(T, p.seg);
-    // One block per SM: two states per lane and twice the warps (training step above: 605 us against 699).  More blocks than
+    // One block per SM: two states per lane and twice the warps (4 x 2048 x 2048 x 16, training: 622 us against 699).  More blocks than
     // SMs: four, and two blocks on an SM (288 blocks: 212 us against 277).
     p.S = (blocks * p.segments > 148 || p.NP > 64) ? 4 : 2;
     p.L = p.NP / p.S;

@@ -316,8 +316,8 @@ constexpr int forward_smem_bytes()
     return (int)sizeof(float) * 2 * (Q::KF * Q::CC * 5 + 2 * Q::KF * Q::NP);
 }
 
-// Measured (N = 16, bfloat16, gated): 1 x 16384 x 1024 in 18 pieces 125 us, half of the issue slots busy, the rest barrier
-// and fixed latencies; 4 x 2048 x 2048 whole, with checkpoints, 169 us on 128 of the 148 SMs (S = 2; with S = 4 one
+// Measured (N = 16, bfloat16, gated): 1 x 16384 x 1024 in 18 pieces 128 us, half of the issue slots busy, the rest barrier
+// and fixed latencies; 4 x 2048 x 2048 whole, with checkpoints, 160 us on 128 of the 148 SMs (S = 2; with S = 4 one
 // recurrence warp per scheduler, 182 us).  Exponentials: 58 us of either.
 template <typename T, int L, int S, bool VEC>
 __global__ void __launch_bounds__(Geo<L, S>::NT + Geo<L, S>::NH, Geo<L, S>::BLOCKS) sel_forward_kernel(const SelArgs a)
@@ -504,7 +504,7 @@ constexpr int state_smem_bytes()
 }
 
 // What a piece of time hands on when nothing enters it, and its sum of step sizes: the state behind its last step, or
-// (REVERSE) the gradient that goes to the step in front of its first one.  1 x 16384 x 1024 x 16 in 18 pieces: 88 us.
+// (REVERSE) the gradient that goes to the step in front of its first one.  1 x 16384 x 1024 x 16 in 18 pieces: 92 us.
 template <typename T, int L, int S, bool VEC, bool REVERSE>
 __global__ void __launch_bounds__(Geo<L, S>::NT + Geo<L, S>::NH, Geo<L, S>::BLOCKS) sel_state_kernel(const SelArgs a)
 {
@@ -687,9 +687,9 @@ constexpr int backward_smem_bytes()
 // With four states to a lane it does so by halves of a chunk, the later one first, for which the earlier one is run through
 // once more: a quarter more exponentials, and registers for two blocks on an SM, whose barriers then do not stop all of it.
 // The launch gives every thread 128 registers, of which the preparing warps hand 40 to those of the recurrence.
-// Measured (N = 16, bfloat16, gated): 4 x 2048 x 2048 whole 424 us, issue slots 63 % busy (about 106 instructions per 128
-// element-steps, of which the sums over lanes take a third); S = 4 in this place 495 us, and split into nine pieces 338 us
-// and 80 us more for what enters them.  Sums over channels through shared memory instead would cost 1 KB per warp and step.
+// Measured (N = 16, bfloat16, gated): 4 x 2048 x 2048 whole 445 us, issue slots 61 % busy, a third of the
+// recurrence's instructions for the sums over lanes.  Before the decays' correction, whole 424 us, S = 4 in this place 495, and
+// split into nine pieces 338 us and 80 more for what enters them.  Sums over channels through shared memory instead would cost 1 KB per warp and step.
 template <typename T, int L, int S, bool VEC>
 __global__ void __launch_bounds__(Geo<L, S>::NT + Geo<L, S>::NH, Geo<L, S>::BLOCKS) sel_backward_kernel(const SelArgs a)
 {
