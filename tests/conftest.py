@@ -18,3 +18,16 @@ def _built_checker():
     from oracle import build as oracle_build
 
     oracle_build.build_oracle()
+
+
+@pytest.fixture(autouse=True)
+def _queues_by_value(request, monkeypatch):
+    """Results of worker processes that end right after they have put them."""
+    if request.module.__name__.split(".")[-1] == "test_dist_cpu":
+        import copy
+
+        import torch.multiprocessing as mp
+
+        from tests import _by_value
+        get_context = mp.get_context
+        monkeypatch.setattr(mp, "get_context", lambda method=None: _by_value.context_with(copy.copy(get_context(method))))
