@@ -195,6 +195,7 @@ __global__ void __launch_bounds__(TX * TY, W <= 4 ? 3 : 1) conv_backward_kernel(
         using Ring = Rows<T, V, VEC>;
         Ring ring(reinterpret_cast<char *>(s_raw));
         float2 row[STEP + W - 1][V / 2], d[STEP + W - 1][V / 2];      // entry j: step t - (W - 1) + j
+        const int64_t own_end = s.t1 < s.len ? s.t1 : s.len;
         const int64_t end = s.t1 + W - 1;      // rows t - (W - 1) in [t0 (or the state's), t1) come out
         const T *x = static_cast<const T *>(a.x.p) + s.b * a.x.sb + s.m, *dy = static_cast<const T *>(a.dy.p) + s.b * a.dy.sb + s.m;
         auto there = [&](int64_t t) { return t < s.len && t < end; };
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(TX * TY, W <= 4 ? 3 : 1) conv_backward_kernel(
 #pragma unroll
             for (int j = 0; j < STEP; ++j) {
                 const int64_t now = t + j, r = now - (W - 1);
-                const bool counts = now < s.t1;
+                const bool counts = now < own_end;
                 Pack<T, V> g;
 #pragma unroll
                 for (int i = 0; i < V / 2; ++i) {
@@ -254,10 +255,11 @@ __global__ void __launch_bounds__(TX * TY, W <= 4 ? 3 : 1) conv_backward_kernel(
                         e = now < s.len ? mul2(e, slope) : both(0.0f);
                     }
                     d[W - 1 + j][i] = e;
-                    const float2 own = counts ? e : both(0.0f);
+                    if (counts) {      // not e = 0: the rows may hold infinities, which belong to others' sums or to none
 #pragma unroll
-                    for (int k = 0; k < W; ++k) dw[k][i] = fma2(own, row[j + k][i], dw[k][i]);
-                    dw[W][i] = add2(dw[W][i], own);
+                        for (int k = 0; k < W; ++k) dw[k][i] = fma2(e, row[j + k][i], dw[k][i]);
+                        dw[W][i] = add2(dw[W][i], e);
+                    }
                     float2 v = mul2(f.w[0][i], d[W - 1 + j][i]);
 #pragma unroll
                     for (int k = 1; k < W; ++k) v = fma2(f.w[k][i], d[W - 1 + j - k][i], v);

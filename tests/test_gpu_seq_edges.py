@@ -91,3 +91,19 @@ def test_truncated_training_in_a_graph():
         torch.testing.assert_close(out, want[c][0], rtol=1e-5, atol=1e-6)
         for k, p in layer.named_parameters():
             torch.testing.assert_close(p.grad, want[c][1][k], rtol=1e-4, atol=1e-5)
+
+
+@pytest.mark.parametrize("kind", [F32, torch.bfloat16])
+@pytest.mark.parametrize("M", [8, 7])      # packs of channels, and single ones
+def test_an_infinity_reaches_only_the_taps_that_meet_it(kind, M):
+    """The last row meets the current tap alone: the gradients of the others stay finite, and the infinite one is not NaN.  One in
+    the middle, next to the end of a thread's run, meets all of them."""
+    import sinabs_exodus_b200 as ex
+    x = torch.ones(2, 70, M, device=DEV).to(kind)
+    x[0, 69, 2] = x[1, 15, 3] = x[1, 16, 4] = float("inf")
+    w = torch.ones(M, 4, device=DEV, requires_grad=True)
+    y, _ = ex.causal_conv(x, w, lengths=torch.tensor([70, 60], device=DEV))
+    dw, = torch.autograd.grad(y, w, torch.ones_like(y))
+    want = torch.tensor([67.0 + 57, 68 + 58, 69 + 59, 70 + 60], device=DEV).repeat(M, 1)      # rows that each tap meets
+    want[2, 3] = want[3] = want[4] = float("inf")
+    assert torch.equal(dw, want)
