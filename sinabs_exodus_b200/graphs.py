@@ -86,6 +86,7 @@ class GraphedStep:
                     fixed = buf.detach().clone()
                     m.register_buffer(name, fixed)
                     self._fixed_state.append((m, name, fixed))
+                    buf = None      # the last one, too: its graph must not live while the step is captured
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
             out = self._step()
@@ -111,6 +112,7 @@ class GraphedStep:
                 for name, buf in list(m.named_buffers(recurse=False)):
                     if buf.requires_grad or buf.grad_fn is not None:
                         m.register_buffer(name, buf.detach())
+                    buf = None
         if not self.training_step:
             with torch.no_grad():
                 return self.module(self.static_input)

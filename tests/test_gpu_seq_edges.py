@@ -107,3 +107,24 @@ def test_an_infinity_reaches_only_the_taps_that_meet_it(kind, M):
     want = torch.tensor([67.0 + 57, 68 + 58, 69 + 59, 70 + 60], device=DEV).repeat(M, 1)      # rows that each tap meets
     want[2, 3] = want[3] = want[4] = float("inf")
     assert torch.equal(dw, want)
+
+
+def test_no_graph_of_the_warm_up_lives_while_a_step_is_captured(monkeypatch):
+    """The leaves' accumulators of an older graph belong to another stream than the one that captures."""
+    import weakref
+
+    import sinabs_exodus_b200 as ex
+    torch.manual_seed(0)
+    layer = ex.layers.SelectiveLeak(24, num_states=8).to(DEV)
+    states, alive = [], []
+    layer.register_forward_hook(lambda module, args, out: states.extend(weakref.ref(t) for t in (module.h, module.conv_state)))
+    capture = torch.cuda.graph
+
+    def watched(graph):
+        alive.append(sum(r() is not None for r in states))
+        return capture(graph)
+
+    monkeypatch.setattr(torch.cuda, "graph", watched)
+    x, g = torch.randn(2, 40, 24, device=DEV), torch.randn(2, 40, 24, device=DEV)
+    ex.GraphedStep(layer, x, g, carry_state=True)
+    assert alive == [0] and len(states) == 8
